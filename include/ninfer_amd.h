@@ -87,6 +87,39 @@ typedef struct nmi_cyclic_kv_layer_view {
     int32_t quant_group;
 } nmi_cyclic_kv_layer_view;
 
+/* EXTENSION: K/V of many sequences in pages of a pool. k/v are I8 or BF16 [D, page_size, Hkv, pages],
+ * k_scale/v_scale (I8) FP16 [D/64, page_size, Hkv, pages]; a page is contiguous, nb[3] may be any multiple
+ * of 16 bytes from a page's size up (a pool that several layers share). page_table I32 [max_pages, B]: row r
+ * of sequence b lies in row r % page_size of page page_table[r / page_size, b]; nb[1] may be larger than
+ * max_pages entries. An entry outside [0, pages) is an absent page: nothing is written to it or seen in it.
+ * page_size is a power of two from 16 to 4096, head_dim 128 or 256, B at most 1024. */
+typedef struct nmi_paged_kv_layer_view {
+    nmi_tensor k;
+    nmi_tensor v;
+    nmi_tensor k_scale;
+    nmi_tensor v_scale;
+    nmi_tensor page_table;
+    int32_t page_size;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int32_t dtype; /* NMI_I8 (INT8-G64) or NMI_BF16 */
+    int32_t quant_group;
+} nmi_paged_kv_layer_view;
+
+/* EXTENSION: what a paged attention call is sized for: most new tokens of a sequence, and most rows of a
+ * sequence, its new ones included. */
+typedef struct nmi_paged_envelope {
+    uint32_t max_new_tokens;
+    uint32_t max_visible_keys;
+} nmi_paged_envelope;
+
+/* EXTENSION: a token at position p sees the rows j <= p with p - j < size or j < sinks; size 0 (and no
+ * sinks): every row j <= p. */
+typedef struct nmi_attention_window {
+    uint32_t size;
+    uint32_t sinks;
+} nmi_attention_window;
+
 /* include/ninfer/ops/gqa_attention.h:13-16 */
 typedef struct nmi_gqa_envelope {
     uint32_t min_visible_keys;
@@ -208,6 +241,43 @@ int nmi_gqa_attention_tree(const nmi_tensor* q, const nmi_tensor* k, const nmi_t
                            const nmi_kv_layer_view* cache, nmi_gqa_envelope envelope,
                            int32_t write_cache, void* workspace, size_t workspace_bytes,
                            nmi_tensor* out, nmi_stream_t stream);
+
+/* ---------------------------------------------------------------- paged cache (EXTENSION) */
+
+/* The new tokens of all sequences are packed: sequence b has the tokens starts[b] .. starts[b+1]-1
+ * (starts I32 [B+1], not decreasing; a sequence may have none), the first of them at position history[b]
+ * (I32 [B]). Tokens outside [starts[0], starts[B]) belong to no sequence: their rows of `out`, k_out and
+ * v_out are left as they were. Packed tensors are [D, heads, N] with contiguous heads of a token and any
+ * token stride nb[2] that is a multiple of 16 bytes (slices of a fused projection); data is 16-byte aligned. */
+
+/* Writes token i of sequence b to row history[b] + i: codes and scales as nmi_gqa_kv_append (I8), or the
+ * values (BF16). k/v BF16 [D, Hkv, N]. A row past the page table or in an absent page is dropped. Two
+ * sequences that share the page of a new row race on it. */
+int nmi_paged_kv_append(const nmi_tensor* k, const nmi_tensor* v, const nmi_tensor* starts,
+                        const nmi_tensor* history, const nmi_paged_kv_layer_view* cache,
+                        nmi_stream_t stream);
+
+/* Reads rows back as values: token starts[b] + i of k_out/v_out (BF16 or FP32 [D, Hkv, N]) becomes row
+ * first[b] + i of sequence b, FP32(code) * FP32(scale) rounded once to the output's type (I8) or the stored value
+ * (BF16). Rows past the page table or in absent pages read as zero. */
+int nmi_paged_kv_read(const nmi_paged_kv_layer_view* cache, const nmi_tensor* starts,
+                      const nmi_tensor* first, nmi_tensor* k_out, nmi_tensor* v_out,
+                      nmi_stream_t stream);
+
+/* Attention of the new tokens over their sequences' rows, which hold the new rows already
+ * (nmi_paged_kv_append): token i of sequence b stands at p = history[b] + i,
+ * out = sum_j softmax_j(scale * q . K_j) V_j over the rows it sees (nmi_attention_window), zero where it
+ * sees none. q/out BF16 [D, Hq, N], Hq a multiple of Hkv; scale positive. Sequences of one token, chunks of
+ * prompts and both in one batch are served alike. A sequence whose device scalars lie outside the envelope
+ * (more new tokens or rows, a negative history, tokens past N) is left out: its rows of `out` stay as they were.
+ * Pages of rows that no new token sees may be absent. Workspace from the query, for the same arguments. */
+size_t nmi_paged_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                           int32_t tokens, int32_t batch, nmi_paged_envelope envelope,
+                                           nmi_attention_window window);
+int nmi_paged_attention(const nmi_tensor* q, const nmi_tensor* starts, const nmi_tensor* history,
+                        float scale, nmi_attention_window window, const nmi_paged_kv_layer_view* cache,
+                        nmi_paged_envelope envelope, void* workspace, size_t workspace_bytes,
+                        nmi_tensor* out, nmi_stream_t stream);
 
 /* ---------------------------------------------------------------- acceptance (part b) */
 

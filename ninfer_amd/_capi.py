@@ -105,6 +105,31 @@ class CyclicKVLayerView(C.Structure):
     ]
 
 
+class PagedKVLayerView(C.Structure):
+    """nmi_paged_kv_layer_view."""
+
+    _fields_ = [
+        ("k", Tensor),
+        ("v", Tensor),
+        ("k_scale", Tensor),
+        ("v_scale", Tensor),
+        ("page_table", Tensor),
+        ("page_size", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("dtype", C.c_int32),
+        ("quant_group", C.c_int32),
+    ]
+
+
+class PagedEnvelope(C.Structure):
+    _fields_ = [("max_new_tokens", C.c_uint32), ("max_visible_keys", C.c_uint32)]
+
+
+class AttentionWindow(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("sinks", C.c_uint32)]
+
+
 class GqaEnvelope(C.Structure):
     _fields_ = [("min_visible_keys", C.c_uint32), ("max_visible_keys", C.c_uint32)]
 
@@ -148,6 +173,12 @@ _SIGNATURES = {
     "nmi_gqa_kv_append": (C.c_int, [_T, _T, _T, P(KVLayerView), _STREAM]),
     "nmi_gqa_attention_cached": (C.c_int, [_T, _T, C.c_float, P(KVLayerView), GqaEnvelope, C.c_void_p, C.c_size_t, _T, _STREAM]),
     "nmi_gqa_attention_tree": (C.c_int, [_T, _T, _T, _T, _T, C.c_float, P(KVLayerView), GqaEnvelope, C.c_int32, C.c_void_p, C.c_size_t, _T, _STREAM]),
+    "nmi_paged_kv_append": (C.c_int, [_T, _T, _T, _T, P(PagedKVLayerView), _STREAM]),
+    "nmi_paged_kv_read": (C.c_int, [P(PagedKVLayerView), _T, _T, _T, _T, _STREAM]),
+    "nmi_paged_attention_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, PagedEnvelope,
+                                                         AttentionWindow]),
+    "nmi_paged_attention": (C.c_int, [_T, _T, _T, C.c_float, AttentionWindow, P(PagedKVLayerView), PagedEnvelope, C.c_void_p,
+                                      C.c_size_t, _T, _STREAM]),
     "nmi_argmax": (C.c_int, [_T, _T, C.c_int32, _STREAM]),
     "nmi_sampling_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
     "nmi_speculative_prepare_verify_inputs": (C.c_int, [_T, _T, _T, _T, _T, _STREAM]),

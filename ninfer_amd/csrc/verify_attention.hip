@@ -34,6 +34,7 @@
 #include "attn_math.h"
 #include "common.h"
 #include "device_utils.h"
+#include "kv_codec.h"
 #include "ops_internal.h"
 
 #include <algorithm>
@@ -2397,32 +2398,11 @@ __global__ __launch_bounds__(256) void kv_quant_append_rows_kernel(const uint16_
     if (u >= units) { return; } // units is a multiple of 8: whole groups stay together
     const i4 raw = *reinterpret_cast<const i4*>((blockIdx.y ? v : k) + static_cast<int64_t>(u) * 8);
     const AppendUnit a = append_unit(u, D / 8, col0, positions, count, cb, T, Hkv, P);
-    float x[8];
-    float amax = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const uint32_t w = static_cast<uint32_t>(raw[e >> 1]);
-        x[e] = bf16_to_f32(static_cast<uint16_t>((e & 1) ? w >> 16 : w & 0xffffu));
-        amax = fmaxf(amax, fabsf(x[e]));
-    }
-    amax = fmaxf(amax, dpp_from<0xB1, 0xf>(amax, 0.0f));  // lane ^ 1
-    amax = fmaxf(amax, dpp_from<0x4E, 0xf>(amax, 0.0f));  // lane ^ 2
-    amax = fmaxf(amax, dpp_from<0x141, 0xf>(amax, 0.0f)); // the other four of the eight
-    const uint16_t sbits = f32_to_f16_bits(amax > 0.0f ? amax / 127.0f : 0.0f);
-    const float s = f16_bits_to_f32(sbits);
-    const float inv = s > 0.0f ? 1.0f / s : 0.0f;
-    uint32_t code[2] = {0u, 0u};
-    if (inv != 0.0f) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float rr = rintf(x[e] * inv);
-            rr = fminf(127.0f, fmaxf(-127.0f, rr));
-            code[e >> 2] |= (static_cast<uint32_t>(static_cast<int8_t>(rr)) & 0xffu) << (8 * (e & 3));
-        }
-    }
+    uint16_t sbits;
+    const i2 code = quantize_g64(raw, sbits);
     if (a.row < 0) { return; }
     int8_t* cdst = (blockIdx.y ? vc : kc) + static_cast<int64_t>(a.b) * code_seq + static_cast<int64_t>(D) * (a.row + static_cast<int64_t>(P) * a.h);
-    *reinterpret_cast<i2*>(cdst + 8 * a.piece) = i2{static_cast<int>(code[0]), static_cast<int>(code[1])};
+    *reinterpret_cast<i2*>(cdst + 8 * a.piece) = code;
     if ((a.piece & 7) == 0) {
         uint16_t* sdst = (blockIdx.y ? vs : ks) + static_cast<int64_t>(a.b) * scale_seq + static_cast<int64_t>(D / 64) * (a.row + static_cast<int64_t>(P) * a.h);
         sdst[a.piece >> 3] = sbits;

@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _capi
-from ._capi import CommitEnvelope, GqaEnvelope, Tensor, check, lib
+from ._capi import AttentionWindow, CommitEnvelope, GqaEnvelope, PagedEnvelope, Tensor, check, lib
 
 
 def _s(stream):
@@ -76,6 +76,35 @@ def gqa_attention_tree(q, k, v, positions, parents, scale, cache, envelope, writ
     check(lib().nmi_gqa_attention_tree(_p(q), _p(k), _p(v), _p(positions), _p(parents), float(scale),
                                        C.byref(cache), GqaEnvelope(*envelope), int(bool(write_cache)),
                                        ws, nb, _p(out), _s(stream)))
+
+
+# ---- paged cache (extension) -------------------------------------------------------------------
+#
+# Packed tokens: sequence b has tokens starts[b] .. starts[b + 1] - 1, the first at position history[b]
+# (both I32 on the device). `cache` is a PagedKVLayerView (ninfer_amd.kv_cache.PagedKVCacheLayer.view()).
+
+def paged_kv_append(k, v, starts, history, cache, stream=None) -> None:
+    """Token i of sequence b to row history[b] + i of its pages (INT8-G64 quantised, or BF16 copied)."""
+    check(lib().nmi_paged_kv_append(_p(k), _p(v), _p(starts), _p(history), C.byref(cache), _s(stream)))
+
+
+def paged_kv_read(cache, starts, first, k_out, v_out, stream=None) -> None:
+    """Row first[b] + i of sequence b to token starts[b] + i of k_out/v_out (BF16 or FP32 values)."""
+    check(lib().nmi_paged_kv_read(C.byref(cache), _p(starts), _p(first), _p(k_out), _p(v_out), _s(stream)))
+
+
+def paged_attention_workspace_bytes(q_heads: int, kv_heads: int, head_dim: int, tokens: int, batch: int, envelope,
+                                    window=(0, 0)) -> int:
+    return int(lib().nmi_paged_attention_workspace_bytes(q_heads, kv_heads, head_dim, tokens, batch, PagedEnvelope(*envelope),
+                                                         AttentionWindow(*window)))
+
+
+def paged_attention(q, starts, history, scale, window, cache, envelope, workspace, out, stream=None) -> None:
+    """Causal attention of the packed tokens over their pages, new rows included. `window` (size, sinks): the last
+    `size` rows and the first `sinks` ones, (0, 0) for every row. `envelope`: (most new tokens, most rows) of a sequence."""
+    ws, nb = _ws(workspace)
+    check(lib().nmi_paged_attention(_p(q), _p(starts), _p(history), float(scale), AttentionWindow(*window), C.byref(cache),
+                                    PagedEnvelope(*envelope), ws, nb, _p(out), _s(stream)))
 
 
 # ---- acceptance (argmax.h, sampling.h, speculative_round.h) ------------------------------------
