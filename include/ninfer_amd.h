@@ -267,7 +267,7 @@ int nmi_paged_kv_read(const nmi_paged_kv_layer_view* cache, const nmi_tensor* st
 /* Attention of the new tokens over their sequences' rows, which hold the new rows already
  * (nmi_paged_kv_append): token i of sequence b stands at p = history[b] + i,
  * out = sum_j softmax_j(scale * q . K_j) V_j over the rows it sees (nmi_attention_window), zero where it
- * sees none. q/out BF16 [D, Hq, N], Hq a multiple of Hkv; scale positive. Sequences of one token, chunks of
+ * sees none. q/out BF16 [D, Hq, N], Hq a multiple of Hkv; scale from 2^-40 to 2^40. Sequences of one token, chunks of
  * prompts and both in one batch are served alike. A sequence whose device scalars lie outside the envelope
  * (more new tokens or rows, a negative history, tokens past N) is left out: its rows of `out` stay as they were.
  * Pages of rows that no new token sees may be absent. Workspace from the query, for the same arguments. */

@@ -187,7 +187,7 @@ int nmi_paged_attention(const nmi_tensor* q, const nmi_tensor* starts, const nmi
         a.out = validate_packed(out, NMI_BF16, c.D, a.Hq, n, op, "out");
         a.starts = validate_index(starts, c.B + 1, op, "starts");
         a.history = validate_index(history, c.B, op, "history");
-        require(std::isfinite(scale) && scale > 0.0f, op, "scale must be positive and finite");
+        require(scale >= 0x1p-40f && scale <= 0x1p40f, op, "scale must be positive, from 2^-40 to 2^40");
         a.scale = scale;
         validate_envelope(envelope, window, op);
         require(static_cast<int64_t>(envelope.max_visible_keys) <= (static_cast<int64_t>(c.max_pages) << c.page_shift), op,

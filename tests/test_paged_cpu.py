@@ -115,10 +115,10 @@ Q = T(na.BF16, 128, 8, 5)
     (dict(q=T(na.FP32, 128, 8, 5)), ValueError), (dict(q=T(na.BF16, 128, 7, 5)), ValueError), (dict(q=T(na.BF16, 256, 8, 5)), ValueError),
     (dict(q=None), ValueError), (dict(out=None), ValueError), (dict(out=T(na.FP32, 128, 8, 5)), ValueError),
     (dict(out=T(na.BF16, 128, 8, 4)), ValueError), (dict(out=T(na.BF16, 128, 8, 5, nb={2: 2056})), ValueError),
-    (dict(scale=0.0), ValueError), (dict(scale=-1.0), ValueError), (dict(scale=float("nan")), ValueError), (dict(scale=float("inf")), ValueError),
+    (dict(scale=0.0), ValueError), (dict(scale=-1.0), ValueError), (dict(scale=float("nan")), ValueError), (dict(scale=float("inf")), ValueError), (dict(scale=2.0**-41), ValueError), (dict(scale=2.0**41), ValueError),
     (dict(envelope=(0, 32)), ValueError), (dict(envelope=(33, 32)), ValueError), (dict(envelope=(5, 65)), ValueError),
     (dict(envelope=(5, 1 << 31)), OverflowError), (dict(window=(1 << 31, 0)), OverflowError), (dict(window=(0, 4)), ValueError),
-    (dict(ws=Ws(ptr=FAKE + 16)), ValueError),
+    (dict(ws=Ws(nbytes=0)), ValueError), (dict(ws=Ws(ptr=FAKE + 16)), ValueError), (dict(ws=None), ValueError),
 ])
 def test_attention_arguments(kw, error):
     a = dict(q=Q, out=T(na.BF16, 128, 8, 5), scale=0.1, envelope=(5, 64), window=(0, 0), ws=Ws())
@@ -133,6 +133,7 @@ def test_attention_arguments(kw, error):
 
 def test_workspace_query():
     q = ops.paged_attention_workspace_bytes
+    assert q(40, 8, 128, 1, 1, (1, 65536)) > 0
     # what the op refuses needs none
     for bad in [(40, 7, 128, 1, 1, (1, 64)), (0, 8, 128, 1, 1, (1, 64)), (40, 8, 64, 1, 1, (1, 64)), (40, 8, 128, 0, 1, (1, 64)),
                 (40, 8, 128, 1, 0, (1, 64)), (40, 8, 128, 1, 1025, (1, 64)), (40, 8, 128, 1, 1, (0, 64)), (40, 8, 128, 1, 1, (65, 64)),
