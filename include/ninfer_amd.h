@@ -270,7 +270,8 @@ int nmi_paged_kv_read(const nmi_paged_kv_layer_view* cache, const nmi_tensor* st
  * sees none. q/out BF16 [D, Hq, N], Hq a multiple of Hkv; scale from 2^-40 to 2^40. Sequences of one token, chunks of
  * prompts and both in one batch are served alike. A sequence whose device scalars lie outside the envelope
  * (more new tokens or rows, a negative history, tokens past N) is left out: its rows of `out` stay as they were.
- * Pages of rows that no new token sees may be absent. Workspace from the query, for the same arguments. */
+ * Pages of rows that no new token sees may be absent. max_visible_keys is at most 2^23 and the rows of the page table,
+ * N * Hq at most 2^30. Workspace from the query, for the same arguments. */
 size_t nmi_paged_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                            int32_t tokens, int32_t batch, nmi_paged_envelope envelope,
                                            nmi_attention_window window);

@@ -164,7 +164,8 @@ size_t nmi_paged_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, in
     // 0 for what the op itself refuses
     if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads != 0 || (head_dim != 128 && head_dim != 256) || tokens <= 0 || batch <= 0 ||
         batch > kPagedMaxBatch || envelope.max_new_tokens == 0 || envelope.max_new_tokens > envelope.max_visible_keys ||
-        envelope.max_visible_keys > top || window.size > top || window.sinks > top) {
+        envelope.max_visible_keys > static_cast<uint32_t>(kPagedMaxKeys) || window.size > top || window.sinks > top ||
+        static_cast<int64_t>(tokens) * q_heads > (int64_t{1} << 30)) {
         return 0;
     }
     return paged_attention_bytes(q_heads, kv_heads, head_dim, tokens, batch, static_cast<int32_t>(envelope.max_new_tokens),
@@ -192,6 +193,10 @@ int nmi_paged_attention(const nmi_tensor* q, const nmi_tensor* starts, const nmi
         validate_envelope(envelope, window, op);
         require(static_cast<int64_t>(envelope.max_visible_keys) <= (static_cast<int64_t>(c.max_pages) << c.page_shift), op,
                 "the execution envelope exceeds the page table");
+        if (envelope.max_visible_keys > static_cast<uint32_t>(kPagedMaxKeys)) {
+            throw Unsupported(op + ": more than 2^23 rows of a sequence are not built");
+        }
+        if (static_cast<int64_t>(n) * a.Hq > (int64_t{1} << 30)) { throw Unsupported(op + ": more than 2^30 query rows in one call are not built"); }
         a.max_new = static_cast<int32_t>(envelope.max_new_tokens);
         a.max_keys = static_cast<int32_t>(envelope.max_visible_keys);
         a.window = static_cast<int32_t>(window.size);

@@ -37,6 +37,9 @@ struct PagedAttnArgs {
     float* part_o;     // FP32 O [partial row][D] and (log2-domain maximum, sum) [partial row][2]
     float* part_ml;
     int32_t* seq_table; // per sequence: first slot, splits
+    int32_t nsplit;     // key splits of a many-row workgroup's rows, and their parts as above
+    float* many_o;
+    float* many_ml;
 };
 
 // Sequence b's tokens and history, checked against the call's bounds: a sequence outside them takes no part.
@@ -55,7 +58,7 @@ __device__ __forceinline__ Seq sequence(const PagedAttnArgs& x, int b) {
     return s;
 }
 
-// The 32-key tiles that tokens at positions p0 .. p1 need: [0, sink) and [first, end) of the sequence's tiles,
+// The tiles (of 2^lg keys) that tokens at positions p0 .. p1 need: [0, sink) and [first, end) of the sequence's tiles,
 // numbered on without the gap.
 struct Tiles {
     int32_t sink;
@@ -64,12 +67,35 @@ struct Tiles {
     __device__ __forceinline__ int32_t tile(int32_t i) const { return i < sink ? i : i - sink + first; }
 };
 
-__device__ __forceinline__ Tiles tiles_of(const PagedAttnArgs& x, int32_t p0, int32_t p1) {
-    const int32_t first = x.a.window > 0 ? max(0, p0 + 1 - x.a.window) : 0;
-    Tiles t{(min(x.a.sinks, first) + 31) >> 5, first >> 5, 0};
+__device__ __forceinline__ Tiles tiles_of(const PagedAttnArgs& x, int32_t p0, int32_t p1, int lg) {
+    const int32_t first = max(0, p0 + 1 - x.a.window);
+    Tiles t{(min(x.a.sinks, first) + (1 << lg) - 1) >> lg, first >> lg, 0};
     if (t.sink >= t.first) { t.sink = t.first = 0; }
-    t.count = t.sink + ((p1 + 32) >> 5) - t.first;
+    t.count = t.sink + (p1 >> lg) + 1 - t.first;
     return t;
+}
+
+// The weights of two parts of a row, log2-domain maxima and sums M, L and m, l, in their merge. A part that saw nothing
+// weighs nothing, one whose sum is NaN stays NaN.
+struct Weights {
+    float M, a, b;
+};
+
+__device__ __forceinline__ Weights weights(float M, float L, float m, float l) {
+    Weights w;
+    w.M = fmaxf(M, m);
+    w.a = M == -INFINITY ? (L == L ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(M - w.M);
+    w.b = m == -INFINITY ? (l == l ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m - w.M);
+    return w;
+}
+
+// Four outputs O / L as BF16, zero where the sum is.
+__device__ __forceinline__ u2 out_pair(f4 O, float L) {
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { y[e] = f32_to_bf16_bits(L == 0.0f ? 0.0f : O[e] * inv); }
+    return u2{y[0] | (y[1] << 16), y[2] | (y[3] << 16)};
 }
 
 // ---- one wave: 16 NT query rows against 32 keys straight from the cache -------------------------
@@ -235,15 +261,15 @@ __device__ __forceinline__ void init_rows(const PagedAttnArgs& x, const Seq& s, 
     }
 }
 
-// Whether a token at `pos` sees row `key` (of an existing page).
-__device__ __forceinline__ bool sees(const PagedAttnArgs& x, int pos, int key) {
-    return key <= pos && (x.a.window == 0 || pos - key < x.a.window || key < x.a.sinks);
+// Whether a token at `pos` sees row `key` of page `page`: no row of an absent page (negative), nor from pos -1.
+__device__ __forceinline__ bool sees(const PagedAttnArgs& x, int pos, int key, int page) {
+    return (key <= (pos | (page >> 31))) & ((pos - key < x.a.window) | (key < x.a.sinks));
 }
 
 // Whether every row of the wave sees all 32 keys of the tile.
 __device__ __forceinline__ bool all_seen(const PagedAttnArgs& x, int lo, int hi, int tile, Halves hv) {
     const int k0 = 32 * tile, k1 = k0 + 31;
-    return hv.page[0] >= 0 && hv.page[1] >= 0 && k1 <= lo && (x.a.window == 0 || hi - k0 < x.a.window || k1 < x.a.sinks);
+    return (hv.page[0] | hv.page[1]) >= 0 && k1 <= lo && (hi - k0 < x.a.window || k1 < x.a.sinks);
 }
 
 // An infinite or NaN BF16 in either half of a word: that half's sign bit (of the result) set.
@@ -292,7 +318,7 @@ __device__ __forceinline__ void attend_chunk(const PagedAttnArgs& x, int tile, H
             seen[nt] = 0u;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const bool ok = hv.page[i >> 2] >= 0 && sees(x, s.pos[nt], 32 * tile + 16 * (i >> 2) + 4 * g + (i & 3));
+                const bool ok = sees(x, s.pos[nt], 32 * tile + 16 * (i >> 2) + 4 * g + (i & 3), hv.page[i >> 2]);
                 seen[nt] |= ok ? 1u << i : 0u;
                 sv[nt][i] = ok ? sv[nt][i] : -INFINITY;
             }
@@ -300,7 +326,7 @@ __device__ __forceinline__ void attend_chunk(const PagedAttnArgs& x, int tile, H
         // keys that no row of the wave may see: whatever their rows hold is taken out
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bool dead = hv.page[i >> 2] < 0 || 32 * tile + 16 * (i >> 2) + 4 * g + (i & 3) > s.hi;
+            const bool dead = 32 * tile + 16 * (i >> 2) + 4 * g + (i & 3) > (s.hi | (hv.page[i >> 2] >> 31));
             if constexpr (BF) {
 #pragma unroll
                 for (int w = 0; w < CK::VP; ++w) {
@@ -478,7 +504,7 @@ constexpr int kUnit = 4; // tiles of a split's unit: one for each wave
 __device__ __forceinline__ int few_units(const PagedAttnArgs& x, int b, Seq& s, Tiles& t) {
     s = sequence(x, b);
     if (s.tokens == 0 || s.tokens * x.G > x.few_rows) { return 0; }
-    t = tiles_of(x, s.history, s.history + s.tokens - 1);
+    t = tiles_of(x, s.history, s.history + s.tokens - 1, 5);
     return (t.count + kUnit - 1) / kUnit;
 }
 
@@ -565,7 +591,7 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
     const FewWork w = few_work(x, blockIdx.x / x.c.Hkv, lane);
     if (w.b < 0) { return; }
     const Seq s = sequence(x, w.b);
-    const Tiles tiles = tiles_of(x, s.history, s.history + s.tokens - 1);
+    const Tiles tiles = tiles_of(x, s.history, s.history + s.tokens - 1, 5);
     const int per = (w.units + w.splits - 1) / w.splits * kUnit; // tiles of a split
     const int t0 = min(w.split * per, tiles.count), t1 = min(t0 + per, tiles.count);
     const int each = (t1 - t0 + kFewWaves - 1) / kFewWaves;
@@ -633,18 +659,16 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const float2 o = xm[wave][nt * 64 + lane];
-                const float Mx = fmaxf(M[nt], o.x);
-                const float a = M[nt] == -INFINITY ? (L[nt] == L[nt] ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(M[nt] - Mx);
-                const float b = o.x == -INFINITY ? (o.y == o.y ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(o.x - Mx);
-                L[nt] = L[nt] * a + o.y * b;
-                M[nt] = Mx;
+                const Weights q = weights(M[nt], L[nt], o.x, o.y);
+                L[nt] = L[nt] * q.a + o.y * q.b;
+                M[nt] = q.M;
 #pragma unroll
                 for (int t = 0; t < D / 16; ++t) {
                     const f4 y = xo[wave][(nt * (D / 16) + t) * 64 + lane];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         // a part without weight adds nothing, whatever it holds
-                        r.O[nt][t][e] = (a == 0.0f ? 0.0f : r.O[nt][t][e] * a) + (b == 0.0f ? 0.0f : y[e] * b);
+                        r.O[nt][t][e] = (q.a == 0.0f ? 0.0f : r.O[nt][t][e] * q.a) + (q.b == 0.0f ? 0.0f : y[e] * q.b);
                     }
                 }
             }
@@ -675,20 +699,17 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
             if (g == 0) { *reinterpret_cast<float2*>(x.part_ml + 2 * at) = float2{M[nt], L[nt]}; }
         } else {
             const int t = row / x.G;
-            const float inv = L[nt] == 0.0f ? 0.0f : 1.0f / L[nt];
             uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + (s.start + t) * x.a.out.token_stride) + (h * x.G + row - t * x.G) * D;
 #pragma unroll
             for (int i = 0; i < D / (16 * RUN); ++i) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    uint32_t y[RUN / 2];
+                    uint16_t* dst = out + out_dim<BF>(RUN * i, 4 * g + e);
 #pragma unroll
-                    for (int q = 0; q < RUN / 2; ++q) {
-                        const float o0 = L[nt] == 0.0f ? 0.0f : r.O[nt][RUN * i + 2 * q][e] * inv;
-                        const float o1 = L[nt] == 0.0f ? 0.0f : r.O[nt][RUN * i + 2 * q + 1][e] * inv;
-                        y[q] = static_cast<uint32_t>(f32_to_bf16_bits(o0)) | (static_cast<uint32_t>(f32_to_bf16_bits(o1)) << 16);
+                    for (int q = 0; q < RUN; q += 4) {
+                        const f4 o = {r.O[nt][RUN * i + q][e], r.O[nt][RUN * i + q + 1][e], r.O[nt][RUN * i + q + 2][e], r.O[nt][RUN * i + q + 3][e]};
+                        *reinterpret_cast<u2*>(dst + q) = out_pair(o, L[nt]);
                     }
-                    __builtin_memcpy(__builtin_assume_aligned(out + out_dim<BF>(RUN * i, 4 * g + e), RUN * 2), y, sizeof(y));
                 }
             }
         }
@@ -713,13 +734,11 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs x, 
     float M = -INFINITY, L = 0.0f;
     f4 O = {0.f, 0.f, 0.f, 0.f};
     const auto add = [&](float m, float l, f4 o) {
-        const float Mx = fmaxf(M, m);
-        const float a = M == -INFINITY ? (L == L ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(M - Mx);
-        const float q = m == -INFINITY ? (l == l ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m - Mx);
-        L = L * a + l * q;
+        const Weights w = weights(M, L, m, l);
+        L = L * w.a + l * w.b;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { O[e] = (a == 0.0f ? 0.0f : O[e] * a) + (q == 0.0f ? 0.0f : o[e] * q); }
-        M = Mx;
+        for (int e = 0; e < 4; ++e) { O[e] = (w.a == 0.0f ? 0.0f : O[e] * w.a) + (w.b == 0.0f ? 0.0f : o[e] * w.b); }
+        M = w.M;
     };
 #pragma unroll 4
     for (int k = grp; k < splits; k += GRP) {
@@ -734,110 +753,577 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs x, 
 #pragma unroll
     for (int k = 1; k < GRP; ++k) { add(xm[k].x, xm[k].y, xo[k][threadIdx.x]); }
     const int t = row / x.G;
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + (s.start + t) * x.a.out.token_stride) + (h * x.G + row - t * x.G) * D + d;
-    uint32_t y[2];
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const float o0 = L == 0.0f ? 0.0f : O[2 * q] * inv;
-        const float o1 = L == 0.0f ? 0.0f : O[2 * q + 1] * inv;
-        y[q] = static_cast<uint32_t>(f32_to_bf16_bits(o0)) | (static_cast<uint32_t>(f32_to_bf16_bits(o1)) << 16);
-    }
-    *reinterpret_cast<u2*>(out) = u2{y[0], y[1]};
+    *reinterpret_cast<u2*>(out) = out_pair(O, L);
 }
 
-// One workgroup per (token, query head).
+// ---- many rows: tiles of query rows over key tiles that a workgroup decodes once ------------------
+//
+// A workgroup of 8 waves owns a tile of query rows of one (sequence, KV head): WR row waves of 16 NT rows, each
+// times WK waves that take different 32-key chunks (short prompts). It walks the keys in tiles of 16,384 values per
+// plane: the rows of tile j + 2 are on their way to registers while tile j + 1 is decoded into the spare half of a
+// double LDS buffer and tile j is multiplied, one barrier per tile. A wave stages 16 (head_dim 256: 8) whole rows of
+// a tile, so its page is a scalar. K and V keep their row order in LDS: K pieces are swizzled for the 16-byte operand
+// reads, V in 32-byte segments for the transposing reads (ds_read_b64_tr_b16), which deliver V^T operands in the key
+// order that the S^T accumulator leaves P in.
+// Operands are FP16 (K and Q of BF16 caches stay BF16): K' = code * scale and V' = code * scale or value, times a
+// power of two that the workgroup takes from its first tile (three bits of room above its largest scale or value),
+// rounded once (2^-11). A tile with a larger, infinite or NaN value or (INT8) a V scale below 2^-18 of the top is left
+// out, and its chunks are walked with attend_chunk afterwards, which has no such range; BF16 values down to 2^-29 of the
+// top are exact.
+
+constexpr int kManyThreads = 512;
+constexpr int kManyMarks = 131072;          // key tiles of a workgroup, at most
+static_assert(kPagedMaxKeys <= 64 * kManyMarks);
+
+template <int D, int WK>
+struct ManyGeo {
+    static constexpr int NT = D == 128 ? 2 : 1;
+    static constexpr int WR = 8 / WK;
+    static constexpr int BM = 16 * NT * WR; // query rows of a workgroup
+    static constexpr int KT = 16384 / D;    // keys of a tile
+    static constexpr int LG = D == 128 ? 7 : 6;
+    static constexpr int NCH = KT / 32;
+    static constexpr int RW = KT / 8;       // rows that a wave stages
+    static constexpr int kPlane = 32768;
+    static constexpr int kBuf = 2 * kPlane;
+    static_assert(NCH % WK == 0, "every wave takes whole chunks");
+};
+
+// A wave's rows of a tile on their way.
 template <int D, bool BF>
-__global__ __launch_bounds__(256) void paged_attn_row_kernel(PagedAttnArgs x) {
-    __shared__ float xq[D], xp[256], xr[8], xv[256 / (D / 4)][D];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t n = blockIdx.x / x.a.Hq;
-    const int qh = static_cast<int>(blockIdx.x % x.a.Hq);
-    const int h = qh / x.G;
-    int lo = 0, hi = x.c.B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (x.a.starts[mid] <= n) { lo = mid; } else { hi = mid; }
+struct StageRegs {
+    static constexpr int U = BF ? 4 : 2; // 16-byte units of a lane and plane
+    u4 k[U], v[U];
+    uint32_t ks[BF ? 1 : U], vs[BF ? 1 : U];
+};
+
+template <int D, bool BF>
+__device__ __forceinline__ void stage_load(const PagedAttnArgs& x, int h, int key0, int page, int lane, StageRegs<D, BF>& r) {
+    constexpr int kRow = BF ? 2 * D : D;
+    constexpr int PR = kRow / 16; // units of a row
+    constexpr int RW = ManyGeo<D, 1>::RW;
+    const bool there = page >= 0;
+    const int64_t pg = there ? page : 0;
+    const int64_t row = (static_cast<int64_t>(h) << x.c.page_shift) + (key0 & ((1 << x.c.page_shift) - 1));
+    const __amdgpu_buffer_rsrc_t kb = raw_buffer(x.c.k + pg * x.c.k_page + row * kRow, there ? RW * kRow : 0);
+    const __amdgpu_buffer_rsrc_t vb = raw_buffer(x.c.v + pg * x.c.v_page + row * kRow, there ? RW * kRow : 0);
+#pragma unroll
+    for (int i = 0; i < StageRegs<D, BF>::U; ++i) {
+        r.k[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(kb, 16 * (lane + 64 * i), 0, 0));
+        r.v[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(vb, 16 * (lane + 64 * i), 0, 0));
     }
-    const Seq s = sequence(x, lo);
-    if (n < s.start || n >= s.start + s.tokens || s.tokens * x.G <= x.few_rows) { return; }
-    const int p = s.history + static_cast<int>(n - s.start);
-    const int first = x.a.window > 0 ? max(0, p + 1 - x.a.window) : 0;
-    const int nsink = min(x.a.sinks, first);
-    const int keys = nsink + p + 1 - first;
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(x.a.q.data + n * x.a.q.token_stride) + qh * D;
-    if (tid < D) { xq[tid] = bf16_to_f32(q[tid]) * x.scale_log2; }
-    __syncthreads();
-    const int32_t* table = x.c.table + lo * x.c.table_row;
-    const int mask = (1 << x.c.page_shift) - 1;
-    const auto where = [&](int i, int& page) {
-        const int key = i < nsink ? i : first + i - nsink;
-        const int slot = key >> x.c.page_shift;
-        page = slot < x.c.max_pages ? table[slot] : -1;
-        page = page >= 0 && page < x.c.pages ? page : -1;
-        return (h << x.c.page_shift) + (key & mask);
+    if constexpr (!BF) {
+        constexpr int kScaleRow = D / 32;
+        const __amdgpu_buffer_rsrc_t ksb = raw_buffer(x.c.ks + pg * x.c.ks_page + row * kScaleRow, there ? RW * kScaleRow : 0);
+        const __amdgpu_buffer_rsrc_t vsb = raw_buffer(x.c.vs + pg * x.c.vs_page + row * kScaleRow, there ? RW * kScaleRow : 0);
+#pragma unroll
+        for (int i = 0; i < StageRegs<D, BF>::U; ++i) {
+            const int u = lane + 64 * i;
+            const int off = (u / PR) * kScaleRow + 2 * ((u % PR) / 4);
+            r.ks[i] = __builtin_amdgcn_raw_buffer_load_b16(ksb, off, 0, 0) & 0xffffu;
+            r.vs[i] = __builtin_amdgcn_raw_buffer_load_b16(vsb, off, 0, 0) & 0xffffu;
+        }
+    }
+}
+
+// Rows at or past `live` (of the wave's RW) belong to no visible key: their scales and values become zero.
+template <int D, bool BF>
+__device__ __forceinline__ void stage_trim(StageRegs<D, BF>& r, int live, int lane) {
+    constexpr int PR = (BF ? 2 * D : D) / 16;
+#pragma unroll
+    for (int i = 0; i < StageRegs<D, BF>::U; ++i) {
+        const bool dead = (lane + 64 * i) / PR >= live;
+        if constexpr (BF) {
+            r.v[i] = dead ? u4{0u, 0u, 0u, 0u} : r.v[i];
+        } else {
+            r.ks[i] = dead ? 0u : r.ks[i];
+            r.vs[i] = dead ? 0u : r.vs[i];
+        }
+    }
+}
+
+// The largest magnitudes of a thread's part, NaN kept: K's and V's scales, or (BF16) V's values.
+template <int D, bool BF>
+__device__ __forceinline__ void stage_top(const StageRegs<D, BF>& r, float& kt, float& vt) {
+    kt = vt = 0.0f;
+#pragma unroll
+    for (int i = 0; i < StageRegs<D, BF>::U; ++i) {
+        if constexpr (BF) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                vt = fmax_ieee(vt, fmax_ieee(fabsf(__uint_as_float(r.v[i][w] << 16)), fabsf(__uint_as_float(r.v[i][w] & 0xffff0000u))));
+            }
+        } else {
+            kt = fmax_ieee(kt, fabsf(f16_bits_to_f32(static_cast<uint16_t>(r.ks[i]))));
+            vt = fmax_ieee(vt, fabsf(f16_bits_to_f32(static_cast<uint16_t>(r.vs[i]))));
+        }
+    }
+}
+
+// The workgroup's powers of two and the bounds of what they can hold.
+struct ManyScale {
+    float k, v;       // factors of K' and V'
+    float klim, vlim; // a tile with a larger scale (BF16: value) needs care
+};
+
+// INT8: |code| <= 128, so scales below 2^E give K' below 2^15; BF16: values below 2^E.
+__device__ __forceinline__ void pick(float top, int shift, float& factor, float& lim) {
+    const uint32_t b = __float_as_uint(top) >> 23;
+    // no finite top (or none): factor one
+    const int E = top > 0.0f && b < 255u ? max(-100, min(100, static_cast<int>(b) - 126 + 3)) : shift;
+    factor = __uint_as_float(static_cast<uint32_t>(127 + shift - E) << 23);
+    lim = __uint_as_float(static_cast<uint32_t>(127 + E) << 23);
+}
+
+// Decodes a thread's part into a tile; returns whether it holds what the FP16 operands cannot.
+template <int D, bool BF>
+__device__ __forceinline__ bool stage_store(const StageRegs<D, BF>& r, const ManyScale& sc, char* buf, int row0, int lane) {
+    constexpr int kRow = BF ? 2 * D : D;
+    constexpr int PR = kRow / 16;
+    char* vp = buf + ManyGeo<D, 1>::kPlane;
+    float kt, vt;
+    stage_top<D, BF>(r, kt, vt);
+    bool small = false; // an INT8 V scale that FP16 would round
+#pragma unroll
+    for (int i = 0; i < StageRegs<D, BF>::U; ++i) {
+        const int u = lane + 64 * i;
+        const int row = row0 + u / PR;
+        const int at = row * 2 * D;
+        const int k7 = row & 7;
+        if constexpr (BF) {
+            const int p = u % PR; // piece of eight dims
+            *reinterpret_cast<u4*>(buf + at + 16 * (p ^ (row & 15))) = r.k[i];
+            u4 y;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const h2 z = {static_cast<_Float16>(__uint_as_float(r.v[i][w] << 16) * sc.v),
+                              static_cast<_Float16>(__uint_as_float(r.v[i][w] & 0xffff0000u) * sc.v)};
+                y[w] = __builtin_bit_cast(uint32_t, z);
+            }
+            *reinterpret_cast<u4*>(vp + at + 32 * ((p >> 1) ^ k7) + 16 * (p & 1)) = y;
+        } else {
+            const int p = 2 * (u % PR); // two pieces of eight dims
+            const _Float16 k1 = static_cast<_Float16>(f16_bits_to_f32(static_cast<uint16_t>(r.ks[i])) * sc.k);
+            const _Float16 v1 = static_cast<_Float16>(f16_bits_to_f32(static_cast<uint16_t>(r.vs[i])) * sc.v);
+            const h2 k2 = {k1, k1}, v2 = {v1, v1};
+            small |= r.vs[i] != 0u && fabsf(static_cast<float>(v1)) < 0x1p-14f;
+            *reinterpret_cast<h8*>(buf + at + 16 * (p ^ (row & 15))) = scale_h8(codes8(r.k[i][0], r.k[i][1]), k2);
+            *reinterpret_cast<h8*>(buf + at + 16 * ((p + 1) ^ (row & 15))) = scale_h8(codes8(r.k[i][2], r.k[i][3]), k2);
+            char* vr = vp + at + 32 * ((p >> 1) ^ k7);
+            *reinterpret_cast<h8*>(vr) = scale_h8(codes8(r.v[i][0], r.v[i][1]), v2);
+            *reinterpret_cast<h8*>(vr + 16) = scale_h8(codes8(r.v[i][2], r.v[i][3]), v2);
+        }
+    }
+    return small || !(kt <= sc.klim && vt <= sc.vlim); // NaN: care
+}
+
+struct ManyWork {
+    int b; // -1: none
+    int tile;
+};
+
+// The sequences' row tiles in order; `slot` counts them over the batch.
+__device__ __forceinline__ ManyWork many_work(const PagedAttnArgs& x, int slot, int bm, int lane) {
+    ManyWork w{-1, 0};
+    int sum = 0;
+    for (int base = 0; base < x.c.B; base += 64) {
+        int n = 0;
+        if (base + lane < x.c.B) {
+            const Seq s = sequence(x, base + lane);
+            const int rows = s.tokens * x.G;
+            n = rows > x.few_rows ? (rows + bm - 1) / bm : 0;
+        }
+        const int end = sum + wave_inclusive_scan(n);
+        const uint64_t mine = __ballot(n > 0 && slot >= end - n && slot < end);
+        if (mine != 0u) {
+            const int at = __ffsll(static_cast<long long>(mine)) - 1;
+            w.b = base + at;
+            // the last tokens see the most keys: their tiles first
+            w.tile = __builtin_amdgcn_readlane(end, at) - 1 - slot;
+            return w;
+        }
+        sum = __builtin_amdgcn_readlane(end, 63);
+    }
+    return w;
+}
+
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ u2 read_tr(const char* p) {
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((NMI_AS3 s4*)(p)));
+}
+
+template <int D, bool BF, int WK>
+__global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_many_kernel(PagedAttnArgs x) {
+    using MG = ManyGeo<D, WK>;
+    constexpr int NT = MG::NT, KT = MG::KT;
+    __shared__ __attribute__((aligned(256))) char smem[2 * MG::kBuf];
+    __shared__ uint32_t marks[kManyMarks / 32]; // tiles that need care
+    __shared__ uint32_t state[2][8];            // per buffer and wave: bit 0 its page exists, bit 1 care
+    __shared__ float tops[2][8];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int wr = wave / WK, wk = wave % WK;
+    const int h = blockIdx.x % x.c.Hkv;
+    const int unit = blockIdx.x / x.c.Hkv;
+    const int split = unit % x.nsplit;
+    const int slot = unit / x.nsplit;
+    const ManyWork w = many_work(x, slot, MG::BM, lane);
+    if (w.b < 0) { return; }
+    const Seq s = sequence(x, w.b);
+    const int rows = s.tokens * x.G;
+    const int r0 = w.tile * MG::BM;
+    const int p0 = s.history + r0 / x.G, p1 = s.history + (min(r0 + MG::BM, rows) - 1) / x.G;
+    const Tiles tiles = tiles_of(x, p0, p1, MG::LG);
+    const int per = (tiles.count + x.nsplit - 1) / x.nsplit;
+    const int j0 = min(split * per, tiles.count), j1 = min(j0 + per, tiles.count);
+
+    // pages of the wave's rows, 64 tiles at a time
+    const int32_t* table = x.c.table + w.b * x.c.table_row;
+    const auto pages_from = [&](int j) {
+        const int key = tiles.tile(j + lane) * KT + wave * MG::RW;
+        int page = -1;
+        if (j + lane < j1 && key <= p1) { page = table[key >> x.c.page_shift]; }
+        return page >= 0 && page < x.c.pages ? page : -1;
     };
-    float M = -INFINITY, L = 0.0f;
-    f4 O = {0.f, 0.f, 0.f, 0.f};
-    constexpr int TPR = D / 4, PARTS = 256 / TPR;
-    const int d4 = 4 * (tid % TPR), part = tid / TPR;
-    for (int base = 0; base < keys; base += 256) {
-        float sc = -INFINITY;
-        int page;
-        if (base + tid < keys) {
-            const int64_t row = where(base + tid, page);
-            if (page >= 0) {
-                sc = 0.0f;
-                const char* kp = x.c.k + page * x.c.k_page + row * D * (BF ? 2 : 1);
-                for (int d = 0; d < D; ++d) {
-                    float k;
-                    if constexpr (BF) {
-                        k = bf16_to_f32(reinterpret_cast<const uint16_t*>(kp)[d]);
-                    } else {
-                        k = static_cast<float>(reinterpret_cast<const int8_t*>(kp)[d]) *
-                            f16_bits_to_f32(reinterpret_cast<const uint16_t*>(x.c.ks + page * x.c.ks_page)[row * (D / 64) + d / 64]);
+    int ids = pages_from(j0), next_ids = pages_from(j0 + 64);
+    StageRegs<D, BF> sr;
+    int page = -1; // of the rows in `sr`
+    const auto fetch = [&](int j) {
+        const int i = j - j0;
+        if ((i & 63) == 0 && i > 0) { // a new 64: they were fetched 64 tiles ago
+            ids = next_ids;
+            next_ids = pages_from(j + 64);
+        }
+        page = __builtin_amdgcn_readlane(ids, i & 63);
+        stage_load<D, BF>(x, h, tiles.tile(j) * KT + wave * MG::RW, page, lane, sr);
+    };
+    ManyScale sc{1.0f, 1.0f, INFINITY, INFINITY};
+    const auto trim = [&](int j) {
+        const int live = p1 + 1 - (tiles.tile(j) * KT + wave * MG::RW);
+        if (live < MG::RW) { stage_trim<D, BF>(sr, live, lane); }
+    };
+    const auto put = [&](int j) {
+        trim(j);
+        const bool care = stage_store<D, BF>(sr, sc, smem + ((j - j0) & 1) * MG::kBuf, wave * MG::RW, lane);
+        const uint32_t st = (page >= 0 ? 1u : 0u) | (__any(care) ? 2u : 0u);
+        if (lane == 0) { state[(j - j0) & 1][wave] = st; }
+    };
+
+    if (j0 < j1) { fetch(j0); }
+    Rows<D, BF, NT> r;
+    const int row0 = r0 + 16 * NT * wr;
+    init_rows<D, BF, NT>(x, s, h, row0, c, g, r);
+    f4 l[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) { l[nt] = f4{0.f, 0.f, 0.f, 0.f}; }
+    bool cared = false;
+    if (j0 < j1) {
+        for (int i = threadIdx.x; 32 * i < j1 - j0; i += kManyThreads) { marks[i] = 0u; }
+        trim(j0);
+        float kt, vt;
+        stage_top<D, BF>(sr, kt, vt);
+        kt = wave_max(kt < INFINITY ? kt : 0.0f);
+        vt = wave_max(vt < INFINITY ? vt : 0.0f);
+        if (lane == 0) {
+            tops[0][wave] = kt;
+            tops[1][wave] = vt;
+        }
+        __syncthreads();
+        kt = vt = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            kt = fmaxf(kt, tops[0][i]);
+            vt = fmaxf(vt, tops[1][i]);
+        }
+        pick(kt, 8, sc.k, sc.klim);
+        pick(vt, BF ? 15 : 8, sc.v, sc.vlim);
+        put(j0);
+        if (j0 + 1 < j1) { fetch(j0 + 1); }
+        __syncthreads();
+    }
+    float mul[NT]; // raw score of the FP16 K' -> log2 domain
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) { mul[nt] = BF ? r.rowmul[nt] : r.rowmul[nt] / sc.k; }
+    // the wave's V^T reads: lane (c, g) addresses key 4 g + (c >> 2), dims 4 (c & 3) .. of a 16-dim segment
+    const int vkey = 4 * g + (c >> 2);
+    const int voff = vkey * 2 * D + 32 * (vkey & 7) + 8 * (c & 3);
+    const int low = min(r.lo, kPagedMaxKeys) + 1 - x.a.window; // the wave sees nothing below it but sinks
+#pragma unroll 1
+    for (int j = j0; j < j1; ++j) {
+        const char* buf = smem + ((j - j0) & 1) * MG::kBuf;
+        uint32_t here = 0u, care = 0u;
+        {
+            const u4* st = reinterpret_cast<const u4*>(state[(j - j0) & 1]);
+            const u4 a = st[0], b = st[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                here |= (a[i] & 1u) << i | (b[i] & 1u) << (4 + i);
+                care |= (a[i] | b[i]) & 2u;
+            }
+            here = __builtin_amdgcn_readfirstlane(here);
+            care = __builtin_amdgcn_readfirstlane(care);
+        }
+        if (j + 1 < j1) {
+            put(j + 1);
+            if (j + 2 < j1) { fetch(j + 2); }
+        }
+        const int key0 = tiles.tile(j) * KT;
+        if (care != 0u) {
+            cared = true;
+            if (threadIdx.x == 0) { marks[(j - j0) >> 5] |= 1u << ((j - j0) & 31); }
+        } else {
+#pragma unroll 1
+            for (int cw = 0; cw < MG::NCH / WK; ++cw) {
+                const int ci = cw * WK + wk;
+                const int c0 = key0 + 32 * ci;
+                // the halves' pages: two waves' rows each at head_dim 256
+                const uint32_t bits = D == 128 ? here >> (2 * ci) : (here >> (4 * ci) & 1u) | (here >> (4 * ci + 1) & 2u);
+                // by arithmetic: hipcc 7.2 inverted a select on a bit of a scalar here (s_bitcmp0 for s_bitcmp1)
+                const Halves hv{{static_cast<int>(bits & 1u) - 1, static_cast<int>((bits >> 1) & 1u) - 1}};
+                if (c0 > r.hi || (c0 + 31 < low && c0 >= x.a.sinks) || (hv.page[0] & hv.page[1]) < 0) { continue; }
+                f4 sacc[2][NT];
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    const char* krow = buf + (32 * ci + 16 * kt + c) * 2 * D;
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k) {
+                        const int piece = BF ? 4 * k + g : 8 * (k >> 1) + 2 * g + (k & 1);
+                        const u4 ka = *reinterpret_cast<const u4*>(krow + 16 * (piece ^ c));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const f4 acc = k == 0 ? f4{0.f, 0.f, 0.f, 0.f} : sacc[kt][nt];
+                            if constexpr (BF) {
+                                sacc[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, ka), __builtin_bit_cast(bf8, r.q[nt][k]), acc, 0, 0, 0);
+                            } else {
+                                sacc[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, ka), __builtin_bit_cast(h8, r.q[nt][k]), acc, 0, 0, 0);
+                            }
+                        }
                     }
-                    sc = fmaf(xq[d], k, sc);
+                }
+                float sv[NT][8];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { sv[nt][i] = sacc[i >> 2][nt][i & 3]; }
+                }
+                if (!all_seen(x, r.lo, r.hi, c0 >> 5, hv)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const bool ok = sees(x, r.pos[nt], c0 + 16 * (i >> 2) + 4 * g + (i & 3), hv.page[i >> 2]);
+                            sv[nt][i] = ok ? sv[nt][i] : -INFINITY;
+                        }
+                    }
+                }
+                float cmax[NT];
+                bool any = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    cmax[nt] = score_max(sv[nt]);
+                    any |= (cmax[nt] - r.m[nt]) * mul[nt] > kLazyTau;
+                }
+                if (__any(any)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const bool need = (cmax[nt] - r.m[nt]) * mul[nt] > kLazyTau;
+                        const float mn = need ? cmax[nt] : r.m[nt];
+                        const float alpha = need ? __builtin_amdgcn_exp2f((r.m[nt] - mn) * mul[nt]) : 1.0f;
+#pragma unroll
+                        for (int t = 0; t < D / 16; ++t) { r.O[nt][t] *= alpha; }
+                        l[nt] *= alpha;
+                        r.m[nt] = mn;
+                    }
+                }
+                h8 p[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float bias = r.m[nt] == -INFINITY ? 0.0f : fmaf(-r.m[nt], mul[nt], kPOffset);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { p[nt][i] = static_cast<_Float16>(__builtin_amdgcn_exp2f(fmaf(sv[nt][i], mul[nt], bias))); }
+                }
+                const char* vp = buf + MG::kPlane + 32 * ci * 2 * D;
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) {
+                    const int at = (voff ^ (32 * (t & 7))) + 256 * (t >> 3);
+                    const u2 a = read_tr(vp + at), b = read_tr(vp + at + 16 * 2 * D);
+                    const u4 va = {a[0], a[1], b[0], b[1]};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        r.O[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, va), p[nt], r.O[nt][t], 0, 0, 0);
+                    }
+                }
+                const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) { l[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[nt], l[nt], 0, 0, 0); }
+            }
+        }
+        __syncthreads(); // this buffer is free, the next tile is in place
+    }
+    const float unit_v = 1.0f / sc.v; // an exact power of two
+    float M[NT], L[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        M[nt] = r.m[nt] == -INFINITY ? -INFINITY : r.m[nt] * mul[nt];
+        L[nt] = l[nt][0];
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) { r.O[nt][t] *= unit_v; }
+    }
+    if (__builtin_expect(cared, 0)) {
+        // the state so far to LDS (each wave its own part), then the marked tiles with a new one
+        float* keep = reinterpret_cast<float*>(smem) + wave * (16 * NT * D);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) {
+                *reinterpret_cast<f4*>(keep + (16 * nt + c) * D + 16 * t + 4 * g) = r.O[nt][t];
+                r.O[nt][t] = f4{0.f, 0.f, 0.f, 0.f};
+            }
+            r.m[nt] = -INFINITY;
+            r.l[nt] = 0.0f;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int base = 0; base < j1 - j0; base += 32) {
+            uint32_t bits = __builtin_amdgcn_readfirstlane(marks[base >> 5]);
+#pragma unroll 1
+            for (; bits != 0u; bits &= bits - 1u) {
+                const int key0 = tiles.tile(j0 + base + __builtin_ctz(bits)) * KT;
+#pragma unroll 1
+                for (int cw = 0; cw < MG::NCH / WK; ++cw) {
+                    const int c0 = key0 + 32 * (cw * WK + wk);
+                    if (c0 > r.hi) { continue; }
+                    Halves hv;
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt) {
+                        const int key = c0 + 16 * kt;
+                        const int pg = key <= p1 ? table[key >> x.c.page_shift] : -1;
+                        hv.page[kt] = __builtin_amdgcn_readfirstlane(pg >= 0 && pg < x.c.pages ? pg : -1);
+                    }
+                    Chunk<D, BF> ck;
+                    load_chunk<D, BF>(x, h, c0 >> 5, hv, c, g, ck);
+                    attend_chunk<D, BF, NT>(x, c0 >> 5, hv, c, g, ck, r);
                 }
             }
         }
-        const float wm = wave_max(sc);
-        if (lane == 0) { xr[wave] = wm; }
-        __syncthreads();
-        float Mn = M;
-        for (int w = 0; w < 4; ++w) { Mn = fmaxf(Mn, xr[w]); }
-        const float alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
-        const float pr = sc == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sc - Mn);
-        xp[tid] = pr;
-        const float ws = wave_sum(pr);
-        if (lane == 0) { xr[4 + wave] = ws; }
-        __syncthreads();
-        L = fmaf(L, alpha, xr[4] + xr[5] + xr[6] + xr[7]);
-        O *= alpha;
-        for (int i = part; i < 256; i += PARTS) {
-            if (base + i >= keys) { break; }
-            const int64_t row = where(base + i, page);
-            if (page < 0) { continue; }
-            const char* vp = x.c.v + page * x.c.v_page + row * D * (BF ? 2 : 1);
-            float s8 = 1.0f;
-            if constexpr (!BF) { s8 = f16_bits_to_f32(reinterpret_cast<const uint16_t*>(x.c.vs + page * x.c.vs_page)[row * (D / 64) + d4 / 64]); }
-            for (int e = 0; e < 4; ++e) {
-                const float v = BF ? bf16_to_f32(reinterpret_cast<const uint16_t*>(vp)[d4 + e])
-                                   : static_cast<float>(reinterpret_cast<const int8_t*>(vp)[d4 + e]) * s8;
-                O[e] = fmaf(xp[i], v, O[e]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const float m2 = r.m[nt] == -INFINITY ? -INFINITY : r.m[nt] * r.rowmul[nt], l2 = group4_sum(r.l[nt]);
+            const Weights q = weights(M[nt], L[nt], m2, l2);
+            L[nt] = L[nt] * q.a + l2 * q.b;
+            M[nt] = q.M;
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) {
+                f4 o; // back in the first walk's order of dims, so that what follows is the same
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { o[e] = q.b == 0.0f ? 0.0f : r.O[nt][t][e] * q.b; }
+                r.O[nt][t] = o;
+            }
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float* y = keep + (16 * nt + c) * D + out_dim<BF>(t, 4 * g + e);
+                    *y = (q.a == 0.0f ? 0.0f : *y * q.a) + r.O[nt][t][e];
+                }
             }
         }
-        M = Mn;
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) { r.O[nt][t] = *reinterpret_cast<const f4*>(keep + (16 * nt + c) * D + 16 * t + 4 * g); }
+        }
         __syncthreads();
     }
-    *reinterpret_cast<f4*>(&xv[part][d4]) = O;
-    __syncthreads();
-    if (tid < D) {
-        float o = 0.0f;
-        for (int w = 0; w < PARTS; ++w) { o += xv[w][tid]; }
-        o = L > 0.0f || L != L ? o / L : 0.0f;
-        (reinterpret_cast<uint16_t*>(x.a.out.data + n * x.a.out.token_stride) + qh * D)[tid] = f32_to_bf16_bits(o);
+    // ---- the WK key waves of a row tile through LDS
+    if constexpr (WK > 1) {
+        f4* xo = reinterpret_cast<f4*>(smem);
+        constexpr int kPer = NT * (D / 16) * 64;
+        static_assert((WK - 1) * MG::WR * kPer * 16 + (WK - 1) * MG::WR * NT * 64 * 8 <= 2 * MG::kBuf, "merge exceeds the buffers");
+        float2* xm = reinterpret_cast<float2*>(smem + (WK - 1) * MG::WR * kPer * 16);
+        if (wk > 0) {
+            const int at = (wk - 1) * MG::WR + wr;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) { xo[at * kPer + (nt * (D / 16) + t) * 64 + lane] = r.O[nt][t]; }
+                xm[(at * NT + nt) * 64 + lane] = float2{M[nt], L[nt]};
+            }
+        }
+        __syncthreads();
+        if (wk > 0) { return; }
+#pragma unroll
+        for (int i = 0; i < WK - 1; ++i) {
+            const int at = i * MG::WR + wr;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float2 o = xm[(at * NT + nt) * 64 + lane];
+                const Weights q = weights(M[nt], L[nt], o.x, o.y);
+                L[nt] = L[nt] * q.a + o.y * q.b;
+                M[nt] = q.M;
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) {
+                    const f4 y = xo[at * kPer + (nt * (D / 16) + t) * 64 + lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { r.O[nt][t][e] = (q.a == 0.0f ? 0.0f : r.O[nt][t][e] * q.a) + (q.b == 0.0f ? 0.0f : y[e] * q.b); }
+                }
+            }
+        }
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int rr = 16 * (NT * wr + nt) + c; // of the workgroup's rows
+        const int row = r0 + rr;
+        if (row >= rows) { continue; }
+        if (x.nsplit > 1) {
+            const int64_t at = ((static_cast<int64_t>(slot) * x.c.Hkv + h) * x.nsplit + split) * MG::BM + rr;
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) { *reinterpret_cast<f4*>(x.many_o + at * D + 16 * t + 4 * g) = r.O[nt][t]; }
+            if (g == 0) { *reinterpret_cast<float2*>(x.many_ml + 2 * at) = float2{M[nt], L[nt]}; }
+        } else {
+            const int t1 = row / x.G;
+            uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + (s.start + t1) * x.a.out.token_stride) + (h * x.G + row - t1 * x.G) * D + 4 * g;
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) { *reinterpret_cast<u2*>(out + 16 * t) = out_pair(r.O[nt][t], L[nt]); }
+        }
+    }
+}
+
+// The splits of a many-row workgroup's rows: D / 4 threads per row.
+template <int D>
+__global__ __launch_bounds__(256) void paged_attn_many_merge_kernel(PagedAttnArgs x, int bm) {
+    constexpr int TPR = D / 4, RPB = 256 / TPR;
+    const int per = bm / RPB; // workgroups of a (row tile, head)
+    const int h = blockIdx.x / per % x.c.Hkv;
+    const int slot = blockIdx.x / per / x.c.Hkv;
+    const int rr = blockIdx.x % per * RPB + threadIdx.x / TPR;
+    const ManyWork w = many_work(x, slot, bm, threadIdx.x & 63);
+    if (w.b < 0) { return; }
+    const Seq s = sequence(x, w.b);
+    const int row = w.tile * bm + rr;
+    if (row >= s.tokens * x.G) { return; }
+    const int d = 4 * (threadIdx.x % TPR);
+    float M = -INFINITY, L = 0.0f;
+    f4 O = {0.f, 0.f, 0.f, 0.f};
+    const int64_t first = ((static_cast<int64_t>(slot) * x.c.Hkv + h) * x.nsplit) * bm + rr;
+#pragma unroll 4
+    for (int k = 0; k < x.nsplit; ++k) {
+        const int64_t at = first + static_cast<int64_t>(k) * bm;
+        const float2 ml = *reinterpret_cast<const float2*>(x.many_ml + 2 * at);
+        const f4 o = *reinterpret_cast<const f4*>(x.many_o + at * D + d);
+        const Weights q = weights(M, L, ml.x, ml.y);
+        L = L * q.a + ml.y * q.b;
+        M = q.M;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { O[e] = (q.a == 0.0f ? 0.0f : O[e] * q.a) + (q.b == 0.0f ? 0.0f : o[e] * q.b); }
+    }
+    const int t = row / x.G;
+    uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + (s.start + t) * x.a.out.token_stride) + (h * x.G + row - t * x.G) * D + d;
+    *reinterpret_cast<u2*>(out) = out_pair(O, L);
 }
 
 } // namespace
@@ -848,13 +1334,20 @@ namespace {
 struct PagedPlan {
     int32_t nt = 1;        // 16-row tiles of a few-row workgroup
     int32_t few_rows = 0;
-    int32_t slots = 0;
+    int32_t slots = 0;     // 0: no sequence of few rows is possible
     int32_t min_units = 2;
     bool merge = false;
+    int32_t wk = 1;        // many rows: waves of a row tile over the keys
+    int32_t tiles = 0;     // row tiles of the batch, at most (0: no sequence of many rows is possible)
+    int32_t nsplit = 1;
     size_t ml_offset = 0;
     size_t table_offset = 0;
+    size_t many_offset = 0;
+    size_t many_ml_offset = 0;
     size_t bytes = 0;
 };
+
+size_t align_up(size_t v) { return (v + 255) & ~size_t{255}; }
 
 PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t B, int32_t max_new, int32_t max_keys, int32_t window,
                      int32_t sinks) {
@@ -862,49 +1355,97 @@ PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t
     PagedPlan p;
     p.nt = static_cast<int64_t>(max_new) * G <= 16 ? 1 : 2;
     p.few_rows = 16 * p.nt;
-    // the most tiles that a few-row sequence walks
-    int64_t keys = max_keys;
-    if (window > 0) {
-        const int64_t most = static_cast<int64_t>(window) + std::min<int64_t>(max_new, p.few_rows) + 62 + (static_cast<int64_t>(sinks) + 31) / 32 * 32;
-        keys = std::min(keys, most);
-    }
-    const int64_t units = (keys + 127) / 128;
-    if (units <= p.min_units) {
-        p.slots = B + 1;
-    } else {
-        p.slots = static_cast<int32_t>(std::max<int64_t>(std::min<int64_t>(512 / Hkv, B * ((units + p.min_units - 1) / p.min_units)), 2 * B));
-        p.merge = true;
-    }
+    const int64_t most_rows = std::min<int64_t>(max_new, tokens) * G; // of a sequence
+    // the most keys that `n` tokens see
+    const auto seen = [&](int64_t n) {
+        if (window == 0) { return static_cast<int64_t>(max_keys); }
+        return std::min<int64_t>(max_keys, static_cast<int64_t>(window) + n + 126 + (static_cast<int64_t>(sinks) + 127) / 128 * 128);
+    };
     size_t at = 0;
-    if (p.merge) {
-        const size_t rows = static_cast<size_t>(p.slots) * Hkv * p.few_rows;
-        at = rows * D * sizeof(float);
-        p.ml_offset = at;
-        at += rows * 2 * sizeof(float);
+    {
+        const int64_t units = (seen(std::min<int64_t>(max_new, p.few_rows)) + 127) / 128;
+        if (units <= p.min_units) {
+            p.slots = B + 1;
+        } else {
+            p.slots = static_cast<int32_t>(std::max<int64_t>(std::min<int64_t>(512 / Hkv, B * ((units + p.min_units - 1) / p.min_units)), 2 * B));
+            p.merge = true;
+        }
+        if (p.merge) {
+            const size_t rows = static_cast<size_t>(p.slots) * Hkv * p.few_rows;
+            p.ml_offset = align_up(rows * D * sizeof(float));
+            at = align_up(p.ml_offset + rows * 2 * sizeof(float));
+        }
+        p.table_offset = at;
+        at = align_up(at + static_cast<size_t>(B) * 2 * sizeof(int32_t));
     }
-    p.table_offset = at;
-    p.bytes = at + static_cast<size_t>(B) * 2 * sizeof(int32_t);
+    if (most_rows > p.few_rows) {
+        const int64_t rows = tokens * G;
+        const int64_t seqs = std::min<int64_t>(B, rows / (p.few_rows + 1));
+        const int64_t keys = seen(max_new);
+        const int64_t kt = 16384 / D;
+        double best = 1e30;
+        int32_t best_bm = 0;
+        for (int32_t wk = 1; wk <= (D == 128 ? 4 : 2); wk *= 2) {
+            const int32_t bm = (D == 128 ? 256 : 128) / wk;
+            const double tile_us = D == 128 ? (wk == 1 ? 4.7 : wk == 2 ? 2.8 : 1.95) : (wk == 1 ? 2.75 : 1.95);
+            const int64_t tiles = rows / bm + seqs;
+            const double longest = static_cast<double>(keys) / kt;
+            for (int32_t ns = 1; ns == 1 || (ns <= 32 && 2 * ns <= longest); ++ns) {
+                const double wgs = static_cast<double>(rows) / bm * Hkv * ns / 256.0; // per CU
+                double us = ns > 1 ? 5.0 + 1e-6 * static_cast<double>(tiles) * Hkv * ns * bm * D / 256.0 : 0.0;
+                us += 5.0 * std::max(1.0, wgs) + tile_us * longest / ns * (wgs <= 1.0 ? 1.0 : wgs + 0.5);
+                if (us < best) {
+                    best = us;
+                    p.wk = wk;
+                    p.nsplit = ns;
+                    p.tiles = static_cast<int32_t>(tiles);
+                    best_bm = bm;
+                }
+            }
+        }
+        if (p.nsplit > 1) {
+            const size_t parts = static_cast<size_t>(p.tiles) * Hkv * p.nsplit * best_bm;
+            p.many_offset = at;
+            p.many_ml_offset = align_up(at + parts * D * sizeof(float));
+            at = align_up(p.many_ml_offset + parts * 2 * sizeof(float));
+        }
+    }
+    p.bytes = at;
     return p;
 }
 
 template <int D, bool BF>
 void launch(PagedAttnArgs& x, const PagedPlan& p, hipStream_t stream) {
-    const uint32_t grid = static_cast<uint32_t>(p.slots) * x.c.Hkv;
-    if (p.nt == 1) {
-        hipLaunchKernelGGL((paged_attn_few_kernel<D, BF, 1>), dim3(grid), dim3(kFewThreads), 0, stream, x);
-    } else {
-        hipLaunchKernelGGL((paged_attn_few_kernel<D, BF, 2>), dim3(grid), dim3(kFewThreads), 0, stream, x);
+    if (p.slots > 0) {
+        const uint32_t grid = static_cast<uint32_t>(p.slots) * x.c.Hkv;
+        if (p.nt == 1) {
+            hipLaunchKernelGGL((paged_attn_few_kernel<D, BF, 1>), dim3(grid), dim3(kFewThreads), 0, stream, x);
+        } else {
+            hipLaunchKernelGGL((paged_attn_few_kernel<D, BF, 2>), dim3(grid), dim3(kFewThreads), 0, stream, x);
+        }
+        check_launch("paged_attn_few_kernel");
+        if (p.merge) {
+            hipLaunchKernelGGL((paged_attn_merge_kernel<D>), dim3(p.few_rows * x.c.Hkv, x.c.B), dim3(256), 0, stream, x, p.few_rows);
+            check_launch("paged_attn_merge_kernel");
+        }
     }
-    check_launch("paged_attn_few_kernel");
-    if (p.merge) {
-        hipLaunchKernelGGL((paged_attn_merge_kernel<D>), dim3(p.few_rows * x.c.Hkv, x.c.B), dim3(256), 0, stream, x, p.few_rows);
-        check_launch("paged_attn_merge_kernel");
+    if (p.tiles == 0) { return; }
+    const int64_t blocks = static_cast<int64_t>(p.tiles) * x.c.Hkv * p.nsplit;
+    if (blocks > 0x7FFFFF) { throw Unsupported("paged attention: more than 2^23 workgroups are not built"); }
+    const dim3 grid(static_cast<uint32_t>(blocks));
+    if (p.wk == 1) {
+        hipLaunchKernelGGL((paged_attn_many_kernel<D, BF, 1>), grid, dim3(kManyThreads), 0, stream, x);
+    } else if (p.wk == 2) {
+        hipLaunchKernelGGL((paged_attn_many_kernel<D, BF, 2>), grid, dim3(kManyThreads), 0, stream, x);
+    } else if constexpr (D == 128) {
+        hipLaunchKernelGGL((paged_attn_many_kernel<D, BF, 4>), grid, dim3(kManyThreads), 0, stream, x);
     }
-    if (static_cast<int64_t>(x.a.max_new) * x.G > p.few_rows) {
-        const int64_t blocks = x.a.tokens * x.a.Hq;
-        if (blocks > 0x7FFFFFFF) { throw Unsupported("paged attention: more than 2^31 query rows are not built"); }
-        hipLaunchKernelGGL((paged_attn_row_kernel<D, BF>), dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream, x);
-        check_launch("paged_attn_row_kernel");
+    check_launch("paged_attn_many_kernel");
+    if (p.nsplit > 1) {
+        const int bm = (D == 128 ? 256 : 128) / p.wk;
+        hipLaunchKernelGGL((paged_attn_many_merge_kernel<D>), dim3(static_cast<uint32_t>(static_cast<int64_t>(p.tiles) * x.c.Hkv * (bm / (256 / (D / 4))))),
+                           dim3(256), 0, stream, x, bm);
+        check_launch("paged_attn_many_merge_kernel");
     }
 }
 
@@ -919,16 +1460,20 @@ void launch_paged_attention(const PagedAttention& a, const PagedRef& c, void* wo
     const PagedPlan p = plan_paged(a.Hq, c.Hkv, c.D, a.tokens, c.B, a.max_new, a.max_keys, a.window, a.sinks);
     PagedAttnArgs x{};
     x.a = a;
+    if (a.window == 0) { x.a.window = 0x7FFFFFFF; } // every row of at most kPagedMaxKeys
     x.c = c;
     x.G = a.Hq / c.Hkv;
     x.scale_log2 = a.scale * 1.4426950408889634f;
     x.few_rows = p.few_rows;
     x.slots = p.slots;
     x.min_units = p.min_units;
+    x.nsplit = p.nsplit;
     char* ws = static_cast<char*>(workspace);
     x.part_o = reinterpret_cast<float*>(ws);
     x.part_ml = reinterpret_cast<float*>(ws + p.ml_offset);
     x.seq_table = reinterpret_cast<int32_t*>(ws + p.table_offset);
+    x.many_o = reinterpret_cast<float*>(ws + p.many_offset);
+    x.many_ml = reinterpret_cast<float*>(ws + p.many_ml_offset);
     if (c.D == 128 && !c.bf16) {
         launch<128, false>(x, p, stream);
     } else if (c.D == 128) {

@@ -9,6 +9,9 @@ namespace nmi {
 // Sequences of one call: the kernels keep their first tokens in LDS or spread them over a wave.
 inline constexpr int32_t kPagedMaxBatch = 1024;
 
+// Rows of a sequence in an attention call: a workgroup marks key tiles of 64 rows in a bit field in LDS.
+inline constexpr int32_t kPagedMaxKeys = 1 << 23;
+
 // A validated paged cache view. Row r of a page: plane + page * page_stride + (h * page_size + r) * row bytes.
 struct PagedRef {
     char* k = nullptr; // I8 codes or BF16 values

@@ -159,7 +159,14 @@ class PagedCase:
                             o += np.where(m[:, None, j, None] & ~np.isfinite(v[j]), v[j], 0.0)
                         A = p @ np.where(np.isfinite(v), np.abs(v), 0.0)
                         d = size.max(-1, initial=0.0, keepdims=True) * 2.0**-11
-                        tol[n0 + i0:n0 + i1, hh * G:(hh + 1) * G] = 2.0**-8 * np.abs(o) + A * (2 * np.expm1(np.minimum(2 * d, 50.0)) + 2.0**-10 + 2.0**-20) + 1e-30
+                        # a score error of d changes a probability by a factor of exp(2 d) at most; past 2 d = 50 that bounds nothing
+                        # (a p of 1e-320 is 0 in `A` and may be 1), but any two weighted means of v lie within 2 max |v|
+                        loose = 2.0 * np.where(m[:, :, None], np.where(np.isfinite(v), np.abs(v), 0.0)[None], 0.0).max(1, initial=0.0)[:, None]
+                        e = np.where(2 * d > 50, loose, A * (2 * np.expm1(np.minimum(2 * d, 50.0)) + 2.0**-10 + 2.0**-20))
+                        # FP16 holds p * 2^8 down to steps of 2^-24: every key's p is off by 2^-33 at least, and its V scale's share
+                        # of the largest one by as much
+                        floor = 2.0**-32 * m.sum(-1)[:, None, None] * np.where(np.isfinite(v), np.abs(v), 0.0).max(initial=0.0)
+                        tol[n0 + i0:n0 + i1, hh * G:(hh + 1) * G] = 2.0**-8 * np.abs(o) + e + floor + 1e-30
                     out[n0 + i0:n0 + i1, hh * G:(hh + 1) * G] = o
         return out, tol
 

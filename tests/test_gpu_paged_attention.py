@@ -144,6 +144,27 @@ def test_small_values_next_to_large_ones(gpu, kv, tokens):
 
 
 @pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("geo", ["40-8-128", "24-4-256"])
+@pytest.mark.parametrize("tokens,window", [(13, 0), (90, 0), (300, 0), (300, 200)])
+def test_large_values_in_later_tiles(gpu, geo, kv, tokens, window):
+    """Keys and values that outgrow what the first key tile led to expect: a V of 1,000 times the size that counts, one of
+    1e5 times that hardly does, a K of 300 times, in tiles of their own and among new tokens."""
+    Hq, Hkv, D = GEO[geo]
+
+    def grow(x, f):
+        x[:] = bf16_bits((x.astype(np.uint32) << 16).view(np.float32) * np.float32(f))
+
+    def edit(c):
+        grow(c.v[0][310], 1e3)
+        grow(c.k[0][450, 0], 300.0)
+        grow(c.v[0][600 + tokens // 2, Hkv - 1], 3e3)
+        c.q[:, :, 1] = bf16_bits(np.float32(8.0))
+        c.k[0][590, :, 1] = bf16_bits(np.float32(-60.0))
+        grow(c.v[0][590], 1e5)
+    _run(PagedCase([(tokens, 600)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=21, window=window, sinks=3 if window else 0, edit=edit))
+
+
+@pytest.mark.parametrize("kv", CACHES)
 @pytest.mark.parametrize("scale", [1e-4, 1.0, 3.0])
 def test_scale(gpu, kv, scale):
     _run(PagedCase([(1, 300), (70, 30)], Hq=8, Hkv=2, kv=kv, seed=11, scale=scale))

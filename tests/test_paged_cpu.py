@@ -117,7 +117,7 @@ Q = T(na.BF16, 128, 8, 5)
     (dict(out=T(na.BF16, 128, 8, 4)), ValueError), (dict(out=T(na.BF16, 128, 8, 5, nb={2: 2056})), ValueError),
     (dict(scale=0.0), ValueError), (dict(scale=-1.0), ValueError), (dict(scale=float("nan")), ValueError), (dict(scale=float("inf")), ValueError), (dict(scale=2.0**-41), ValueError), (dict(scale=2.0**41), ValueError),
     (dict(envelope=(0, 32)), ValueError), (dict(envelope=(33, 32)), ValueError), (dict(envelope=(5, 65)), ValueError),
-    (dict(envelope=(5, 1 << 31)), OverflowError), (dict(window=(1 << 31, 0)), OverflowError), (dict(window=(0, 4)), ValueError),
+    (dict(envelope=(5, (1 << 23) + 1)), NotImplementedError), (dict(envelope=(5, 1 << 31)), OverflowError), (dict(window=(1 << 31, 0)), OverflowError), (dict(window=(0, 4)), ValueError),
     (dict(ws=Ws(nbytes=0)), ValueError), (dict(ws=Ws(ptr=FAKE + 16)), ValueError), (dict(ws=None), ValueError),
 ])
 def test_attention_arguments(kw, error):
@@ -127,6 +127,8 @@ def test_attention_arguments(kw, error):
     if "ws" in kw:  # a plan that needs a workspace
         v = view(max_pages=4096, pages=4096)
         a["envelope"] = (5, 65536)
+    if error is NotImplementedError:
+        v = view(max_pages=1 << 20)
     with pytest.raises(error):
         ops.paged_attention(a["q"], T(na.I32, 4), T(na.I32, 3), a["scale"], a["window"], v, a["envelope"], a["ws"], a["out"])
 
@@ -137,7 +139,7 @@ def test_workspace_query():
     # what the op refuses needs none
     for bad in [(40, 7, 128, 1, 1, (1, 64)), (0, 8, 128, 1, 1, (1, 64)), (40, 8, 64, 1, 1, (1, 64)), (40, 8, 128, 0, 1, (1, 64)),
                 (40, 8, 128, 1, 0, (1, 64)), (40, 8, 128, 1, 1025, (1, 64)), (40, 8, 128, 1, 1, (0, 64)), (40, 8, 128, 1, 1, (65, 64)),
-                (40, 8, 128, 1, 1, (1, 1 << 31))]:
+                (40, 8, 128, 1, 1, (1, 1 << 31)), (40, 8, 128, 1, 1, (1, (1 << 23) + 1)), (40, 8, 128, 1 << 27, 1, (1, 64))]:
         assert q(*bad) == 0
     # a window bounds the rows that are split
     assert q(40, 8, 128, 1, 1, (1, 1 << 20), (64, 4)) <= q(40, 8, 128, 1, 1, (1, 1 << 20))
