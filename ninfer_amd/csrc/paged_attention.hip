@@ -20,6 +20,15 @@
 
 #include <algorithm>
 #include <type_traits>
+#ifndef FEW_WAVES
+#define FEW_WAVES 2
+#endif
+#ifndef FEW_WAVES256
+#define FEW_WAVES256 1
+#endif
+#ifndef FEW_DEEP
+#define FEW_DEEP 1
+#endif
 
 namespace nmi {
 namespace {
@@ -37,7 +46,7 @@ struct PagedAttnArgs {
     float* part_o;     // FP32 O [partial row][D] and (log2-domain maximum, sum) [partial row][2]
     float* part_ml;
     int32_t* seq_table; // per sequence: first slot, splits
-    int32_t nsplit;     // key splits of a many-row workgroup's rows, and their parts as above
+    int32_t many_parts; // parts that the many-row workgroups' splits may have (0: none), and those as above
     float* many_o;
     float* many_ml;
 };
@@ -112,10 +121,18 @@ struct Chunk {
     static constexpr int VP = BF ? D / 128 : D / 64; // V pieces of a lane and key
     static constexpr int VW = BF ? 4 : 1;            // words of a V piece
     static constexpr int SW = BF ? 1 : D / 128;      // 16-byte words of four keys' scales
-    u4 k[2][KP];
-    uint32_t v[8][VP][VW];
-    u4 ks[2][SW];
-    u4 vs[2][SW];
+};
+
+template <int D, bool BF>
+struct ChunkK {
+    u4 k[2][Chunk<D, BF>::KP];
+    u4 ks[2][Chunk<D, BF>::SW];
+};
+
+template <int D, bool BF>
+struct ChunkV {
+    uint32_t v[8][Chunk<D, BF>::VP][Chunk<D, BF>::VW];
+    u4 vs[2][Chunk<D, BF>::SW];
 };
 
 // What a chunk's loads are aimed at: the 16-row halves' pages (-1: none).
@@ -123,42 +140,64 @@ struct Halves {
     int32_t page[2];
 };
 
+// One plane's rows of a half tile as a buffer; an absent half is a buffer of no bytes, whose loads give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t half_rows(const PagedAttnArgs& x, const char* plane, int64_t page_stride, int bytes, int h, int tile,
+                                                           int kt, Halves hv) {
+    const bool there = hv.page[kt] >= 0;
+    const int64_t page = there ? hv.page[kt] : 0;
+    const int64_t row = (static_cast<int64_t>(h) << x.c.page_shift) + ((32 * tile + 16 * kt) & ((1 << x.c.page_shift) - 1));
+    return raw_buffer(plane + page * page_stride + row * bytes, there ? 16 * bytes : 0);
+}
+
+constexpr int kOnce = 2; // cache policy of rows that a call reads once (non-temporal)
+
 template <int D, bool BF>
-__device__ __forceinline__ void load_chunk(const PagedAttnArgs& x, int h, int tile, Halves hv, int c, int g, Chunk<D, BF>& r) {
+__device__ __forceinline__ void load_keys(const PagedAttnArgs& x, int h, int tile, Halves hv, int c, int g, ChunkK<D, BF>& r) {
     using CK = Chunk<D, BF>;
     constexpr int kRow = BF ? 2 * D : D;
     constexpr int kScaleRow = D / 32; // bytes of a row's scales
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-        // an absent half loads nothing (a buffer of no bytes): zeros
-        const bool there = hv.page[kt] >= 0;
-        const int64_t page = there ? hv.page[kt] : 0;
-        const int64_t row = (static_cast<int64_t>(h) << x.c.page_shift) + ((32 * tile + 16 * kt) & ((1 << x.c.page_shift) - 1));
-        const __amdgpu_buffer_rsrc_t kb = raw_buffer(x.c.k + page * x.c.k_page + row * kRow, there ? 16 * kRow : 0);
-        const __amdgpu_buffer_rsrc_t vb = raw_buffer(x.c.v + page * x.c.v_page + row * kRow, there ? 16 * kRow : 0);
+        const __amdgpu_buffer_rsrc_t kb = half_rows(x, x.c.k, x.c.k_page, kRow, h, tile, kt, hv);
 #pragma unroll
         for (int i = 0; i < CK::KP; ++i) {
-            r.k[kt][i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(kb, c * kRow + 64 * i + 16 * g, 0, 2));
+            r.k[kt][i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(kb, c * kRow + 64 * i + 16 * g, 0, kOnce));
         }
         if constexpr (!BF) {
-            const __amdgpu_buffer_rsrc_t ksb = raw_buffer(x.c.ks + page * x.c.ks_page + row * kScaleRow, there ? 16 * kScaleRow : 0);
-            const __amdgpu_buffer_rsrc_t vsb = raw_buffer(x.c.vs + page * x.c.vs_page + row * kScaleRow, there ? 16 * kScaleRow : 0);
+            const __amdgpu_buffer_rsrc_t ksb = half_rows(x, x.c.ks, x.c.ks_page, kScaleRow, h, tile, kt, hv);
 #pragma unroll
             for (int w = 0; w < CK::SW; ++w) {
                 r.ks[kt][w] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(ksb, 4 * g * kScaleRow + 16 * w, 0, 0));
+            }
+        }
+    }
+}
+
+template <int D, bool BF>
+__device__ __forceinline__ void load_values(const PagedAttnArgs& x, int h, int tile, Halves hv, int c, int g, ChunkV<D, BF>& r) {
+    using CK = Chunk<D, BF>;
+    constexpr int kRow = BF ? 2 * D : D;
+    constexpr int kScaleRow = D / 32;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+        if constexpr (!BF) {
+            const __amdgpu_buffer_rsrc_t vsb = half_rows(x, x.c.vs, x.c.vs_page, kScaleRow, h, tile, kt, hv);
+#pragma unroll
+            for (int w = 0; w < CK::SW; ++w) {
                 r.vs[kt][w] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(vsb, 4 * g * kScaleRow + 16 * w, 0, 0));
             }
         }
+        const __amdgpu_buffer_rsrc_t vb = half_rows(x, x.c.v, x.c.v_page, kRow, h, tile, kt, hv);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
             for (int i = 0; i < CK::VP; ++i) {
                 if constexpr (BF) {
-                    const u4 w = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(vb, (4 * g + j) * kRow + 256 * i + 16 * c, 0, 2));
+                    const u4 w = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(vb, (4 * g + j) * kRow + 256 * i + 16 * c, 0, kOnce));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) { r.v[4 * kt + j][i][e] = w[e]; }
                 } else {
-                    r.v[4 * kt + j][i][0] = __builtin_amdgcn_raw_buffer_load_b32(vb, (4 * g + j) * kRow + 64 * i + 4 * c, 0, 2);
+                    r.v[4 * kt + j][i][0] = __builtin_amdgcn_raw_buffer_load_b32(vb, (4 * g + j) * kRow + 64 * i + 4 * c, 0, kOnce);
                 }
             }
         }
@@ -275,8 +314,16 @@ __device__ __forceinline__ bool all_seen(const PagedAttnArgs& x, int lo, int hi,
 // An infinite or NaN BF16 in either half of a word: that half's sign bit (of the result) set.
 __device__ __forceinline__ uint32_t nonfinite_bits(uint32_t x) { return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
 
+// A chunk's probabilities (times 2^kPOffset), and which of its keys a lane's rows see.
+template <int NT>
+struct Probs {
+    float p[NT][8];
+    uint32_t seen[NT]; // bit i: row nt's lane sees key i
+    bool whole;        // every row sees every key
+};
+
 template <int D, bool BF, int NT>
-__device__ __forceinline__ void attend_chunk(const PagedAttnArgs& x, int tile, Halves hv, int c, int g, Chunk<D, BF>& r, Rows<D, BF, NT>& s) {
+__device__ __forceinline__ void chunk_probs(const PagedAttnArgs& x, int tile, Halves hv, int g, const ChunkK<D, BF>& r, Rows<D, BF, NT>& s, Probs<NT>& y) {
     using CK = Chunk<D, BF>;
     const bool whole = all_seen(x, s.lo, s.hi, tile, hv);
     float sv[NT][8];
@@ -309,20 +356,49 @@ __device__ __forceinline__ void attend_chunk(const PagedAttnArgs& x, int tile, H
             }
         }
     }
-    uint32_t seen[NT]; // bit i: row nt's lane sees key i (masked chunks)
+    y.whole = whole;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) { seen[nt] = 0xffu; }
+    for (int nt = 0; nt < NT; ++nt) { y.seen[nt] = 0xffu; }
     if (!whole) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            seen[nt] = 0u;
+            y.seen[nt] = 0u;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const bool ok = sees(x, s.pos[nt], 32 * tile + 16 * (i >> 2) + 4 * g + (i & 3), hv.page[i >> 2]);
-                seen[nt] |= ok ? 1u << i : 0u;
+                y.seen[nt] |= ok ? 1u << i : 0u;
                 sv[nt][i] = ok ? sv[nt][i] : -INFINITY;
             }
         }
+    }
+    // ---- running maximum (it moves only when a score tops it by 2^kLazyTau), probabilities, sums
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const float cmax = score_max(sv[nt]);
+        const bool need = (cmax - s.m[nt]) * s.rowmul[nt] > kLazyTau;
+        if (__any(need)) {
+            const float mn = need ? cmax : s.m[nt];
+            const float alpha = need ? __builtin_amdgcn_exp2f((s.m[nt] - mn) * s.rowmul[nt]) : 1.0f;
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) { s.O[nt][t] *= alpha; }
+            s.l[nt] *= alpha;
+            s.m[nt] = mn;
+        }
+        const float bias = s.m[nt] == -INFINITY ? 0.0f : fmaf(-s.m[nt], s.rowmul[nt], kPOffset);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            y.p[nt][i] = __builtin_amdgcn_exp2f(fmaf(sv[nt][i], s.rowmul[nt], bias));
+        }
+        const float(&p)[8] = y.p[nt];
+        s.l[nt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    }
+}
+
+template <int D, bool BF, int NT>
+__device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const Probs<NT>& y, ChunkV<D, BF>& r, Rows<D, BF, NT>& s) {
+    using CK = Chunk<D, BF>;
+    const float(&p)[NT][8] = y.p;
+    if (!y.whole) {
         // keys that no row of the wave may see: whatever their rows hold is taken out
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -345,28 +421,6 @@ __device__ __forceinline__ void attend_chunk(const PagedAttnArgs& x, int tile, H
             }
         }
     }
-    // ---- running maximum (it moves only when a score tops it by 2^kLazyTau), probabilities, sums
-    float p[NT][8];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const float cmax = score_max(sv[nt]);
-        const bool need = (cmax - s.m[nt]) * s.rowmul[nt] > kLazyTau;
-        if (__any(need)) {
-            const float mn = need ? cmax : s.m[nt];
-            const float alpha = need ? __builtin_amdgcn_exp2f((s.m[nt] - mn) * s.rowmul[nt]) : 1.0f;
-#pragma unroll
-            for (int t = 0; t < D / 16; ++t) { s.O[nt][t] *= alpha; }
-            s.l[nt] *= alpha;
-            s.m[nt] = mn;
-        }
-        const float bias = s.m[nt] == -INFINITY ? 0.0f : fmaf(-s.m[nt], s.rowmul[nt], kPOffset);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            p[nt][i] = __builtin_amdgcn_exp2f(fmaf(sv[nt][i], s.rowmul[nt], bias));
-        }
-        s.l[nt] += ((p[nt][0] + p[nt][1]) + (p[nt][2] + p[nt][3])) + ((p[nt][4] + p[nt][5]) + (p[nt][6] + p[nt][7]));
-    }
-    // ---- values
     if constexpr (!BF) {
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
@@ -388,9 +442,9 @@ __device__ __forceinline__ void attend_chunk(const PagedAttnArgs& x, int tile, H
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    float y = p[nt][k] * (sc[k] * down);
-                    if (!whole) { y = ((seen[nt] >> k) & 1u) ? y : 0.0f; } // an unseen row's scale may be anything
-                    w[nt][k] = static_cast<_Float16>(y);
+                    float z = p[nt][k] * (sc[k] * down);
+                    if (!y.whole) { z = ((y.seen[nt] >> k) & 1u) ? z : 0.0f; } // an unseen row's scale may be anything
+                    w[nt][k] = static_cast<_Float16>(z);
                 }
             }
             const auto tile4 = [&](auto byte) {
@@ -437,17 +491,17 @@ __device__ __forceinline__ void attend_chunk(const PagedAttnArgs& x, int tile, H
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) { one[nt][k] = ((seen[nt] >> k) & 1u) ? static_cast<_Float16>(1.0f) : static_cast<_Float16>(0.0f); }
+                for (int k = 0; k < 8; ++k) { one[nt][k] = ((y.seen[nt] >> k) & 1u) ? static_cast<_Float16>(1.0f) : static_cast<_Float16>(0.0f); }
             }
 #pragma unroll
             for (int i = 0; i < CK::VP; ++i) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
+                    __builtin_amdgcn_sched_barrier(0); // one at a time: the registers are full
                     h8 up, dn;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const uint32_t y = r.v[k][i][e >> 1];
-                        const uint32_t z = ((e & 1) ? y >> 16 : y) & 0xffffu;
+                        const uint32_t z = ((e & 1) ? r.v[k][i][e >> 1] >> 16 : r.v[k][i][e >> 1]) & 0xffffu;
                         const bool nan = (z & 0x7fffu) > 0x7f80u;
                         up[k] = nan || z == 0x7f80u ? static_cast<_Float16>(1.0f) : static_cast<_Float16>(0.0f);
                         dn[k] = nan || z == 0xff80u ? static_cast<_Float16>(1.0f) : static_cast<_Float16>(0.0f);
@@ -576,11 +630,13 @@ __device__ __forceinline__ FewWork few_work(const PagedAttnArgs& x, int slot, in
     return w;
 }
 
-// Waves per SIMD: one where two would not hold the chunk in flight, the chunk at hand and the accumulators.
-constexpr int few_waves(int D, bool, int NT) { return D == 128 && NT == 1 ? 2 : 1; }
+// Waves per SIMD: one where two would not hold a chunk and the accumulators. Chunks in flight next to the one at hand
+// where there is room for them.
+constexpr int few_waves(int D, int NT) { return D == 128 ? FEW_WAVES : NT == 1 ? FEW_WAVES256 : 1; }
+constexpr bool few_deep(int D, int NT) { return D == 128 && NT == 1 && FEW_DEEP; }
 
 template <int D, bool BF, int NT>
-__global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few_waves(D, BF, NT), few_waves(D, BF, NT)))) void paged_attn_few_kernel(PagedAttnArgs x) {
+__global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few_waves(D, NT), few_waves(D, NT)))) void paged_attn_few_kernel(PagedAttnArgs x) {
     // two waves' O and (m, l) at a time
     __shared__ f4 xo[2][NT * (D / 16) * 64];
     __shared__ float2 xm[2][NT * 64];
@@ -613,30 +669,63 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
         return page >= 0 && page < x.c.pages ? page : -1;
     };
     int ids = pages_from(j0), next_ids = pages_from(j0 + 32);
+    // at even tiles: past the 32nd of a fetch the other one is refilled for tiles j + 34 ..
+    const auto refill = [&](int j) {
+        if (((j - j0) & 63) == 30) { ids = pages_from(j + 34); }
+        if (((j - j0) & 63) == 62) { next_ids = pages_from(j + 34); }
+    };
     const auto halves = [&](int j) { // of tile j in [j0, ...): past the end no page
         const int i = 2 * (j - j0);
-        const int from = (i & 127) < 64 ? 0 : 1; // this or the next 64 (see the turn below)
+        const int from = (i & 127) < 64 ? 0 : 1; // this or the next 64
         Halves hv;
         hv.page[0] = __builtin_amdgcn_readlane(from ? next_ids : ids, i & 63);
         hv.page[1] = __builtin_amdgcn_readlane(from ? next_ids : ids, (i & 63) + 1);
         return hv;
     };
-    Chunk<D, BF> ca, cb;
-    Halves ha = halves(j0), hb;
-    load_chunk<D, BF>(x, h, tiles.tile(j0), ha, c, g, ca);
-    init_rows<D, BF, NT>(x, s, h, 0, c, g, r);
+    Probs<NT> pr;
+    if constexpr (few_deep(D, NT)) { // the next chunk is on its way while one is worked on
+        ChunkK<D, BF> ka, kb;
+        ChunkV<D, BF> va, vb;
+        Halves ha = halves(j0), hb;
+        load_keys<D, BF>(x, h, tiles.tile(j0), ha, c, g, ka);
+        load_values<D, BF>(x, h, tiles.tile(j0), ha, c, g, va);
+        init_rows<D, BF, NT>(x, s, h, 0, c, g, r);
 #pragma unroll 1
-    for (int j = j0; j < j1; j += 2) {
-        const int in = (j - j0) & 63; // 0 .. 62: two fetches of 32 tiles
-        hb = halves(j + 1);
-        load_chunk<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, cb);
-        attend_chunk<D, BF, NT>(x, tiles.tile(j), ha, c, g, ca, r);
-        // tiles j + 2 .. : past the 32nd of this fetch the other one is refilled
-        if (in == 30) { ids = pages_from(j + 34); }
-        if (in == 62) { next_ids = pages_from(j + 34); }
-        ha = halves(j + 2);
-        load_chunk<D, BF>(x, h, tiles.tile(j + 2), ha, c, g, ca);
-        if (j + 1 < j1) { attend_chunk<D, BF, NT>(x, tiles.tile(j + 1), hb, c, g, cb, r); }
+        for (int j = j0; j < j1; j += 2) {
+            hb = halves(j + 1);
+            load_keys<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, kb);
+            load_values<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, vb);
+            chunk_probs<D, BF, NT>(x, tiles.tile(j), ha, g, ka, r, pr);
+            chunk_values<D, BF, NT>(tiles.tile(j), ha, g, pr, va, r);
+            refill(j);
+            ha = halves(j + 2);
+            load_keys<D, BF>(x, h, tiles.tile(j + 2), ha, c, g, ka);
+            load_values<D, BF>(x, h, tiles.tile(j + 2), ha, c, g, va);
+            if (j + 1 < j1) {
+                chunk_probs<D, BF, NT>(x, tiles.tile(j + 1), hb, g, kb, r, pr);
+                chunk_values<D, BF, NT>(tiles.tile(j + 1), hb, g, pr, vb, r);
+            }
+        }
+    } else { // registers for one chunk: its keys make room for the next ones' as soon as the scores are there, then its values
+        ChunkK<D, BF> ka;
+        ChunkV<D, BF> va;
+        Halves ha = halves(j0);
+        load_keys<D, BF>(x, h, tiles.tile(j0), ha, c, g, ka);
+        load_values<D, BF>(x, h, tiles.tile(j0), ha, c, g, va);
+        init_rows<D, BF, NT>(x, s, h, 0, c, g, r);
+#pragma unroll 1
+        for (int j = j0; j < j1; ++j) {
+            chunk_probs<D, BF, NT>(x, tiles.tile(j), ha, g, ka, r, pr);
+            if (((j - j0) & 1) == 0) { refill(j); }
+            const Halves hb = halves(j + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            load_keys<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, ka);
+            __builtin_amdgcn_sched_barrier(0);
+            chunk_values<D, BF, NT>(tiles.tile(j), ha, g, pr, va, r);
+            __builtin_amdgcn_sched_barrier(0);
+            load_values<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, va);
+            ha = hb;
+        }
     }
     // ---- the four waves' states into wave 0's: 2 and 3 into 0 and 1, then 1 into 0
     float M[NT], L[NT];
@@ -769,7 +858,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs x, 
 // Operands are FP16 (K and Q of BF16 caches stay BF16): K' = code * scale and V' = code * scale or value, times a
 // power of two that the workgroup takes from its first tile (three bits of room above its largest scale or value),
 // rounded once (2^-11). A tile with a larger, infinite or NaN value or (INT8) a V scale below 2^-18 of the top is left
-// out, and its chunks are walked with attend_chunk afterwards, which has no such range; BF16 values down to 2^-29 of the
+// out, and its chunks are walked as the few-row kernel does it afterwards, which has no such range; BF16 values down to 2^-29 of the
 // top are exact.
 
 constexpr int kManyThreads = 512;
@@ -918,6 +1007,65 @@ __device__ __forceinline__ bool stage_store(const StageRegs<D, BF>& r, const Man
     return small || !(kt <= sc.klim && vt <= sc.vlim); // NaN: care
 }
 
+constexpr int kCus = 256;
+
+// Time of a key tile in us with WK = 1, 2, 4 waves per row tile: what the choices below weigh.
+__host__ __device__ constexpr float tile_us(int D, int wk) {
+    return D == 128 ? (wk == 1 ? 4.0f : wk == 2 ? 2.4f : 1.7f) : (wk == 1 ? 2.4f : 1.7f);
+}
+
+// The last `rem` row tiles x heads that do not fill the chip: key splits of each, and the time they take. A
+// workgroup costs about 4 us besides its key tiles; parts are written and read at 4 TB/s and cost a launch.
+struct Tail {
+    int splits;
+    float us;
+};
+
+__host__ __device__ inline Tail tail_of(int rem, int longest, float us_tile, int elements, int parts) {
+    Tail best{1, 0.0f};
+    if (rem <= 0) { return best; }
+    best.us = 4.0f + static_cast<float>(longest) * us_tile;
+    for (int ns = 2; ns <= 32 && ns * rem <= parts && ns <= longest; ++ns) {
+        const int rounds = (rem * ns + kCus - 1) / kCus;
+        const float us = static_cast<float>(rounds) * (4.0f + static_cast<float>((longest + ns - 1) / ns) * us_tile) + 4.0f +
+                         static_cast<float>(rem * ns) * static_cast<float>(elements) * 2.0e-6f;
+        if (us < best.us) { best = Tail{ns, us}; }
+    }
+    return best;
+}
+
+// Row tiles x heads of the batch: the first `full` fill the chip's rounds, each of the others has `splits` workgroups.
+struct ManyPlan {
+    int units;
+    int full;
+    int splits;
+};
+
+template <int D, int WK>
+__device__ __forceinline__ ManyPlan many_plan(const PagedAttnArgs& x, int lane) {
+    constexpr int BM = ManyGeo<D, WK>::BM;
+    int total = 0, longest = 0;
+    for (int base = 0; base < x.c.B; base += 64) {
+        int n = 0, len = 0;
+        if (base + lane < x.c.B) {
+            const Seq s = sequence(x, base + lane);
+            const int rows = s.tokens * x.G;
+            if (rows > x.few_rows) {
+                n = (rows + BM - 1) / BM;
+                const int last = s.history + s.tokens - 1;
+                len = tiles_of(x, max(s.history, last - (BM - 1) / x.G), last, ManyGeo<D, WK>::LG).count;
+            }
+        }
+        total += __builtin_amdgcn_readlane(wave_inclusive_scan(n), 63);
+        longest = max(longest, static_cast<int>(wave_max(static_cast<float>(len))));
+    }
+    ManyPlan p{total * x.c.Hkv, 0, 1};
+    p.full = p.units / kCus * kCus;
+    p.splits = tail_of(p.units - p.full, longest, tile_us(D, WK), BM * D, x.many_parts).splits;
+    if (p.splits == 1) { p.full = p.units; }
+    return p;
+}
+
 struct ManyWork {
     int b; // -1: none
     int tile;
@@ -966,18 +1114,21 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int wr = wave / WK, wk = wave % WK;
-    const int h = blockIdx.x % x.c.Hkv;
-    const int unit = blockIdx.x / x.c.Hkv;
-    const int split = unit % x.nsplit;
-    const int slot = unit / x.nsplit;
-    const ManyWork w = many_work(x, slot, MG::BM, lane);
+    const ManyPlan plan = many_plan<D, WK>(x, lane);
+    const int id = blockIdx.x;
+    const int unit = id < plan.full ? id : plan.full + (id - plan.full) / plan.splits;
+    const int splits = id < plan.full ? 1 : plan.splits;
+    const int split = id < plan.full ? 0 : (id - plan.full) % plan.splits;
+    if (unit >= plan.units) { return; }
+    const int h = unit % x.c.Hkv;
+    const ManyWork w = many_work(x, unit / x.c.Hkv, MG::BM, lane);
     if (w.b < 0) { return; }
     const Seq s = sequence(x, w.b);
     const int rows = s.tokens * x.G;
     const int r0 = w.tile * MG::BM;
     const int p0 = s.history + r0 / x.G, p1 = s.history + (min(r0 + MG::BM, rows) - 1) / x.G;
     const Tiles tiles = tiles_of(x, p0, p1, MG::LG);
-    const int per = (tiles.count + x.nsplit - 1) / x.nsplit;
+    const int per = (tiles.count + splits - 1) / splits;
     const int j0 = min(split * per, tiles.count), j1 = min(j0 + per, tiles.count);
 
     // pages of the wave's rows, 64 tiles at a time
@@ -1203,9 +1354,16 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
                         const int pg = key <= p1 ? table[key >> x.c.page_shift] : -1;
                         hv.page[kt] = __builtin_amdgcn_readfirstlane(pg >= 0 && pg < x.c.pages ? pg : -1);
                     }
-                    Chunk<D, BF> ck;
-                    load_chunk<D, BF>(x, h, c0 >> 5, hv, c, g, ck);
-                    attend_chunk<D, BF, NT>(x, c0 >> 5, hv, c, g, ck, r);
+                    Probs<NT> pr;
+                    {
+                        ChunkK<D, BF> ck;
+                        load_keys<D, BF>(x, h, c0 >> 5, hv, c, g, ck);
+                        chunk_probs<D, BF, NT>(x, c0 >> 5, hv, g, ck, r, pr);
+                    }
+                    __builtin_amdgcn_sched_barrier(0); // the registers hold one plane's rows at a time
+                    ChunkV<D, BF> cv;
+                    load_values<D, BF>(x, h, c0 >> 5, hv, c, g, cv);
+                    chunk_values<D, BF, NT>(c0 >> 5, hv, g, pr, cv, r);
                 }
             }
         }
@@ -1279,8 +1437,8 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
         const int rr = 16 * (NT * wr + nt) + c; // of the workgroup's rows
         const int row = r0 + rr;
         if (row >= rows) { continue; }
-        if (x.nsplit > 1) {
-            const int64_t at = ((static_cast<int64_t>(slot) * x.c.Hkv + h) * x.nsplit + split) * MG::BM + rr;
+        if (splits > 1) {
+            const int64_t at = static_cast<int64_t>(id - plan.full) * MG::BM + rr;
 #pragma unroll
             for (int t = 0; t < D / 16; ++t) { *reinterpret_cast<f4*>(x.many_o + at * D + 16 * t + 4 * g) = r.O[nt][t]; }
             if (g == 0) { *reinterpret_cast<float2*>(x.many_ml + 2 * at) = float2{M[nt], L[nt]}; }
@@ -1293,26 +1451,29 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
     }
 }
 
-// The splits of a many-row workgroup's rows: D / 4 threads per row.
-template <int D>
-__global__ __launch_bounds__(256) void paged_attn_many_merge_kernel(PagedAttnArgs x, int bm) {
-    constexpr int TPR = D / 4, RPB = 256 / TPR;
-    const int per = bm / RPB; // workgroups of a (row tile, head)
-    const int h = blockIdx.x / per % x.c.Hkv;
-    const int slot = blockIdx.x / per / x.c.Hkv;
-    const int rr = blockIdx.x % per * RPB + threadIdx.x / TPR;
-    const ManyWork w = many_work(x, slot, bm, threadIdx.x & 63);
+// The parts of the split row tiles: D / 4 threads per row.
+template <int D, int WK>
+__global__ __launch_bounds__(256) void paged_attn_many_merge_kernel(PagedAttnArgs x) {
+    constexpr int TPR = D / 4, RPB = 256 / TPR, BM = ManyGeo<D, WK>::BM;
+    const int lane = threadIdx.x & 63;
+    const ManyPlan plan = many_plan<D, WK>(x, lane);
+    const int tail = blockIdx.x / (BM / RPB);
+    if (plan.full + tail >= plan.units) { return; }
+    const int unit = plan.full + tail;
+    const int h = unit % x.c.Hkv;
+    const int rr = blockIdx.x % (BM / RPB) * RPB + threadIdx.x / TPR;
+    const ManyWork w = many_work(x, unit / x.c.Hkv, BM, lane);
     if (w.b < 0) { return; }
     const Seq s = sequence(x, w.b);
-    const int row = w.tile * bm + rr;
+    const int row = w.tile * BM + rr;
     if (row >= s.tokens * x.G) { return; }
     const int d = 4 * (threadIdx.x % TPR);
     float M = -INFINITY, L = 0.0f;
     f4 O = {0.f, 0.f, 0.f, 0.f};
-    const int64_t first = ((static_cast<int64_t>(slot) * x.c.Hkv + h) * x.nsplit) * bm + rr;
+    const int64_t first = static_cast<int64_t>(tail) * plan.splits * BM + rr;
 #pragma unroll 4
-    for (int k = 0; k < x.nsplit; ++k) {
-        const int64_t at = first + static_cast<int64_t>(k) * bm;
+    for (int k = 0; k < plan.splits; ++k) {
+        const int64_t at = first + static_cast<int64_t>(k) * BM;
         const float2 ml = *reinterpret_cast<const float2*>(x.many_ml + 2 * at);
         const f4 o = *reinterpret_cast<const f4*>(x.many_o + at * D + d);
         const Weights q = weights(M, L, ml.x, ml.y);
@@ -1339,7 +1500,7 @@ struct PagedPlan {
     bool merge = false;
     int32_t wk = 1;        // many rows: waves of a row tile over the keys
     int32_t tiles = 0;     // row tiles of the batch, at most (0: no sequence of many rows is possible)
-    int32_t nsplit = 1;
+    int32_t parts = 0;     // of the split row tiles
     size_t ml_offset = 0;
     size_t table_offset = 0;
     size_t many_offset = 0;
@@ -1367,7 +1528,7 @@ PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t
         if (units <= p.min_units) {
             p.slots = B + 1;
         } else {
-            p.slots = static_cast<int32_t>(std::max<int64_t>(std::min<int64_t>(512 / Hkv, B * ((units + p.min_units - 1) / p.min_units)), 2 * B));
+            p.slots = static_cast<int32_t>(std::max<int64_t>(std::min<int64_t>(kCus * few_waves(D, p.nt) / Hkv, B * ((units + p.min_units - 1) / p.min_units)), 2 * B));
             p.merge = true;
         }
         if (p.merge) {
@@ -1382,32 +1543,29 @@ PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t
         const int64_t rows = tokens * G;
         const int64_t seqs = std::min<int64_t>(B, rows / (p.few_rows + 1));
         const int64_t keys = seen(max_new);
-        const int64_t kt = 16384 / D;
+        const int32_t kt = 16384 / D;
+        const int32_t longest = static_cast<int32_t>((keys + kt - 1) / kt);
+        const double mean = std::max(1.0, (static_cast<double>(keys) - (window == 0 ? 0.5 * std::min<double>(static_cast<double>(keys), max_new) : 0.0)) / kt);
         double best = 1e30;
-        int32_t best_bm = 0;
         for (int32_t wk = 1; wk <= (D == 128 ? 4 : 2); wk *= 2) {
             const int32_t bm = (D == 128 ? 256 : 128) / wk;
-            const double tile_us = D == 128 ? (wk == 1 ? 4.7 : wk == 2 ? 2.8 : 1.95) : (wk == 1 ? 2.75 : 1.95);
             const int64_t tiles = rows / bm + seqs;
-            const double longest = static_cast<double>(keys) / kt;
-            for (int32_t ns = 1; ns == 1 || (ns <= 32 && 2 * ns <= longest); ++ns) {
-                const double wgs = static_cast<double>(rows) / bm * Hkv * ns / 256.0; // per CU
-                double us = ns > 1 ? 5.0 + 1e-6 * static_cast<double>(tiles) * Hkv * ns * bm * D / 256.0 : 0.0;
-                us += 5.0 * std::max(1.0, wgs) + tile_us * longest / ns * (wgs <= 1.0 ? 1.0 : wgs + 0.5);
-                if (us < best) {
-                    best = us;
-                    p.wk = wk;
-                    p.nsplit = ns;
-                    p.tiles = static_cast<int32_t>(tiles);
-                    best_bm = bm;
-                }
+            const int32_t parts = static_cast<int32_t>(std::min<int64_t>((1 << 23) / (bm * D), longest > 1 ? tiles * Hkv * 32 : 0));
+            const int64_t units = (rows + bm - 1) / bm * Hkv; // as if one sequence had them
+            const double us = static_cast<double>(units / kCus) * (4.0 + mean * tile_us(D, wk)) +
+                              tail_of(static_cast<int>(units % kCus), longest, tile_us(D, wk), bm * D, parts).us;
+            if (us < best) {
+                best = us;
+                p.wk = wk;
+                p.parts = parts;
+                p.tiles = static_cast<int32_t>(tiles);
             }
         }
-        if (p.nsplit > 1) {
-            const size_t parts = static_cast<size_t>(p.tiles) * Hkv * p.nsplit * best_bm;
+        if (p.parts > 0) {
+            const size_t part_rows = static_cast<size_t>(p.parts) * ((D == 128 ? 256 : 128) / p.wk);
             p.many_offset = at;
-            p.many_ml_offset = align_up(at + parts * D * sizeof(float));
-            at = align_up(p.many_ml_offset + parts * 2 * sizeof(float));
+            p.many_ml_offset = align_up(at + part_rows * D * sizeof(float));
+            at = align_up(p.many_ml_offset + part_rows * 2 * sizeof(float));
         }
     }
     p.bytes = at;
@@ -1430,22 +1588,25 @@ void launch(PagedAttnArgs& x, const PagedPlan& p, hipStream_t stream) {
         }
     }
     if (p.tiles == 0) { return; }
-    const int64_t blocks = static_cast<int64_t>(p.tiles) * x.c.Hkv * p.nsplit;
+    const int64_t blocks = static_cast<int64_t>(p.tiles) * x.c.Hkv;
     if (blocks > 0x7FFFFF) { throw Unsupported("paged attention: more than 2^23 workgroups are not built"); }
-    const dim3 grid(static_cast<uint32_t>(blocks));
+    const dim3 grid(static_cast<uint32_t>(blocks) + p.parts);
+    const uint32_t tails = static_cast<uint32_t>(std::min<int64_t>(blocks, kCus - 1)); // units that may be split
+    const auto go = [&](auto wkc) {
+        constexpr int WK = decltype(wkc)::value;
+        hipLaunchKernelGGL((paged_attn_many_kernel<D, BF, WK>), grid, dim3(kManyThreads), 0, stream, x);
+        check_launch("paged_attn_many_kernel");
+        if (p.parts > 0) {
+            hipLaunchKernelGGL((paged_attn_many_merge_kernel<D, WK>), dim3(tails * (ManyGeo<D, WK>::BM / (1024 / D))), dim3(256), 0, stream, x);
+            check_launch("paged_attn_many_merge_kernel");
+        }
+    };
     if (p.wk == 1) {
-        hipLaunchKernelGGL((paged_attn_many_kernel<D, BF, 1>), grid, dim3(kManyThreads), 0, stream, x);
+        go(std::integral_constant<int, 1>{});
     } else if (p.wk == 2) {
-        hipLaunchKernelGGL((paged_attn_many_kernel<D, BF, 2>), grid, dim3(kManyThreads), 0, stream, x);
+        go(std::integral_constant<int, 2>{});
     } else if constexpr (D == 128) {
-        hipLaunchKernelGGL((paged_attn_many_kernel<D, BF, 4>), grid, dim3(kManyThreads), 0, stream, x);
-    }
-    check_launch("paged_attn_many_kernel");
-    if (p.nsplit > 1) {
-        const int bm = (D == 128 ? 256 : 128) / p.wk;
-        hipLaunchKernelGGL((paged_attn_many_merge_kernel<D>), dim3(static_cast<uint32_t>(static_cast<int64_t>(p.tiles) * x.c.Hkv * (bm / (256 / (D / 4))))),
-                           dim3(256), 0, stream, x, bm);
-        check_launch("paged_attn_many_merge_kernel");
+        go(std::integral_constant<int, 4>{});
     }
 }
 
@@ -1467,7 +1628,7 @@ void launch_paged_attention(const PagedAttention& a, const PagedRef& c, void* wo
     x.few_rows = p.few_rows;
     x.slots = p.slots;
     x.min_units = p.min_units;
-    x.nsplit = p.nsplit;
+    x.many_parts = p.parts;
     char* ws = static_cast<char*>(workspace);
     x.part_o = reinterpret_cast<float*>(ws);
     x.part_ml = reinterpret_cast<float*>(ws + p.ml_offset);
