@@ -26,9 +26,6 @@
 #ifndef FEW_WAVES256
 #define FEW_WAVES256 1
 #endif
-#ifndef FEW_DEEP
-#define FEW_DEEP 1
-#endif
 
 namespace nmi {
 namespace {
@@ -41,11 +38,11 @@ struct PagedAttnArgs {
     int32_t G;
     float scale_log2;
     int32_t few_rows;  // sequences with at most this many rows (tokens x G) are the few-row kernel's
-    int32_t slots;     // its key splits per KV head
-    int32_t min_units; // its shortest split, in units of 128 keys
+    int32_t slots;     // its workgroups per KV head
+    int32_t min_units; // the least share of one, in units of 128 keys
     float* part_o;     // FP32 O [partial row][D] and (log2-domain maximum, sum) [partial row][2]
     float* part_ml;
-    int32_t* seq_table; // per sequence: first slot, splits
+    int32_t* seq_table; // per sequence: first slot, parts
     int32_t many_parts; // parts that the many-row workgroups' splits may have (0: none), and those as above
     float* many_o;
     float* many_ml;
@@ -552,7 +549,7 @@ __device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const P
 
 constexpr int kFewWaves = 4;
 constexpr int kFewThreads = 64 * kFewWaves;
-constexpr int kUnit = 4; // tiles of a split's unit: one for each wave
+constexpr int kUnit = 4; // tiles of a unit: one for each wave
 
 // The units of sequence b's keys that the few-row kernel walks (0: not its sequence).
 __device__ __forceinline__ int few_units(const PagedAttnArgs& x, int b, Seq& s, Tiles& t) {
@@ -562,105 +559,96 @@ __device__ __forceinline__ int few_units(const PagedAttnArgs& x, int b, Seq& s, 
     return (t.count + kUnit - 1) / kUnit;
 }
 
-struct FewWork {
-    int b;      // -1: none
-    int first;  // the sequence's first slot
-    int split;
-    int splits;
-    int units;  // of the sequence
+// The batch's units in a row, sequence after sequence, are cut into `shares` equal runs, one for a workgroup: no workgroup
+// has more than one unit above another, whatever the lengths. A run may end one sequence and begin another: its part of a
+// sequence goes to the slot (share + rank of the sequence among those that have units), a number that no other part has.
+struct FewPlan {
+    int total;  // units
+    int shares;
+    __device__ __forceinline__ int begin(int share) const { return static_cast<int>(static_cast<int64_t>(share) * total / shares); }
+    __device__ __forceinline__ int share_of(int unit) const { return static_cast<int>((static_cast<int64_t>(unit + 1) * shares - 1) / total); }
 };
 
-// The split of `slot`: the shortest split length u (in units) for which all sequences' splits, ceil(units / u) of each,
-// fit the slots. Every wave works it out alone (64 sequences and 64 candidates at a time).
-__device__ __forceinline__ FewWork few_work(const PagedAttnArgs& x, int slot, int lane) {
-    const int B = x.c.B;
+// A sequence and its place among the units.
+struct FewSeq {
+    int b;     // -1: none
+    int rank;
+    int first; // its first unit
+    int units;
+};
+
+// The sequences 64 at a time, spread over the lanes of a wave: units and their inclusive sums.
+struct FewLanes {
+    int units;
+    int end;
+};
+
+__device__ __forceinline__ FewLanes few_lanes(const PagedAttnArgs& x, int base, int sum, int lane) {
     Seq s;
     Tiles t;
-    int total = 0, active = 0;
-    int units = 0; // of sequence `lane` of the last 64
-    for (int base = 0; base < B; base += 64) {
-        units = base + lane < B ? few_units(x, base + lane, s, t) : 0;
-        total += __builtin_amdgcn_readlane(wave_inclusive_scan(units), 63);
-        active += __popcll(__ballot(units > 0));
-    }
-    FewWork w{-1, 0, 0, 0, 0};
-    if (active == 0) { return w; }
-    const int lo = max(x.min_units, (total + x.slots - 1) / x.slots);
-    const int spare = x.slots - active; // the host gives more slots than sequences
-    const int hi = max(lo, (total + spare - 1) / spare);
-    int u = lo;
-    if (hi > lo && active > 1) {
-        const int step = (hi - lo + 62) / 63;
-        const int mine = lo + lane * step;
-        const float inv = 1.0f / static_cast<float>(mine);
-        int need = 0;
-        for (int base = 0; base < B; base += 64) {
-            if (B > 64) { units = base + lane < B ? few_units(x, base + lane, s, t) : 0; }
-            const int n = min(64, B - base);
-            for (int i = 0; i < n; ++i) {
-                const int v = __builtin_amdgcn_readlane(units, i);
-                need += static_cast<int>((static_cast<float>(v + mine - 1) + 0.5f) * inv);
-            }
-        }
-        const uint64_t fits = __ballot(need <= x.slots);
-        u = fits ? lo + (__ffsll(static_cast<long long>(fits)) - 1) * step : hi;
-    }
-    // the prefix sums of the sequences' splits; should the estimate above have been one off, `hi` fits for certain
-    for (;;) {
-        int sum = 0;
-        w.b = -1;
-        for (int base = 0; base < B; base += 64) {
-            if (B > 64) { units = base + lane < B ? few_units(x, base + lane, s, t) : 0; }
-            const int n = (units + u - 1) / u;
-            const int end = sum + wave_inclusive_scan(n);
-            const uint64_t mine = __ballot(n > 0 && slot >= end - n && slot < end);
-            if (mine != 0u) {
-                const int at = __ffsll(static_cast<long long>(mine)) - 1;
-                w.b = base + at;
-                w.splits = __builtin_amdgcn_readlane(n, at);
-                w.first = __builtin_amdgcn_readlane(end, at) - w.splits;
-                w.split = slot - w.first;
-                w.units = __builtin_amdgcn_readlane(units, at);
-            }
-            sum = __builtin_amdgcn_readlane(end, 63);
-        }
-        if (sum <= x.slots || u >= hi) { break; }
-        u = hi;
-    }
-    return w;
+    FewLanes f;
+    f.units = base + lane < x.c.B ? few_units(x, base + lane, s, t) : 0;
+    f.end = sum + wave_inclusive_scan(f.units);
+    return f;
 }
 
-// Waves per SIMD: one where two would not hold a chunk and the accumulators. Chunks in flight next to the one at hand
-// where there is room for them.
-constexpr int few_waves(int D, int NT) { return D == 128 ? FEW_WAVES : NT == 1 ? FEW_WAVES256 : 1; }
-constexpr bool few_deep(int D, int NT) { return D == 128 && NT == 1 && FEW_DEEP; }
+__device__ __forceinline__ FewPlan few_plan(const PagedAttnArgs& x, int lane, FewLanes& f) {
+    FewPlan p{0, 1};
+    for (int base = 0; base < x.c.B; base += 64) {
+        f = few_lanes(x, base, p.total, lane);
+        p.total = __builtin_amdgcn_readlane(f.end, 63);
+    }
+    p.shares = max(1, min(x.slots, p.total / x.min_units));
+    return p;
+}
 
+// The sequence that holds `unit`. `f`: the lanes of the only 64 sequences where there are no more.
+__device__ __forceinline__ FewSeq few_find(const PagedAttnArgs& x, int unit, int lane, FewLanes f) {
+    FewSeq q{-1, 0, 0, 0};
+    int sum = 0;
+    for (int base = 0; base < x.c.B; base += 64) {
+        if (x.c.B > 64) { f = few_lanes(x, base, sum, lane); }
+        const uint64_t some = __ballot(f.units > 0);
+        const uint64_t past = __ballot(f.units > 0 && f.end > unit);
+        if (past != 0u) {
+            const int at = __ffsll(static_cast<long long>(past)) - 1;
+            q.b = base + at;
+            q.rank += __popcll(some & ((uint64_t{1} << at) - 1));
+            q.units = __builtin_amdgcn_readlane(f.units, at);
+            q.first = __builtin_amdgcn_readlane(f.end, at) - q.units;
+            return q;
+        }
+        q.rank += __popcll(some);
+        sum = __builtin_amdgcn_readlane(f.end, 63);
+    }
+    return q;
+}
+
+// Waves per SIMD: one where two would not hold a chunk and the accumulators.
+constexpr int few_waves(int D, int NT) { return D == 128 ? FEW_WAVES : NT == 1 ? FEW_WAVES256 : 1; }
+
+// Units [u0, u1) of sequence q: the part goes to its slot, or, where it is the whole sequence, to the output.
 template <int D, bool BF, int NT>
-__global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few_waves(D, NT), few_waves(D, NT)))) void paged_attn_few_kernel(PagedAttnArgs x) {
-    // two waves' O and (m, l) at a time
-    __shared__ f4 xo[2][NT * (D / 16) * 64];
-    __shared__ float2 xm[2][NT * 64];
+__device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const FewSeq& q, const FewPlan& plan, int share, int u0, int u1,
+                                         f4 (&xo)[2][NT * (D / 16) * 64], float2 (&xm)[2][NT * 64]) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int h = blockIdx.x % x.c.Hkv;
-    const FewWork w = few_work(x, blockIdx.x / x.c.Hkv, lane);
-    if (w.b < 0) { return; }
-    const Seq s = sequence(x, w.b);
+    const Seq s = sequence(x, q.b);
     const Tiles tiles = tiles_of(x, s.history, s.history + s.tokens - 1, 5);
-    const int per = (w.units + w.splits - 1) / w.splits * kUnit; // tiles of a split
-    const int t0 = min(w.split * per, tiles.count), t1 = min(t0 + per, tiles.count);
+    const int t0 = min(u0 * kUnit, tiles.count), t1 = min(u1 * kUnit, tiles.count);
     const int each = (t1 - t0 + kFewWaves - 1) / kFewWaves;
     const int j0 = min(t0 + wave * each, t1), j1 = min(j0 + each, t1);
     const int rows = s.tokens * x.G;
     const int end = s.history + s.tokens;
-    if (w.split == 0 && h == 0 && threadIdx.x == 0) {
-        x.seq_table[2 * w.b] = w.first;
-        x.seq_table[2 * w.b + 1] = w.splits;
+    const int head = plan.share_of(q.first), splits = plan.share_of(q.first + q.units - 1) - head + 1;
+    if (u0 == 0 && h == 0 && threadIdx.x == 0) {
+        x.seq_table[2 * q.b] = head + q.rank;
+        x.seq_table[2 * q.b + 1] = splits;
     }
     Rows<D, BF, NT> r;
     // pages of 64 halves (32 tiles) at a time, one per lane, the next 64 fetched ahead
-    const int32_t* table = x.c.table + w.b * x.c.table_row;
+    const int32_t* table = x.c.table + q.b * x.c.table_row;
     const auto pages_from = [&](int j) {
         const int v = j + (lane >> 1);
         const int key = 32 * tiles.tile(v) + 16 * (lane & 1);
@@ -683,49 +671,25 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
         return hv;
     };
     Probs<NT> pr;
-    if constexpr (few_deep(D, NT)) { // the next chunk is on its way while one is worked on
-        ChunkK<D, BF> ka, kb;
-        ChunkV<D, BF> va, vb;
-        Halves ha = halves(j0), hb;
-        load_keys<D, BF>(x, h, tiles.tile(j0), ha, c, g, ka);
-        load_values<D, BF>(x, h, tiles.tile(j0), ha, c, g, va);
-        init_rows<D, BF, NT>(x, s, h, 0, c, g, r);
+    // registers for one chunk: its keys make room for the next ones' as soon as the scores are there, then its values
+    ChunkK<D, BF> ka;
+    ChunkV<D, BF> va;
+    Halves ha = halves(j0);
+    load_keys<D, BF>(x, h, tiles.tile(j0), ha, c, g, ka);
+    load_values<D, BF>(x, h, tiles.tile(j0), ha, c, g, va);
+    init_rows<D, BF, NT>(x, s, h, 0, c, g, r);
 #pragma unroll 1
-        for (int j = j0; j < j1; j += 2) {
-            hb = halves(j + 1);
-            load_keys<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, kb);
-            load_values<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, vb);
-            chunk_probs<D, BF, NT>(x, tiles.tile(j), ha, g, ka, r, pr);
-            chunk_values<D, BF, NT>(tiles.tile(j), ha, g, pr, va, r);
-            refill(j);
-            ha = halves(j + 2);
-            load_keys<D, BF>(x, h, tiles.tile(j + 2), ha, c, g, ka);
-            load_values<D, BF>(x, h, tiles.tile(j + 2), ha, c, g, va);
-            if (j + 1 < j1) {
-                chunk_probs<D, BF, NT>(x, tiles.tile(j + 1), hb, g, kb, r, pr);
-                chunk_values<D, BF, NT>(tiles.tile(j + 1), hb, g, pr, vb, r);
-            }
-        }
-    } else { // registers for one chunk: its keys make room for the next ones' as soon as the scores are there, then its values
-        ChunkK<D, BF> ka;
-        ChunkV<D, BF> va;
-        Halves ha = halves(j0);
-        load_keys<D, BF>(x, h, tiles.tile(j0), ha, c, g, ka);
-        load_values<D, BF>(x, h, tiles.tile(j0), ha, c, g, va);
-        init_rows<D, BF, NT>(x, s, h, 0, c, g, r);
-#pragma unroll 1
-        for (int j = j0; j < j1; ++j) {
-            chunk_probs<D, BF, NT>(x, tiles.tile(j), ha, g, ka, r, pr);
-            if (((j - j0) & 1) == 0) { refill(j); }
-            const Halves hb = halves(j + 1);
-            __builtin_amdgcn_sched_barrier(0);
-            load_keys<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, ka);
-            __builtin_amdgcn_sched_barrier(0);
-            chunk_values<D, BF, NT>(tiles.tile(j), ha, g, pr, va, r);
-            __builtin_amdgcn_sched_barrier(0);
-            load_values<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, va);
-            ha = hb;
-        }
+    for (int j = j0; j < j1; ++j) {
+        chunk_probs<D, BF, NT>(x, tiles.tile(j), ha, g, ka, r, pr);
+        if (((j - j0) & 1) == 0) { refill(j); }
+        const Halves hb = halves(j + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        load_keys<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, ka);
+        __builtin_amdgcn_sched_barrier(0);
+        chunk_values<D, BF, NT>(tiles.tile(j), ha, g, pr, va, r);
+        __builtin_amdgcn_sched_barrier(0);
+        load_values<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, va);
+        ha = hb;
     }
     // ---- the four waves' states into wave 0's: 2 and 3 into 0 and 1, then 1 into 0
     float M[NT], L[NT];
@@ -734,6 +698,7 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
         M[nt] = r.m[nt] == -INFINITY ? -INFINITY : r.m[nt] * r.rowmul[nt];
         L[nt] = group4_sum(r.l[nt]);
     }
+    __syncthreads(); // the last part's states are read
     const auto halve = [&](int half) {
         if (wave >= half && wave < 2 * half) {
 #pragma unroll
@@ -748,16 +713,16 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const float2 o = xm[wave][nt * 64 + lane];
-                const Weights q = weights(M[nt], L[nt], o.x, o.y);
-                L[nt] = L[nt] * q.a + o.y * q.b;
-                M[nt] = q.M;
+                const Weights wt = weights(M[nt], L[nt], o.x, o.y);
+                L[nt] = L[nt] * wt.a + o.y * wt.b;
+                M[nt] = wt.M;
 #pragma unroll
                 for (int t = 0; t < D / 16; ++t) {
                     const f4 y = xo[wave][(nt * (D / 16) + t) * 64 + lane];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         // a part without weight adds nothing, whatever it holds
-                        r.O[nt][t][e] = (q.a == 0.0f ? 0.0f : r.O[nt][t][e] * q.a) + (q.b == 0.0f ? 0.0f : y[e] * q.b);
+                        r.O[nt][t][e] = (wt.a == 0.0f ? 0.0f : r.O[nt][t][e] * wt.a) + (wt.b == 0.0f ? 0.0f : y[e] * wt.b);
                     }
                 }
             }
@@ -772,16 +737,16 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
     for (int nt = 0; nt < NT; ++nt) {
         const int row = 16 * nt + c;
         if (row >= rows) { continue; }
-        if (w.splits > 1) {
-            const int64_t at = (static_cast<int64_t>(w.first + w.split) * x.c.Hkv + h) * (16 * NT) + row;
+        if (splits > 1) {
+            const int64_t at = (static_cast<int64_t>(share + q.rank) * x.c.Hkv + h) * (16 * NT) + row;
 #pragma unroll
             for (int i = 0; i < D / (16 * RUN); ++i) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float* dst = x.part_o + at * D + out_dim<BF>(RUN * i, 4 * g + e);
 #pragma unroll
-                    for (int q = 0; q < RUN; q += 4) {
-                        *reinterpret_cast<f4*>(dst + q) = f4{r.O[nt][RUN * i + q][e], r.O[nt][RUN * i + q + 1][e], r.O[nt][RUN * i + q + 2][e], r.O[nt][RUN * i + q + 3][e]};
+                    for (int k = 0; k < RUN; k += 4) {
+                        *reinterpret_cast<f4*>(dst + k) = f4{r.O[nt][RUN * i + k][e], r.O[nt][RUN * i + k + 1][e], r.O[nt][RUN * i + k + 2][e], r.O[nt][RUN * i + k + 3][e]};
                     }
                 }
             }
@@ -795,9 +760,9 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
                 for (int e = 0; e < 4; ++e) {
                     uint16_t* dst = out + out_dim<BF>(RUN * i, 4 * g + e);
 #pragma unroll
-                    for (int q = 0; q < RUN; q += 4) {
-                        const f4 o = {r.O[nt][RUN * i + q][e], r.O[nt][RUN * i + q + 1][e], r.O[nt][RUN * i + q + 2][e], r.O[nt][RUN * i + q + 3][e]};
-                        *reinterpret_cast<u2*>(dst + q) = out_pair(o, L[nt]);
+                    for (int k = 0; k < RUN; k += 4) {
+                        const f4 o = {r.O[nt][RUN * i + k][e], r.O[nt][RUN * i + k + 1][e], r.O[nt][RUN * i + k + 2][e], r.O[nt][RUN * i + k + 3][e]};
+                        *reinterpret_cast<u2*>(dst + k) = out_pair(o, L[nt]);
                     }
                 }
             }
@@ -805,6 +770,26 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
     }
 }
 
+template <int D, bool BF, int NT>
+__global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few_waves(D, NT), few_waves(D, NT)))) void paged_attn_few_kernel(PagedAttnArgs x) {
+    // two waves' O and (m, l) at a time
+    __shared__ f4 xo[2][NT * (D / 16) * 64];
+    __shared__ float2 xm[2][NT * 64];
+    const int lane = threadIdx.x & 63;
+    const int h = blockIdx.x % x.c.Hkv;
+    FewLanes fl;
+    const FewPlan plan = few_plan(x, lane, fl);
+    const int share = blockIdx.x / x.c.Hkv;
+    if (plan.total == 0 || share >= plan.shares) { return; }
+    const int stop = plan.begin(share + 1);
+#pragma unroll 1
+    for (int u = plan.begin(share); u < stop;) {
+        const FewSeq q = few_find(x, u, lane, fl);
+        const int next = min(stop, q.first + q.units);
+        few_part<D, BF, NT>(x, h, q, plan, share, u - q.first, next - q.first, xo, xm);
+        u = next;
+    }
+}
 // Log-sum-exp merge of a row's splits: a workgroup per row, groups of D / 4 threads taking every group-th split.
 template <int D>
 __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs x, int slot_rows) {
@@ -1525,14 +1510,10 @@ PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t
     size_t at = 0;
     {
         const int64_t units = (seen(std::min<int64_t>(max_new, p.few_rows)) + 127) / 128;
-        if (units <= p.min_units) {
-            p.slots = B + 1;
-        } else {
-            p.slots = static_cast<int32_t>(std::max<int64_t>(std::min<int64_t>(kCus * few_waves(D, p.nt) / Hkv, B * ((units + p.min_units - 1) / p.min_units)), 2 * B));
-            p.merge = true;
-        }
+        p.slots = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(kCus * few_waves(D, p.nt) / Hkv, B * units / p.min_units)));
+        p.merge = p.slots > 1;
         if (p.merge) {
-            const size_t rows = static_cast<size_t>(p.slots) * Hkv * p.few_rows;
+            const size_t rows = static_cast<size_t>(p.slots + B) * Hkv * p.few_rows;
             p.ml_offset = align_up(rows * D * sizeof(float));
             at = align_up(p.ml_offset + rows * 2 * sizeof(float));
         }
