@@ -39,7 +39,6 @@ struct PagedAttnArgs {
     float scale_log2;
     int32_t few_rows;  // sequences with at most this many rows (tokens x G) are the few-row kernel's
     int32_t slots;     // its workgroups per KV head
-    int32_t min_units; // the least share of one, in units of 128 keys
     float* part_o;     // FP32 O [partial row][D] and (log2-domain maximum, sum) [partial row][2]
     float* part_ml;
     int32_t* seq_table; // per sequence: first slot, parts
@@ -391,7 +390,9 @@ __device__ __forceinline__ void chunk_probs(const PagedAttnArgs& x, int tile, Ha
     }
 }
 
-template <int D, bool BF, int NT>
+// O^T += V^T P^T. CARE (BF16): infinite and NaN values reach only the rows that see them; without it they may make any row
+// of the wave NaN.
+template <int D, bool BF, int NT, bool CARE>
 __device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const Probs<NT>& y, ChunkV<D, BF>& r, Rows<D, BF, NT>& s) {
     using CK = Chunk<D, BF>;
     const float(&p)[NT][8] = y.p;
@@ -471,17 +472,7 @@ __device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const P
                 lo[nt][k] = static_cast<__bf16>(p[nt][k] - static_cast<float>(hi[nt][k]));
             }
         }
-        uint32_t odd = 0u;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-#pragma unroll
-            for (int i = 0; i < CK::VP; ++i) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { odd |= nonfinite_bits(r.v[k][i][e]); }
-            }
-        }
-        const bool care = __any(odd != 0u);
-        if (__builtin_expect(care, 0)) {
+        if constexpr (CARE) {
             // infinite and NaN values: counted apart (+: infinity or NaN, -: the same with the other sign) for the
             // rows that see them, and left out of the products
             h8 one[NT];
@@ -598,7 +589,7 @@ __device__ __forceinline__ FewPlan few_plan(const PagedAttnArgs& x, int lane, Fe
         f = few_lanes(x, base, p.total, lane);
         p.total = __builtin_amdgcn_readlane(f.end, 63);
     }
-    p.shares = max(1, min(x.slots, p.total / x.min_units));
+    p.shares = max(1, min(x.slots, p.total));
     return p;
 }
 
@@ -627,28 +618,13 @@ __device__ __forceinline__ FewSeq few_find(const PagedAttnArgs& x, int unit, int
 // Waves per SIMD: one where two would not hold a chunk and the accumulators.
 constexpr int few_waves(int D, int NT) { return D == 128 ? FEW_WAVES : NT == 1 ? FEW_WAVES256 : 1; }
 
-// Units [u0, u1) of sequence q: the part goes to its slot, or, where it is the whole sequence, to the output.
-template <int D, bool BF, int NT>
-__device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const FewSeq& q, const FewPlan& plan, int share, int u0, int u1,
-                                         f4 (&xo)[2][NT * (D / 16) * 64], float2 (&xm)[2][NT * 64]) {
+// A wave's tiles [j0, j1) of a sequence: the state of its rows.
+template <int D, bool BF, int NT, bool CARE>
+__device__ __forceinline__ void few_walk(const PagedAttnArgs& x, int h, const Seq& s, const Tiles& tiles, const int32_t* table, int j0, int j1, int c, int g,
+                                         Rows<D, BF, NT>& r) {
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 15, g = lane >> 4;
-    const Seq s = sequence(x, q.b);
-    const Tiles tiles = tiles_of(x, s.history, s.history + s.tokens - 1, 5);
-    const int t0 = min(u0 * kUnit, tiles.count), t1 = min(u1 * kUnit, tiles.count);
-    const int each = (t1 - t0 + kFewWaves - 1) / kFewWaves;
-    const int j0 = min(t0 + wave * each, t1), j1 = min(j0 + each, t1);
-    const int rows = s.tokens * x.G;
     const int end = s.history + s.tokens;
-    const int head = plan.share_of(q.first), splits = plan.share_of(q.first + q.units - 1) - head + 1;
-    if (u0 == 0 && h == 0 && threadIdx.x == 0) {
-        x.seq_table[2 * q.b] = head + q.rank;
-        x.seq_table[2 * q.b + 1] = splits;
-    }
-    Rows<D, BF, NT> r;
     // pages of 64 halves (32 tiles) at a time, one per lane, the next 64 fetched ahead
-    const int32_t* table = x.c.table + q.b * x.c.table_row;
     const auto pages_from = [&](int j) {
         const int v = j + (lane >> 1);
         const int key = 32 * tiles.tile(v) + 16 * (lane & 1);
@@ -686,10 +662,45 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
         __builtin_amdgcn_sched_barrier(0);
         load_keys<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, ka);
         __builtin_amdgcn_sched_barrier(0);
-        chunk_values<D, BF, NT>(tiles.tile(j), ha, g, pr, va, r);
+        chunk_values<D, BF, NT, CARE>(tiles.tile(j), ha, g, pr, va, r);
         __builtin_amdgcn_sched_barrier(0);
         load_values<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, va);
         ha = hb;
+    }
+}
+
+// Units [u0, u1) of sequence q: the part goes to its slot, or, where it is the whole sequence, to the output.
+template <int D, bool BF, int NT>
+__device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const FewSeq& q, const FewPlan& plan, int share, int u0, int u1,
+                                         f4 (&xo)[2][NT * (D / 16) * 64], float2 (&xm)[2][NT * 64]) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const Seq s = sequence(x, q.b);
+    const Tiles tiles = tiles_of(x, s.history, s.history + s.tokens - 1, 5);
+    const int t0 = min(u0 * kUnit, tiles.count), t1 = min(u1 * kUnit, tiles.count);
+    const int each = (t1 - t0 + kFewWaves - 1) / kFewWaves;
+    const int j0 = min(t0 + wave * each, t1), j1 = min(j0 + each, t1);
+    const int rows = s.tokens * x.G;
+    const int head = plan.share_of(q.first), splits = plan.share_of(q.first + q.units - 1) - head + 1;
+    if (u0 == 0 && h == 0 && threadIdx.x == 0) {
+        x.seq_table[2 * q.b] = head + q.rank;
+        x.seq_table[2 * q.b + 1] = splits;
+    }
+    Rows<D, BF, NT> r;
+    const int32_t* table = x.c.table + q.b * x.c.table_row;
+    few_walk<D, BF, NT, false>(x, h, s, tiles, table, j0, j1, c, g, r);
+    if constexpr (BF) {
+        uint32_t top = 0u;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { top = max(top, __float_as_uint(r.O[nt][t][e]) << 1); }
+            }
+        }
+        if (__builtin_expect(__any(top >= 0xff000000u), 0)) { few_walk<D, BF, NT, true>(x, h, s, tiles, table, j0, j1, c, g, r); }
     }
     // ---- the four waves' states into wave 0's: 2 and 3 into 0 and 1, then 1 into 0
     float M[NT], L[NT];
@@ -1348,7 +1359,7 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
                     __builtin_amdgcn_sched_barrier(0); // the registers hold one plane's rows at a time
                     ChunkV<D, BF> cv;
                     load_values<D, BF>(x, h, c0 >> 5, hv, c, g, cv);
-                    chunk_values<D, BF, NT>(c0 >> 5, hv, g, pr, cv, r);
+                    chunk_values<D, BF, NT, BF>(c0 >> 5, hv, g, pr, cv, r);
                 }
             }
         }
@@ -1481,7 +1492,6 @@ struct PagedPlan {
     int32_t nt = 1;        // 16-row tiles of a few-row workgroup
     int32_t few_rows = 0;
     int32_t slots = 0;     // 0: no sequence of few rows is possible
-    int32_t min_units = 2;
     bool merge = false;
     int32_t wk = 1;        // many rows: waves of a row tile over the keys
     int32_t tiles = 0;     // row tiles of the batch, at most (0: no sequence of many rows is possible)
@@ -1510,7 +1520,7 @@ PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t
     size_t at = 0;
     {
         const int64_t units = (seen(std::min<int64_t>(max_new, p.few_rows)) + 127) / 128;
-        p.slots = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(kCus * few_waves(D, p.nt) / Hkv, B * units / p.min_units)));
+        p.slots = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(kCus * few_waves(D, p.nt) / Hkv, B * units)));
         p.merge = p.slots > 1;
         if (p.merge) {
             const size_t rows = static_cast<size_t>(p.slots + B) * Hkv * p.few_rows;
@@ -1608,7 +1618,6 @@ void launch_paged_attention(const PagedAttention& a, const PagedRef& c, void* wo
     x.scale_log2 = a.scale * 1.4426950408889634f;
     x.few_rows = p.few_rows;
     x.slots = p.slots;
-    x.min_units = p.min_units;
     x.many_parts = p.parts;
     char* ws = static_cast<char*>(workspace);
     x.part_o = reinterpret_cast<float*>(ws);
