@@ -20,13 +20,6 @@
 
 #include <algorithm>
 #include <type_traits>
-#ifndef FEW_WAVES
-#define FEW_WAVES 2
-#endif
-#ifndef FEW_WAVES256
-#define FEW_WAVES256 1
-#endif
-
 namespace nmi {
 namespace {
 
@@ -616,7 +609,7 @@ __device__ __forceinline__ FewSeq few_find(const PagedAttnArgs& x, int unit, int
 }
 
 // Waves per SIMD: one where two would not hold a chunk and the accumulators.
-constexpr int few_waves(int D, int NT) { return D == 128 ? FEW_WAVES : NT == 1 ? FEW_WAVES256 : 1; }
+constexpr int few_waves(int D) { return D == 128 ? 2 : 1; }
 
 // A wave's tiles [j0, j1) of a sequence: the state of its rows.
 template <int D, bool BF, int NT, bool CARE>
@@ -782,7 +775,7 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
 }
 
 template <int D, bool BF, int NT>
-__global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few_waves(D, NT), few_waves(D, NT)))) void paged_attn_few_kernel(PagedAttnArgs x) {
+__global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few_waves(D), few_waves(D)))) void paged_attn_few_kernel(PagedAttnArgs x) {
     // two waves' O and (m, l) at a time
     __shared__ f4 xo[2][NT * (D / 16) * 64];
     __shared__ float2 xm[2][NT * 64];
@@ -1102,6 +1095,7 @@ template <int D, bool BF, int WK>
 __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_many_kernel(PagedAttnArgs x) {
     using MG = ManyGeo<D, WK>;
     constexpr int NT = MG::NT, KT = MG::KT;
+    constexpr int VF = D == 128 ? 8 : 4; // V^T operands in flight
     __shared__ __attribute__((aligned(256))) char smem[2 * MG::kBuf];
     __shared__ uint32_t marks[kManyMarks / 32]; // tiles that need care
     __shared__ uint32_t state[2][8];            // per buffer and wave: bit 0 its page exists, bit 1 care
@@ -1197,31 +1191,39 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
     // the wave's V^T reads: lane (c, g) addresses key 4 g + (c >> 2), dims 4 (c & 3) .. of a 16-dim segment
     const int vkey = 4 * g + (c >> 2);
     const int voff = vkey * 2 * D + 32 * (vkey & 7) + 8 * (c & 3);
+    // waves w and w + 4 share a SIMD: one decodes the next tile before its products, one after them
+    const bool early = wave < 4;
     const int low = min(r.lo, kPagedMaxKeys) + 1 - x.a.window; // the wave sees nothing below it but sinks
 #pragma unroll 1
     for (int j = j0; j < j1; ++j) {
         const char* buf = smem + ((j - j0) & 1) * MG::kBuf;
-        uint32_t here = 0u, care = 0u;
-        {
-            const u4* st = reinterpret_cast<const u4*>(state[(j - j0) & 1]);
-            const u4 a = st[0], b = st[1];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                here |= (a[i] & 1u) << i | (b[i] & 1u) << (4 + i);
-                care |= (a[i] | b[i]) & 2u;
-            }
-            here = __builtin_amdgcn_readfirstlane(here);
-            care = __builtin_amdgcn_readfirstlane(care);
-        }
-        if (j + 1 < j1) {
-            put(j + 1);
-            if (j + 2 < j1) { fetch(j + 2); }
-        }
+        const uint32_t st = lane < 8 ? state[(j - j0) & 1][lane] : 0u;
+        const uint32_t here = static_cast<uint32_t>(__ballot((st & 1u) != 0u));
+        const bool care = __any((st & 2u) != 0u);
         const int key0 = tiles.tile(j) * KT;
-        if (care != 0u) {
+        const auto stage = [&] {
+            if (j + 1 < j1) {
+                put(j + 1);
+                if (j + 2 < j1) { fetch(j + 2); }
+            }
+        };
+        if (early) { stage(); }
+        if (care) {
             cared = true;
             if (threadIdx.x == 0) { marks[(j - j0) >> 5] |= 1u << ((j - j0) & 31); }
         } else {
+            u4 kf[2][D / 32];
+            const auto read_k = [&](const char* from, int chunk) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    const char* krow = from + (32 * chunk + 16 * kt + c) * 2 * D;
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k) {
+                        const int piece = BF ? 4 * k + g : 8 * (k >> 1) + 2 * g + (k & 1);
+                        kf[kt][k] = *reinterpret_cast<const u4*>(krow + 16 * (piece ^ c));
+                    }
+                }
+            };
 #pragma unroll 1
             for (int cw = 0; cw < MG::NCH / WK; ++cw) {
                 const int ci = cw * WK + wk;
@@ -1230,26 +1232,40 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
                 const uint32_t bits = D == 128 ? here >> (2 * ci) : (here >> (4 * ci) & 1u) | (here >> (4 * ci + 1) & 2u);
                 // by arithmetic: hipcc 7.2 inverted a select on a bit of a scalar here (s_bitcmp0 for s_bitcmp1)
                 const Halves hv{{static_cast<int>(bits & 1u) - 1, static_cast<int>((bits >> 1) & 1u) - 1}};
-                if (c0 > r.hi || (c0 + 31 < low && c0 >= x.a.sinks) || (hv.page[0] & hv.page[1]) < 0) { continue; }
+                if (c0 > r.hi || (c0 + 31 < low && c0 >= x.a.sinks) || (hv.page[0] & hv.page[1]) < 0) {
+                    continue;
+                }
+                read_k(buf, ci);
                 f4 sacc[2][NT];
+                __builtin_amdgcn_s_setprio(1); // products first: the SIMD's other wave fills in with its softmax
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt) {
-                    const char* krow = buf + (32 * ci + 16 * kt + c) * 2 * D;
 #pragma unroll
                     for (int k = 0; k < D / 32; ++k) {
-                        const int piece = BF ? 4 * k + g : 8 * (k >> 1) + 2 * g + (k & 1);
-                        const u4 ka = *reinterpret_cast<const u4*>(krow + 16 * (piece ^ c));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             const f4 acc = k == 0 ? f4{0.f, 0.f, 0.f, 0.f} : sacc[kt][nt];
                             if constexpr (BF) {
-                                sacc[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, ka), __builtin_bit_cast(bf8, r.q[nt][k]), acc, 0, 0, 0);
+                                sacc[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, kf[kt][k]), __builtin_bit_cast(bf8, r.q[nt][k]), acc, 0, 0, 0);
                             } else {
-                                sacc[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, ka), __builtin_bit_cast(h8, r.q[nt][k]), acc, 0, 0, 0);
+                                sacc[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, kf[kt][k]), __builtin_bit_cast(h8, r.q[nt][k]), acc, 0, 0, 0);
                             }
                         }
                     }
                 }
+                // the V^T operands are on their way while the softmax is worked out
+                const char* vp = buf + MG::kPlane + 32 * ci * 2 * D;
+                u4 vf[VF];
+                const auto read_v = [&](int t) {
+                    const int at = (voff ^ (32 * (t & 7))) + 256 * (t >> 3);
+                    const u2 a = read_tr(vp + at), b = read_tr(vp + at + 16 * 2 * D);
+                    return u4{a[0], a[1], b[0], b[1]};
+                };
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < VF; ++t) { vf[t] = read_v(t); }
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
                 float sv[NT][8];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -1292,12 +1308,11 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
                     for (int i = 0; i < 8; ++i) { p[nt][i] = static_cast<_Float16>(__builtin_amdgcn_exp2f(fmaf(sv[nt][i], mul[nt], bias))); }
                 }
-                const char* vp = buf + MG::kPlane + 32 * ci * 2 * D;
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int t = 0; t < D / 16; ++t) {
-                    const int at = (voff ^ (32 * (t & 7))) + 256 * (t >> 3);
-                    const u2 a = read_tr(vp + at), b = read_tr(vp + at + 16 * 2 * D);
-                    const u4 va = {a[0], a[1], b[0], b[1]};
+                    const u4 va = vf[t % VF];
+                    if (t + VF < D / 16) { vf[t % VF] = read_v(t + VF); }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         r.O[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, va), p[nt], r.O[nt][t], 0, 0, 0);
@@ -1306,8 +1321,10 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
                 const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) { l[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[nt], l[nt], 0, 0, 0); }
+                __builtin_amdgcn_s_setprio(0);
             }
         }
+        if (!early) { stage(); }
         __syncthreads(); // this buffer is free, the next tile is in place
     }
     const float unit_v = 1.0f / sc.v; // an exact power of two
@@ -1509,7 +1526,8 @@ PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t
                      int32_t sinks) {
     const int32_t G = Hq / Hkv;
     PagedPlan p;
-    p.nt = static_cast<int64_t>(max_new) * G <= 16 ? 1 : 2;
+    // next to sequences of many rows, those of 17 to 32 are theirs: two row tiles cost the single tokens more
+    p.nt = static_cast<int64_t>(max_new) * G <= 16 || static_cast<int64_t>(max_new) * G > 32 ? 1 : 2;
     p.few_rows = 16 * p.nt;
     const int64_t most_rows = std::min<int64_t>(max_new, tokens) * G; // of a sequence
     // the most keys that `n` tokens see
@@ -1520,7 +1538,7 @@ PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t
     size_t at = 0;
     {
         const int64_t units = (seen(std::min<int64_t>(max_new, p.few_rows)) + 127) / 128;
-        p.slots = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(kCus * few_waves(D, p.nt) / Hkv, B * units)));
+        p.slots = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(kCus * few_waves(D) / Hkv, B * units)));
         p.merge = p.slots > 1;
         if (p.merge) {
             const size_t rows = static_cast<size_t>(p.slots + B) * Hkv * p.few_rows;
