@@ -47,6 +47,7 @@ PagedRef validate_cache(const nmi_paged_kv_layer_view* cache, const std::string&
     r.D = cache->head_dim;
     r.pages = cache->k.ne[3];
     require(r.pages > 0, op, "a paged KV cache needs a page");
+    if (r.Hkv > 1024) { throw Unsupported(op + ": more than 1024 KV heads are not built"); }
     if (static_cast<int64_t>(r.Hkv) * ps * r.D * 2 >= (int64_t{1} << 31)) {
         throw Unsupported(op + ": a page of 2^31 bytes or more is not built");
     }

@@ -998,13 +998,18 @@ __device__ __forceinline__ bool stage_store(const StageRegs<D, BF>& r, const Man
 
 constexpr int kCus = 256;
 
-// Time of a key tile in us with WK = 1, 2, 4 waves per row tile: what the choices below weigh.
+// What the choices below weigh, in us on MI355X: a key tile with WK = 1, 2, 4 waves per row tile (8,192 tokens, every WK
+// forced: 802, 1,054 and 1,574 us at head_dim 128, 1,161 and 1,614 us at 256, INT8), and a workgroup besides its tiles
+// (the batch's plan, the first page, the epilogue).
 __host__ __device__ constexpr float tile_us(int D, int wk) {
-    return D == 128 ? (wk == 1 ? 4.0f : wk == 2 ? 2.4f : 1.7f) : (wk == 1 ? 2.4f : 1.7f);
+    return D == 128 ? (wk == 1 ? 4.9f : wk == 2 ? 3.2f : 2.6f) : (wk == 1 ? 2.95f : 2.05f);
 }
+constexpr float kWorkgroupUs = 8.0f;
 
-// The last `rem` row tiles x heads that do not fill the chip: key splits of each, and the time they take. A
-// workgroup costs about 4 us besides its key tiles; parts are written and read at 4 TB/s and cost a launch.
+// The last `rem` row tiles x heads that do not fill the chip: key splits of each, and the time they take. Parts are
+// written and read at 4 TB/s and cost a launch. Measured at 40/8/128 INT8: 200 tokens over 2,000 rows 39.9 us as it
+// chooses (two waves per row tile, four splits), 38.2 and 48.0 us with one and four waves; 700 over 300 rows 41.0 (two
+// waves, no splits), 51.8 and 58.5 us.
 struct Tail {
     int splits;
     float us;
@@ -1013,10 +1018,10 @@ struct Tail {
 __host__ __device__ inline Tail tail_of(int rem, int longest, float us_tile, int elements, int parts) {
     Tail best{1, 0.0f};
     if (rem <= 0) { return best; }
-    best.us = 4.0f + static_cast<float>(longest) * us_tile;
+    best.us = kWorkgroupUs + static_cast<float>(longest) * us_tile;
     for (int ns = 2; ns <= 32 && ns * rem <= parts && ns <= longest; ++ns) {
         const int rounds = (rem * ns + kCus - 1) / kCus;
-        const float us = static_cast<float>(rounds) * (4.0f + static_cast<float>((longest + ns - 1) / ns) * us_tile) + 4.0f +
+        const float us = static_cast<float>(rounds) * (kWorkgroupUs + static_cast<float>((longest + ns - 1) / ns) * us_tile) + 8.0f +
                          static_cast<float>(rem * ns) * static_cast<float>(elements) * 2.0e-6f;
         if (us < best.us) { best = Tail{ns, us}; }
     }
@@ -1530,13 +1535,15 @@ PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t
     p.nt = static_cast<int64_t>(max_new) * G <= 16 || static_cast<int64_t>(max_new) * G > 32 ? 1 : 2;
     p.few_rows = 16 * p.nt;
     const int64_t most_rows = std::min<int64_t>(max_new, tokens) * G; // of a sequence
+    // one sequence of many rows: the many-row kernel serves it, whatever its rows turn out to be (no launches for none)
+    if (B == 1 && most_rows > p.few_rows) { p.few_rows = 0; }
     // the most keys that `n` tokens see
     const auto seen = [&](int64_t n) {
         if (window == 0) { return static_cast<int64_t>(max_keys); }
         return std::min<int64_t>(max_keys, static_cast<int64_t>(window) + n + 126 + (static_cast<int64_t>(sinks) + 127) / 128 * 128);
     };
     size_t at = 0;
-    {
+    if (p.few_rows > 0) {
         const int64_t units = (seen(std::min<int64_t>(max_new, p.few_rows)) + 127) / 128;
         p.slots = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(kCus * few_waves(D) / Hkv, B * units)));
         p.merge = p.slots > 1;
@@ -1561,7 +1568,7 @@ PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t
             const int64_t tiles = rows / bm + seqs;
             const int32_t parts = static_cast<int32_t>(std::min<int64_t>((1 << 23) / (bm * D), longest > 1 ? tiles * Hkv * 32 : 0));
             const int64_t units = (rows + bm - 1) / bm * Hkv; // as if one sequence had them
-            const double us = static_cast<double>(units / kCus) * (4.0 + mean * tile_us(D, wk)) +
+            const double us = static_cast<double>(units / kCus) * (kWorkgroupUs + mean * tile_us(D, wk)) +
                               tail_of(static_cast<int>(units % kCus), longest, tile_us(D, wk), bm * D, parts).us;
             if (us < best) {
                 best = us;

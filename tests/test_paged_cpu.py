@@ -59,6 +59,8 @@ BAD_VIEWS = {
     "table stride": (dict(page_table=T(na.I32, 4, 3, nb={1: 12})), ValueError),
     "table too long": (dict(max_pages=1 << 28), OverflowError),
     "batch": (dict(B=1025), NotImplementedError),
+    "heads": (dict(H=1025), NotImplementedError),
+    "page of 2 GiB": (dict(H=1024, page=4096, D=256), NotImplementedError),
     "bf16 with scales": (dict(kv="bf16", k_scale=T(na.FP16, 2, 16, 2, 8)), ValueError),
     "bf16 with a group": (dict(kv="bf16", quant_group=64), ValueError),
 }
