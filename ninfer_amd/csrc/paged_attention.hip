@@ -56,6 +56,11 @@ __device__ __forceinline__ Seq sequence(const PagedAttnArgs& x, int b) {
     return s;
 }
 
+// Lane `at`'s sequence, for the whole wave.
+__device__ __forceinline__ Seq lane_seq(const Seq& s, int at) {
+    return Seq{__builtin_amdgcn_readlane(s.start, at), __builtin_amdgcn_readlane(s.tokens, at), __builtin_amdgcn_readlane(s.history, at)};
+}
+
 // The tiles (of 2^lg keys) that tokens at positions p0 .. p1 need: [0, sink) and [first, end) of the sequence's tiles,
 // numbered on without the gap.
 struct Tiles {
@@ -536,10 +541,10 @@ constexpr int kFewThreads = 64 * kFewWaves;
 constexpr int kUnit = 4; // tiles of a unit: one for each wave
 
 // The units of sequence b's keys that the few-row kernel walks (0: not its sequence).
-__device__ __forceinline__ int few_units(const PagedAttnArgs& x, int b, Seq& s, Tiles& t) {
+__device__ __forceinline__ int few_units(const PagedAttnArgs& x, int b, Seq& s) {
     s = sequence(x, b);
     if (s.tokens == 0 || s.tokens * x.G > x.few_rows) { return 0; }
-    t = tiles_of(x, s.history, s.history + s.tokens - 1, 5);
+    const Tiles t = tiles_of(x, s.history, s.history + s.tokens - 1, 5);
     return (t.count + kUnit - 1) / kUnit;
 }
 
@@ -559,19 +564,19 @@ struct FewSeq {
     int rank;
     int first; // its first unit
     int units;
+    Seq s;
 };
 
 // The sequences 64 at a time, spread over the lanes of a wave: units and their inclusive sums.
 struct FewLanes {
     int units;
     int end;
+    Seq s;
 };
 
 __device__ __forceinline__ FewLanes few_lanes(const PagedAttnArgs& x, int base, int sum, int lane) {
-    Seq s;
-    Tiles t;
-    FewLanes f;
-    f.units = base + lane < x.c.B ? few_units(x, base + lane, s, t) : 0;
+    FewLanes f{};
+    if (base + lane < x.c.B) { f.units = few_units(x, base + lane, f.s); }
     f.end = sum + wave_inclusive_scan(f.units);
     return f;
 }
@@ -588,7 +593,7 @@ __device__ __forceinline__ FewPlan few_plan(const PagedAttnArgs& x, int lane, Fe
 
 // The sequence that holds `unit`. `f`: the lanes of the only 64 sequences where there are no more.
 __device__ __forceinline__ FewSeq few_find(const PagedAttnArgs& x, int unit, int lane, FewLanes f) {
-    FewSeq q{-1, 0, 0, 0};
+    FewSeq q{-1, 0, 0, 0, {}};
     int sum = 0;
     for (int base = 0; base < x.c.B; base += 64) {
         if (x.c.B > 64) { f = few_lanes(x, base, sum, lane); }
@@ -600,6 +605,7 @@ __device__ __forceinline__ FewSeq few_find(const PagedAttnArgs& x, int unit, int
             q.rank += __popcll(some & ((uint64_t{1} << at) - 1));
             q.units = __builtin_amdgcn_readlane(f.units, at);
             q.first = __builtin_amdgcn_readlane(f.end, at) - q.units;
+            q.s = lane_seq(f.s, at);
             return q;
         }
         q.rank += __popcll(some);
@@ -669,7 +675,7 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const Seq s = sequence(x, q.b);
+    const Seq s = q.s;
     const Tiles tiles = tiles_of(x, s.history, s.history + s.tokens - 1, 5);
     const int t0 = min(u0 * kUnit, tiles.count), t1 = min(u1 * kUnit, tiles.count);
     const int each = (t1 - t0 + kFewWaves - 1) / kFewWaves;
@@ -794,47 +800,6 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
         u = next;
     }
 }
-// Log-sum-exp merge of a row's splits: a workgroup per row, groups of D / 4 threads taking every group-th split.
-template <int D>
-__global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs x, int slot_rows) {
-    constexpr int TPR = D / 4, GRP = 256 / TPR;
-    __shared__ f4 xo[GRP][TPR];
-    __shared__ float2 xm[GRP];
-    const int b = blockIdx.y;
-    const int row = blockIdx.x / x.c.Hkv;
-    const int h = blockIdx.x % x.c.Hkv;
-    const Seq s = sequence(x, b);
-    const int rows = s.tokens * x.G;
-    if (rows > x.few_rows || row >= rows) { return; }
-    const int first = x.seq_table[2 * b], splits = x.seq_table[2 * b + 1];
-    if (splits == 1) { return; } // written already
-    const int grp = threadIdx.x / TPR, d = 4 * (threadIdx.x % TPR);
-    float M = -INFINITY, L = 0.0f;
-    f4 O = {0.f, 0.f, 0.f, 0.f};
-    const auto add = [&](float m, float l, f4 o) {
-        const Weights w = weights(M, L, m, l);
-        L = L * w.a + l * w.b;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { O[e] = (w.a == 0.0f ? 0.0f : O[e] * w.a) + (w.b == 0.0f ? 0.0f : o[e] * w.b); }
-        M = w.M;
-    };
-#pragma unroll 4
-    for (int k = grp; k < splits; k += GRP) {
-        const int64_t at = (static_cast<int64_t>(first + k) * x.c.Hkv + h) * slot_rows + row;
-        const float2 ml = *reinterpret_cast<const float2*>(x.part_ml + 2 * at);
-        add(ml.x, ml.y, *reinterpret_cast<const f4*>(x.part_o + at * D + d));
-    }
-    xo[grp][threadIdx.x % TPR] = O;
-    if (threadIdx.x % TPR == 0) { xm[grp] = float2{M, L}; }
-    __syncthreads();
-    if (grp != 0) { return; }
-#pragma unroll
-    for (int k = 1; k < GRP; ++k) { add(xm[k].x, xm[k].y, xo[k][threadIdx.x]); }
-    const int t = row / x.G;
-    uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + (s.start + t) * x.a.out.token_stride) + (h * x.G + row - t * x.G) * D + d;
-    *reinterpret_cast<u2*>(out) = out_pair(O, L);
-}
-
 // ---- many rows: tiles of query rows over key tiles that a workgroup decodes once ------------------
 //
 // A workgroup of 8 waves owns a tile of query rows of one (sequence, KV head): WR row waves of 16 NT rows, each
@@ -1028,6 +993,24 @@ __host__ __device__ inline Tail tail_of(int rem, int longest, float us_tile, int
     return best;
 }
 
+// The row tiles of 64 sequences, spread over the lanes of a wave: their numbers and inclusive sums.
+struct ManyLanes {
+    int n;
+    int end;
+    Seq s;
+};
+
+__device__ __forceinline__ ManyLanes many_lanes(const PagedAttnArgs& x, int base, int sum, int bm, int lane) {
+    ManyLanes f{};
+    if (base + lane < x.c.B) {
+        f.s = sequence(x, base + lane);
+        const int rows = f.s.tokens * x.G;
+        f.n = rows > x.few_rows ? (rows + bm - 1) / bm : 0;
+    }
+    f.end = sum + wave_inclusive_scan(f.n);
+    return f;
+}
+
 // Row tiles x heads of the batch: the first `full` fill the chip's rounds, each of the others has `splits` workgroups.
 struct ManyPlan {
     int units;
@@ -1036,21 +1019,17 @@ struct ManyPlan {
 };
 
 template <int D, int WK>
-__device__ __forceinline__ ManyPlan many_plan(const PagedAttnArgs& x, int lane) {
+__device__ __forceinline__ ManyPlan many_plan(const PagedAttnArgs& x, int lane, ManyLanes& f) {
     constexpr int BM = ManyGeo<D, WK>::BM;
     int total = 0, longest = 0;
     for (int base = 0; base < x.c.B; base += 64) {
-        int n = 0, len = 0;
-        if (base + lane < x.c.B) {
-            const Seq s = sequence(x, base + lane);
-            const int rows = s.tokens * x.G;
-            if (rows > x.few_rows) {
-                n = (rows + BM - 1) / BM;
-                const int last = s.history + s.tokens - 1;
-                len = tiles_of(x, max(s.history, last - (BM - 1) / x.G), last, ManyGeo<D, WK>::LG).count;
-            }
+        f = many_lanes(x, base, total, BM, lane);
+        int len = 0;
+        if (f.n > 0) {
+            const int last = f.s.history + f.s.tokens - 1;
+            len = tiles_of(x, max(f.s.history, last - (BM - 1) / x.G), last, ManyGeo<D, WK>::LG).count;
         }
-        total += __builtin_amdgcn_readlane(wave_inclusive_scan(n), 63);
+        total = __builtin_amdgcn_readlane(f.end, 63);
         longest = max(longest, static_cast<int>(wave_max(static_cast<float>(len))));
     }
     ManyPlan p{total * x.c.Hkv, 0, 1};
@@ -1063,29 +1042,26 @@ __device__ __forceinline__ ManyPlan many_plan(const PagedAttnArgs& x, int lane) 
 struct ManyWork {
     int b; // -1: none
     int tile;
+    Seq s;
 };
 
-// The sequences' row tiles in order; `slot` counts them over the batch.
-__device__ __forceinline__ ManyWork many_work(const PagedAttnArgs& x, int slot, int bm, int lane) {
-    ManyWork w{-1, 0};
+// The sequences' row tiles in order; `slot` counts them over the batch. `f`: the lanes of the only 64 sequences where
+// there are no more.
+__device__ __forceinline__ ManyWork many_work(const PagedAttnArgs& x, int slot, int bm, int lane, ManyLanes f) {
+    ManyWork w{-1, 0, {}};
     int sum = 0;
     for (int base = 0; base < x.c.B; base += 64) {
-        int n = 0;
-        if (base + lane < x.c.B) {
-            const Seq s = sequence(x, base + lane);
-            const int rows = s.tokens * x.G;
-            n = rows > x.few_rows ? (rows + bm - 1) / bm : 0;
-        }
-        const int end = sum + wave_inclusive_scan(n);
-        const uint64_t mine = __ballot(n > 0 && slot >= end - n && slot < end);
+        if (x.c.B > 64) { f = many_lanes(x, base, sum, bm, lane); }
+        const uint64_t mine = __ballot(f.n > 0 && slot >= f.end - f.n && slot < f.end);
         if (mine != 0u) {
             const int at = __ffsll(static_cast<long long>(mine)) - 1;
             w.b = base + at;
             // the last tokens see the most keys: their tiles first
-            w.tile = __builtin_amdgcn_readlane(end, at) - 1 - slot;
+            w.tile = __builtin_amdgcn_readlane(f.end, at) - 1 - slot;
+            w.s = lane_seq(f.s, at);
             return w;
         }
-        sum = __builtin_amdgcn_readlane(end, 63);
+        sum = __builtin_amdgcn_readlane(f.end, 63);
     }
     return w;
 }
@@ -1109,16 +1085,17 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int wr = wave / WK, wk = wave % WK;
-    const ManyPlan plan = many_plan<D, WK>(x, lane);
+    ManyLanes lanes;
+    const ManyPlan plan = many_plan<D, WK>(x, lane, lanes);
     const int id = blockIdx.x;
     const int unit = id < plan.full ? id : plan.full + (id - plan.full) / plan.splits;
     const int splits = id < plan.full ? 1 : plan.splits;
     const int split = id < plan.full ? 0 : (id - plan.full) % plan.splits;
     if (unit >= plan.units) { return; }
     const int h = unit % x.c.Hkv;
-    const ManyWork w = many_work(x, unit / x.c.Hkv, MG::BM, lane);
+    const ManyWork w = many_work(x, unit / x.c.Hkv, MG::BM, lane, lanes);
     if (w.b < 0) { return; }
-    const Seq s = sequence(x, w.b);
+    const Seq s = w.s;
     const int rows = s.tokens * x.G;
     const int r0 = w.tile * MG::BM;
     const int p0 = s.history + r0 / x.G, p1 = s.history + (min(r0 + MG::BM, rows) - 1) / x.G;
@@ -1469,40 +1446,94 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
     }
 }
 
-// The parts of the split row tiles: D / 4 threads per row.
-template <int D, int WK>
-__global__ __launch_bounds__(256) void paged_attn_many_merge_kernel(PagedAttnArgs x) {
-    constexpr int TPR = D / 4, RPB = 256 / TPR, BM = ManyGeo<D, WK>::BM;
-    const int lane = threadIdx.x & 63;
-    const ManyPlan plan = many_plan<D, WK>(x, lane);
-    const int tail = blockIdx.x / (BM / RPB);
-    if (plan.full + tail >= plan.units) { return; }
-    const int unit = plan.full + tail;
-    const int h = unit % x.c.Hkv;
-    const int rr = blockIdx.x % (BM / RPB) * RPB + threadIdx.x / TPR;
-    const ManyWork w = many_work(x, unit / x.c.Hkv, BM, lane);
-    if (w.b < 0) { return; }
-    const Seq s = sequence(x, w.b);
-    const int row = w.tile * BM + rr;
-    if (row >= s.tokens * x.G) { return; }
-    const int d = 4 * (threadIdx.x % TPR);
+// ---- the parts of a row, one after another in the workspace ----------------------------------------
+//
+// One launch for both kernels' parts. Few rows: a workgroup per row and sequence, groups of D / 4 threads taking every
+// group-th part, joined through LDS. Many rows: D / 4 threads per row of a split row tile.
+
+template <int D>
+__device__ __forceinline__ void store_row(const PagedAttnArgs& x, const Seq& s, int h, int row, int d, f4 O, float L) {
+    const int t = row / x.G;
+    uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + (s.start + t) * x.a.out.token_stride) + (h * x.G + row - t * x.G) * D + d;
+    *reinterpret_cast<u2*>(out) = out_pair(O, L);
+}
+
+struct Merge {
     float M = -INFINITY, L = 0.0f;
     f4 O = {0.f, 0.f, 0.f, 0.f};
+    __device__ __forceinline__ void add(float m, float l, f4 o) {
+        const Weights w = weights(M, L, m, l);
+        L = L * w.a + l * w.b;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { O[e] = (w.a == 0.0f ? 0.0f : O[e] * w.a) + (w.b == 0.0f ? 0.0f : o[e] * w.b); }
+        M = w.M;
+    }
+};
+
+template <int D>
+__device__ __forceinline__ void merge_few(const PagedAttnArgs& x, int block) {
+    constexpr int TPR = D / 4, GRP = 256 / TPR;
+    __shared__ f4 xo[GRP][TPR];
+    __shared__ float2 xm[GRP];
+    const int h = block % x.c.Hkv;
+    const int row = block / x.c.Hkv % x.few_rows;
+    const int b = block / x.c.Hkv / x.few_rows;
+    const int first = x.seq_table[2 * b], splits = x.seq_table[2 * b + 1]; // of a sequence of the kernel's only
+    const Seq s = sequence(x, b);
+    const int rows = s.tokens * x.G;
+    if (rows > x.few_rows || row >= rows || splits == 1) { return; } // one part is written already
+    const int grp = threadIdx.x / TPR, d = 4 * (threadIdx.x % TPR);
+    Merge m;
+#pragma unroll 4
+    for (int k = grp; k < splits; k += GRP) {
+        const int64_t at = (static_cast<int64_t>(first + k) * x.c.Hkv + h) * x.few_rows + row;
+        const float2 ml = *reinterpret_cast<const float2*>(x.part_ml + 2 * at);
+        m.add(ml.x, ml.y, *reinterpret_cast<const f4*>(x.part_o + at * D + d));
+    }
+    xo[grp][threadIdx.x % TPR] = m.O;
+    if (threadIdx.x % TPR == 0) { xm[grp] = float2{m.M, m.L}; }
+    __syncthreads();
+    if (grp != 0) { return; }
+#pragma unroll
+    for (int k = 1; k < GRP; ++k) { m.add(xm[k].x, xm[k].y, xo[k][threadIdx.x]); }
+    store_row<D>(x, s, h, row, d, m.O, m.L);
+}
+
+template <int D, int WK>
+__device__ __forceinline__ void merge_many(const PagedAttnArgs& x, int block) {
+    constexpr int TPR = D / 4, RPB = 256 / TPR, BM = ManyGeo<D, WK>::BM;
+    const int lane = threadIdx.x & 63;
+    ManyLanes lanes;
+    const ManyPlan plan = many_plan<D, WK>(x, lane, lanes);
+    const int tail = block / (BM / RPB);
+    const int unit = plan.full + tail;
+    if (unit >= plan.units) { return; }
+    const int h = unit % x.c.Hkv;
+    const int rr = block % (BM / RPB) * RPB + threadIdx.x / TPR;
+    const ManyWork w = many_work(x, unit / x.c.Hkv, BM, lane, lanes);
+    if (w.b < 0) { return; }
+    const int row = w.tile * BM + rr;
+    if (row >= w.s.tokens * x.G) { return; }
+    const int d = 4 * (threadIdx.x % TPR);
     const int64_t first = static_cast<int64_t>(tail) * plan.splits * BM + rr;
+    Merge m;
 #pragma unroll 4
     for (int k = 0; k < plan.splits; ++k) {
         const int64_t at = first + static_cast<int64_t>(k) * BM;
         const float2 ml = *reinterpret_cast<const float2*>(x.many_ml + 2 * at);
-        const f4 o = *reinterpret_cast<const f4*>(x.many_o + at * D + d);
-        const Weights q = weights(M, L, ml.x, ml.y);
-        L = L * q.a + ml.y * q.b;
-        M = q.M;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { O[e] = (q.a == 0.0f ? 0.0f : O[e] * q.a) + (q.b == 0.0f ? 0.0f : o[e] * q.b); }
+        m.add(ml.x, ml.y, *reinterpret_cast<const f4*>(x.many_o + at * D + d));
     }
-    const int t = row / x.G;
-    uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + (s.start + t) * x.a.out.token_stride) + (h * x.G + row - t * x.G) * D + d;
-    *reinterpret_cast<u2*>(out) = out_pair(O, L);
+    store_row<D>(x, w.s, h, row, d, m.O, m.L);
+}
+
+// The first `few` workgroups merge the few-row kernel's parts, the others the many-row kernel's.
+template <int D, int WK>
+__global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs x, int few) {
+    if (static_cast<int>(blockIdx.x) < few) {
+        merge_few<D>(x, blockIdx.x);
+    } else {
+        merge_many<D, WK>(x, blockIdx.x - few);
+    }
 }
 
 } // namespace
@@ -1588,8 +1619,9 @@ PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t
     return p;
 }
 
-template <int D, bool BF>
-void launch(PagedAttnArgs& x, const PagedPlan& p, hipStream_t stream) {
+template <int D, bool BF, int WK>
+void launch(const PagedAttnArgs& x, const PagedPlan& p, hipStream_t stream) {
+    uint32_t few = 0, tails = 0; // workgroups of the merge
     if (p.slots > 0) {
         const uint32_t grid = static_cast<uint32_t>(p.slots) * x.c.Hkv;
         if (p.nt == 1) {
@@ -1598,31 +1630,29 @@ void launch(PagedAttnArgs& x, const PagedPlan& p, hipStream_t stream) {
             hipLaunchKernelGGL((paged_attn_few_kernel<D, BF, 2>), dim3(grid), dim3(kFewThreads), 0, stream, x);
         }
         check_launch("paged_attn_few_kernel");
-        if (p.merge) {
-            hipLaunchKernelGGL((paged_attn_merge_kernel<D>), dim3(p.few_rows * x.c.Hkv, x.c.B), dim3(256), 0, stream, x, p.few_rows);
-            check_launch("paged_attn_merge_kernel");
-        }
+        if (p.merge) { few = static_cast<uint32_t>(p.few_rows) * x.c.Hkv * x.c.B; }
     }
-    if (p.tiles == 0) { return; }
-    const int64_t blocks = static_cast<int64_t>(p.tiles) * x.c.Hkv;
-    if (blocks > 0x7FFFFF) { throw Unsupported("paged attention: more than 2^23 workgroups are not built"); }
-    const dim3 grid(static_cast<uint32_t>(blocks) + p.parts);
-    const uint32_t tails = static_cast<uint32_t>(std::min<int64_t>(blocks, kCus - 1)); // units that may be split
-    const auto go = [&](auto wkc) {
-        constexpr int WK = decltype(wkc)::value;
-        hipLaunchKernelGGL((paged_attn_many_kernel<D, BF, WK>), grid, dim3(kManyThreads), 0, stream, x);
+    if (p.tiles > 0) {
+        const int64_t blocks = static_cast<int64_t>(p.tiles) * x.c.Hkv;
+        if (blocks > 0x7FFFFF) { throw Unsupported("paged attention: more than 2^23 workgroups are not built"); }
+        hipLaunchKernelGGL((paged_attn_many_kernel<D, BF, WK>), dim3(static_cast<uint32_t>(blocks) + p.parts), dim3(kManyThreads), 0, stream, x);
         check_launch("paged_attn_many_kernel");
-        if (p.parts > 0) {
-            hipLaunchKernelGGL((paged_attn_many_merge_kernel<D, WK>), dim3(tails * (ManyGeo<D, WK>::BM / (1024 / D))), dim3(256), 0, stream, x);
-            check_launch("paged_attn_many_merge_kernel");
-        }
-    };
+        // the row tiles that may be split
+        if (p.parts > 0) { tails = static_cast<uint32_t>(std::min<int64_t>(blocks, kCus - 1)) * (ManyGeo<D, WK>::BM / (1024 / D)); }
+    }
+    if (few + tails == 0) { return; }
+    hipLaunchKernelGGL((paged_attn_merge_kernel<D, WK>), dim3(few + tails), dim3(256), 0, stream, x, static_cast<int>(few));
+    check_launch("paged_attn_merge_kernel");
+}
+
+template <int D, bool BF>
+void launch(const PagedAttnArgs& x, const PagedPlan& p, hipStream_t stream) {
     if (p.wk == 1) {
-        go(std::integral_constant<int, 1>{});
+        launch<D, BF, 1>(x, p, stream);
     } else if (p.wk == 2) {
-        go(std::integral_constant<int, 2>{});
+        launch<D, BF, 2>(x, p, stream);
     } else if constexpr (D == 128) {
-        go(std::integral_constant<int, 4>{});
+        launch<D, BF, 4>(x, p, stream);
     }
 }
 
