@@ -115,6 +115,34 @@ struct CyclicKVCacheLayerView {
     }
 };
 
+// Extension: K/V of many sequences in pages of a pool (nmi_paged_kv_layer_view). `k`, `v` and the scales are
+// [.., page_size, Hkv, pages], page_table I32 [max_pages, B].
+struct PagedKVCacheLayerView {
+    Tensor k, v, k_scale, v_scale, page_table;
+    int32_t page_size = 0;
+    int32_t num_kv_heads = 0;
+    int32_t head_dim = 0;
+    DType dtype = DType::BF16;
+    int32_t quant_group = 0;
+
+    nmi_paged_kv_layer_view c() const {
+        nmi_paged_kv_layer_view r{};
+        r.k = k.c();
+        r.v = v.c();
+        r.k_scale = k_scale.c();
+        r.v_scale = v_scale.c();
+        r.page_table = page_table.c();
+        r.page_size = page_size;
+        r.num_kv_heads = num_kv_heads;
+        r.head_dim = head_dim;
+        r.dtype = static_cast<int32_t>(dtype);
+        r.quant_group = quant_group;
+        return r;
+    }
+};
+
+using PagedExecutionEnvelope = nmi_paged_envelope;
+using AttentionWindow = nmi_attention_window;
 using GqaExecutionEnvelope = nmi_gqa_envelope;
 using KVCacheAppendPrefixExecutionEnvelope = nmi_commit_envelope;
 using SamplingConfig = nmi_sampling_config; // same 40-byte device layout as the reference
@@ -349,6 +377,45 @@ inline void tree_accept_greedy(const Tensor& parents, const Tensor& node_tokens,
                cns = num_sampled.c(), cacc = accepted.c(), cst = stats.c();
     detail::check(nmi_tree_accept_greedy(&cpar, &cnt, &ctt, &cpath, &cpl, &clen, &ctok, &cso, &cns, &cacc, &cst,
                                          detail::st(stream)));
+}
+
+// ---- paged cache (extension) ------------------------------------------------------------------------
+
+// Token i of sequence b (starts[b] + i of the packed k/v) to row history[b] + i of its pages.
+inline void paged_kv_append(const Tensor& k, const Tensor& v, const Tensor& starts, const Tensor& history,
+                            const PagedKVCacheLayerView& cache, hipStream_t stream) {
+    const nmi_tensor ck = k.c(), cv = v.c(), cs = starts.c(), ch = history.c();
+    const nmi_paged_kv_layer_view view = cache.c();
+    detail::check(nmi_paged_kv_append(&ck, &cv, &cs, &ch, &view, detail::st(stream)));
+}
+
+// Row first[b] + i of sequence b to token starts[b] + i of k_out/v_out (BF16 or FP32).
+inline void paged_kv_read(const PagedKVCacheLayerView& cache, const Tensor& starts, const Tensor& first, Tensor& k_out,
+                          Tensor& v_out, hipStream_t stream) {
+    const nmi_tensor cs = starts.c(), cf = first.c();
+    nmi_tensor ck = k_out.c(), cv = v_out.c();
+    const nmi_paged_kv_layer_view view = cache.c();
+    detail::check(nmi_paged_kv_read(&view, &cs, &cf, &ck, &cv, detail::st(stream)));
+}
+
+[[nodiscard]] inline std::size_t paged_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                                                 int32_t tokens, int32_t batch, PagedExecutionEnvelope envelope,
+                                                                 AttentionWindow window) {
+    return nmi_paged_attention_workspace_bytes(q_heads, kv_heads, head_dim, tokens, batch, envelope, window);
+}
+
+// Causal attention of the packed new tokens over their pages, which hold the new rows already.
+inline void paged_attention(const Tensor& q, const Tensor& starts, const Tensor& history, float scale, AttentionWindow window,
+                            const PagedKVCacheLayerView& cache, PagedExecutionEnvelope envelope, WorkspaceArena& workspace,
+                            Tensor& out, hipStream_t stream) {
+    auto scope = workspace.scope();
+    const std::size_t need = paged_attention_workspace_bytes(q.ne[1], cache.num_kv_heads, q.ne[0], q.ne[2],
+                                                             cache.page_table.ne[1], envelope, window);
+    void* ws = need ? workspace.alloc_bytes(need) : nullptr;
+    const nmi_tensor cq = q.c(), cs = starts.c(), ch = history.c();
+    nmi_tensor co = out.c();
+    const nmi_paged_kv_layer_view view = cache.c();
+    detail::check(nmi_paged_attention(&cq, &cs, &ch, scale, window, &view, envelope, ws, need, &co, detail::st(stream)));
 }
 
 // ---- lm_head ----------------------------------------------------------------------------------------

@@ -354,7 +354,7 @@ const char* nmi_build_info(void) {
            "verify_attn_merge (B = 1) and verify_attn_merge_rows (batches), kv_quant_append, bf16_kv_append, argmax, speculative accept (greedy, top-20 "
            "stochastic, general fixed-point), kv commit/rollback/compaction, gdn_recurrent<{16,32,64,128}> "
            "(snapshot), conv1d_silu (snapshot), device scalars, linear_q6<{4,8,16} cols> f16-MFMA (Q6G64 lm_head, "
-           "fused argmax)";
+           "fused argmax), paged KV rows (append, read back), paged_attn_few<{1,2},{128,256}> and paged_attn_many<{1,2,4},{128,256}> (INT8-G64 and BF16)";
 }
 
 size_t nmi_gqa_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,

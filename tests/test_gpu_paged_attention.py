@@ -118,6 +118,56 @@ def test_infinite_and_nan_values_reach_only_rows_that_see_them(gpu, kv, tokens):
 
 
 @pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("tokens", [1, 3, 90])
+def test_rows_behind_the_window_hold_anything(gpu, kv, tokens):
+    """Rows between the sinks and the window, and new rows that their own token no longer counts for: infinite and NaN
+    keys and values there change nothing for the tokens that do not see them."""
+    h, w, s = 700, 64, 5
+
+    def edit(c):
+        for r, bits in ((5, 0x7F80), (40, 0x7FC0), (h + 1 - w - 1, 0xFF80), (h + 1 - w - 20, 0x7FC0)):
+            c.k[0][r] = bits
+            c.v[0][r] = bits
+    c = PagedCase([(tokens, h)], Hq=8, Hkv=2, kv=kv, window=w, sinks=s, seed=22, edit=edit)
+    d = c.upload()
+    d.attend()
+    ref, tol = PagedCase([(tokens, h)], Hq=8, Hkv=2, kv=kv, window=w, sinks=s, seed=22).oracle()
+    g = bf16_values(d.result()).astype(np.float64)
+    assert (np.abs(g - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("kv", CACHES)
+def test_graphs_that_share_a_workspace(gpu, kv):
+    """Two captured calls of different batches with one workspace, replayed in turn on one stream, eager calls between."""
+    cases = [PagedCase([(1, 1500), (1, 300), (4, 900)], Hq=40, Hkv=8, kv=kv, seed=23), PagedCase([(100, 700), (1, 2000)], Hq=40, Hkv=8, kv=kv, seed=24)]
+    devs = [c.upload() for c in cases]
+    stream = Stream()
+    need = max(ops.paged_attention_workspace_bytes(c.Hq, c.Hkv, c.D, c.N, c.B, c.envelope()) for c in cases)
+    ws = DeviceBuffer(need)
+    ws.fill(0xFF)
+    graphs = []
+    for d in devs:
+        with Graph(stream) as g:
+            d.attend(ws=ws, stream=stream)
+        graphs.append(g)
+    first = []
+    for turn in range(3):
+        for i, (c, d, g) in enumerate(zip(cases, devs, graphs)):
+            d.out.buf.fill(0xCD)
+            synchronize()
+            g.launch()
+            stream.synchronize()
+            got = d.result()
+            if turn == 0:
+                check_attention(c, got)
+                first.append(got)
+            assert np.array_equal(got, first[i])
+            d.attend(ws=ws, stream=stream)
+            stream.synchronize()
+            assert np.array_equal(d.result(), first[i])
+
+
+@pytest.mark.parametrize("kv", CACHES)
 @pytest.mark.parametrize("tokens", [1, 90])
 @pytest.mark.parametrize("size", [1e-6, 1e-3, 1e3, 3e4, 2e5])
 def test_range_of_values(gpu, kv, tokens, size):
