@@ -656,8 +656,8 @@ __device__ __forceinline__ void few_walk(const PagedAttnArgs& x, int h, const Se
 #pragma unroll 1
     for (int j = j0; j < j1; ++j) {
         chunk_probs<D, BF, NT>(x, tiles.tile(j), ha, g, ka, r, pr);
+        const Halves hb = halves(j + 1); // before the refill: tile 31 of a fetch is still in it
         if (((j - j0) & 1) == 0) { refill(j); }
-        const Halves hb = halves(j + 1);
         __builtin_amdgcn_sched_barrier(0);
         load_keys<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, ka);
         __builtin_amdgcn_sched_barrier(0);

@@ -230,6 +230,57 @@ def test_growing_scores(gpu, kv):
     _run(PagedCase([(1, 3000), (80, 900)], Hq=8, Hkv=2, kv=kv, seed=12, edit=edit))
 
 
+@pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("Hq,Hkv,D,tokens,rows", [(64, 64, 128, 1, 72000), (40, 8, 128, 1, 400000), (24, 4, 256, 1, 300000), (48, 8, 256, 4, 300000),
+                                                  (40, 8, 128, 100, 600000), (24, 4, 256, 60, 500000)])
+def test_long_walks_over_shared_pages(gpu, kv, Hq, Hkv, D, tokens, rows):
+    """Every workgroup walks more tiles than one fetch of the page table holds. The history is a few pages that appear
+    again and again in the table (a row of them counts as often), so the 64-bit result needs those rows only. One page
+    appears once, at a hundred places in turn, and most of the weight is on it."""
+    page, shared = 64, 13
+    n = rows // page
+
+    def edit(c):
+        c.q[:, :, 1] = bf16_bits(np.float32(8.0))
+        c.k[0][:, :, 1] = bf16_bits(np.float32(0.0))
+        c.k[0][(shared - 1) * page:shared * page, :, 1] = bf16_bits(np.float32(18.0))  # scores 9 to 13 above the others
+    c = PagedCase([(tokens, shared * page + 37)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, page=page, seed=25, spare=0, edit=edit)
+    r = np.random.default_rng(26)
+    order = np.concatenate([np.arange(shared), r.integers(0, shared - 1, n - shared)])
+    own = c.table[0, shared:].copy()  # the last pages: some history, the new rows
+    names = c.table[0, :shared].copy()
+    planes = c.planes()
+    K, V = c.stored(0)
+    h = c.seqs[0][1]
+    c.table, c.max_pages = np.concatenate([names[order], own])[None].astype(np.int32), n + len(own)
+    d = c.upload(planes)
+    d.history.upload(np.array([h + (n - shared) * page], np.int32))
+    env = (tokens, c.max_pages * page)
+    ws = d.workspace(env)
+    G = Hq // Hkv
+    q = bf16_values(c.q).astype(np.float64).reshape(tokens, Hkv, G, D)
+    see = np.arange(h + tokens)[None] <= (h + np.arange(tokens))[:, None]
+    heads = (0, Hkv - 1)
+    sc = [np.where(see[:, None], (q[:, hh] @ K[:, hh].T) * c.scale, -np.inf) for hh in heads]
+    size = [np.where(see[:, None], np.abs(q[:, hh]) @ np.abs(K[:, hh]).T * c.scale, 0.0).max(-1, keepdims=True) * 2.0**-11 for hh in heads]
+    for place in r.integers(0, n, 100):
+        at = order.copy()
+        at[at == shared - 1] = 0
+        at[place] = shared - 1
+        d.table.upload(np.concatenate([names[at], own])[None].astype(np.int32))
+        d.attend(envelope=env, ws=ws)
+        got = bf16_values(d.result()).astype(np.float64)
+        weight = np.ones(h + tokens)
+        weight[:shared * page] = np.repeat(np.bincount(at, minlength=shared), page)
+        for hh, s, e in zip(heads, sc, size):
+            p = np.exp(s - s.max(-1, keepdims=True)) * weight
+            p /= p.sum(-1, keepdims=True)
+            o, A = p @ V[:, hh], p @ np.abs(V[:, hh])
+            # as in PagedCase.oracle; the sums of this many rows in 32 bits add 2^-16 of the terms
+            tol = 2.0**-8 * np.abs(o) + A * (2 * np.expm1(2 * e) + 2.0**-10 + 2.0**-16)
+            assert (np.abs(got[:, hh * G:(hh + 1) * G] - o) <= tol).all(), f"the page at place {place} of {n}"
+
+
 def test_sequences_outside_the_envelope_are_left_out(gpu):
     c = PagedCase([(1, 40), (5, 100), (1, 600), (2, 30)], Hq=8, Hkv=2, seed=13)
     d = c.upload()
