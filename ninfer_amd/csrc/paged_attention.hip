@@ -19,6 +19,7 @@
 #include "paged_internal.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 namespace nmi {
 namespace {
@@ -536,8 +537,6 @@ __device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const P
 
 // ---- few rows: splits of the keys over workgroups and waves --------------------------------------
 
-constexpr int kFewWaves = 4;
-constexpr int kFewThreads = 64 * kFewWaves;
 constexpr int kUnit = 4; // tiles of a unit: one for each wave
 
 // The units of sequence b's keys that the few-row kernel walks (0: not its sequence).
@@ -669,20 +668,20 @@ __device__ __forceinline__ void few_walk(const PagedAttnArgs& x, int h, const Se
 }
 
 // Units [u0, u1) of sequence q: the part goes to its slot, or, where it is the whole sequence, to the output.
-template <int D, bool BF, int NT>
+template <int D, bool BF, int NT, int NW>
 __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const FewSeq& q, const FewPlan& plan, int share, int u0, int u1,
-                                         f4 (&xo)[2][NT * (D / 16) * 64], float2 (&xm)[2][NT * 64]) {
+                                         f4 (&xo)[NW / 2][NT * (D / 16) * 64], float2 (&xm)[NW / 2][NT * 64]) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const Seq s = q.s;
     const Tiles tiles = tiles_of(x, s.history, s.history + s.tokens - 1, 5);
     const int t0 = min(u0 * kUnit, tiles.count), t1 = min(u1 * kUnit, tiles.count);
-    const int each = (t1 - t0 + kFewWaves - 1) / kFewWaves;
+    const int each = (t1 - t0 + NW - 1) / NW;
     const int j0 = min(t0 + wave * each, t1), j1 = min(j0 + each, t1);
     const int rows = s.tokens * x.G;
     const int head = plan.share_of(q.first), splits = plan.share_of(q.first + q.units - 1) - head + 1;
-    if (u0 == 0 && h == 0 && threadIdx.x == 0) {
+    if (x.seq_table != nullptr && u0 == 0 && h == 0 && threadIdx.x == 0) {
         x.seq_table[2 * q.b] = head + q.rank;
         x.seq_table[2 * q.b + 1] = splits;
     }
@@ -701,7 +700,7 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
         }
         if (__builtin_expect(__any(top >= 0xff000000u), 0)) { few_walk<D, BF, NT, true>(x, h, s, tiles, table, j0, j1, c, g, r); }
     }
-    // ---- the four waves' states into wave 0's: 2 and 3 into 0 and 1, then 1 into 0
+    // ---- the waves' states into wave 0's: the upper half into the lower one, again and again
     float M[NT], L[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -738,6 +737,10 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
             }
         }
     };
+    if constexpr (NW == 8) {
+        halve(4);
+        __syncthreads();
+    }
     halve(2);
     __syncthreads();
     halve(1);
@@ -780,12 +783,20 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
     }
 }
 
-template <int D, bool BF, int NT>
-__global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few_waves(D), few_waves(D)))) void paged_attn_few_kernel(PagedAttnArgs x) {
-    // two waves' O and (m, l) at a time
-    __shared__ f4 xo[2][NT * (D / 16) * 64];
-    __shared__ float2 xm[2][NT * 64];
+// WHOLE: a workgroup per sequence and KV head instead of a share.
+template <int D, bool BF, int NT, int NW, bool WHOLE>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW == 8 ? 2 : few_waves(D), NW == 8 ? 2 : few_waves(D)))) void
+paged_attn_few_kernel(PagedAttnArgs x) {
+    // half of the waves' O and (m, l) at a time
+    __shared__ f4 xo[NW / 2][NT * (D / 16) * 64];
+    __shared__ float2 xm[NW / 2][NT * 64];
     const int lane = threadIdx.x & 63;
+    if constexpr (WHOLE) {
+        FewSeq q{static_cast<int>(blockIdx.x) / x.c.Hkv, 0, 0, 0, {}};
+        q.units = few_units(x, q.b, q.s);
+        if (q.units > 0) { few_part<D, BF, NT, NW>(x, blockIdx.x % x.c.Hkv, q, FewPlan{q.units, 1}, 0, 0, q.units, xo, xm); }
+        return;
+    }
     const int h = blockIdx.x % x.c.Hkv;
     FewLanes fl;
     const FewPlan plan = few_plan(x, lane, fl);
@@ -796,7 +807,7 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(few
     for (int u = plan.begin(share); u < stop;) {
         const FewSeq q = few_find(x, u, lane, fl);
         const int next = min(stop, q.first + q.units);
-        few_part<D, BF, NT>(x, h, q, plan, share, u - q.first, next - q.first, xo, xm);
+        few_part<D, BF, NT, NW>(x, h, q, plan, share, u - q.first, next - q.first, xo, xm);
         u = next;
     }
 }
@@ -980,17 +991,31 @@ struct Tail {
     float us;
 };
 
-__host__ __device__ inline Tail tail_of(int rem, int longest, float us_tile, int elements, int parts) {
-    Tail best{1, 0.0f};
-    if (rem <= 0) { return best; }
-    best.us = kWorkgroupUs + static_cast<float>(longest) * us_tile;
-    for (int ns = 2; ns <= 32 && ns * rem <= parts && ns <= longest; ++ns) {
-        const int rounds = (rem * ns + kCus - 1) / kCus;
-        const float us = static_cast<float>(rounds) * (kWorkgroupUs + static_cast<float>((longest + ns - 1) / ns) * us_tile) + 8.0f +
-                         static_cast<float>(rem * ns) * static_cast<float>(elements) * 2.0e-6f;
+constexpr int kMaxSplits = 32;
+
+// The time with `ns` splits; infinite where they are not possible.
+__host__ __device__ inline float tail_us(int rem, int ns, int longest, float us_tile, int elements, int parts) {
+    if (ns == 1) { return kWorkgroupUs + static_cast<float>(longest) * us_tile; }
+    if (ns * rem > parts || ns > longest) { return INFINITY; }
+    const int rounds = (rem * ns + kCus - 1) / kCus;
+    return static_cast<float>(rounds) * (kWorkgroupUs + static_cast<float>((longest + ns - 1) / ns) * us_tile) + 8.0f +
+           static_cast<float>(rem * ns) * static_cast<float>(elements) * 2.0e-6f;
+}
+
+// On the host one after another, on the device a lane each (a loop there took longer than the splits could save).
+inline Tail tail_of(int rem, int longest, float us_tile, int elements, int parts) {
+    Tail best{1, rem > 0 ? tail_us(rem, 1, longest, us_tile, elements, parts) : 0.0f};
+    for (int ns = 2; rem > 0 && ns <= kMaxSplits; ++ns) {
+        const float us = tail_us(rem, ns, longest, us_tile, elements, parts);
         if (us < best.us) { best = Tail{ns, us}; }
     }
     return best;
+}
+
+__device__ __forceinline__ int tail_splits(int rem, int longest, float us_tile, int elements, int parts, int lane) {
+    const float us = lane < kMaxSplits ? tail_us(rem, lane + 1, longest, us_tile, elements, parts) : INFINITY;
+    const uint64_t best = __ballot(us == -wave_max(-us));
+    return __ffsll(static_cast<long long>(best));
 }
 
 // The row tiles of 64 sequences, spread over the lanes of a wave: their numbers and inclusive sums.
@@ -1034,7 +1059,7 @@ __device__ __forceinline__ ManyPlan many_plan(const PagedAttnArgs& x, int lane, 
     }
     ManyPlan p{total * x.c.Hkv, 0, 1};
     p.full = p.units / kCus * kCus;
-    p.splits = tail_of(p.units - p.full, longest, tile_us(D, WK), BM * D, x.many_parts).splits;
+    if (p.units > p.full) { p.splits = tail_splits(p.units - p.full, longest, tile_us(D, WK), BM * D, x.many_parts, lane); }
     if (p.splits == 1) { p.full = p.units; }
     return p;
 }
@@ -1545,6 +1570,7 @@ struct PagedPlan {
     int32_t nt = 1;        // 16-row tiles of a few-row workgroup
     int32_t few_rows = 0;
     int32_t slots = 0;     // 0: no sequence of few rows is possible
+    bool whole = false;    // a workgroup per few-row sequence
     bool merge = false;
     int32_t wk = 1;        // many rows: waves of a row tile over the keys
     int32_t tiles = 0;     // row tiles of the batch, at most (0: no sequence of many rows is possible)
@@ -1576,15 +1602,23 @@ PagedPlan plan_paged(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t
     size_t at = 0;
     if (p.few_rows > 0) {
         const int64_t units = (seen(std::min<int64_t>(max_new, p.few_rows)) + 127) / 128;
-        p.slots = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(kCus * few_waves(D) / Hkv, B * units)));
-        p.merge = p.slots > 1;
+        // Where the sequences' heads are about as many as the CUs and short, a workgroup of eight waves each needs no merge
+        // launch: 32 sequences at 40/8/128 INT8 of 200 rows 17.0 -> 11.1 us, of 500 20.2 -> 14.2, of 1,000 25.4 -> 19.6; 64 at
+        // 24/4/256 of 500 28.6 -> 25.7. Fewer leave CUs idle (16 of 1,000 at 24/4/256 20.3 -> 34.5), more or longer ones gain
+        // nothing or lose by their lengths' differences (200 of 300 rows 78 -> 84).
+        const int64_t heads = static_cast<int64_t>(B) * Hkv;
+        p.whole = p.nt == 1 && units <= 8 && heads > kCus * 3 / 4 && heads <= kCus;
+        p.slots = p.whole ? B : static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(kCus * few_waves(D) / Hkv, B * units)));
+        p.merge = !p.whole && p.slots > 1;
         if (p.merge) {
             const size_t rows = static_cast<size_t>(p.slots + B) * Hkv * p.few_rows;
             p.ml_offset = align_up(rows * D * sizeof(float));
             at = align_up(p.ml_offset + rows * 2 * sizeof(float));
         }
-        p.table_offset = at;
-        at = align_up(at + static_cast<size_t>(B) * 2 * sizeof(int32_t));
+        if (p.merge) {
+            p.table_offset = at;
+            at = align_up(at + static_cast<size_t>(B) * 2 * sizeof(int32_t));
+        }
     }
     if (most_rows > p.few_rows) {
         const int64_t rows = tokens * G;
@@ -1624,10 +1658,12 @@ void launch(const PagedAttnArgs& x, const PagedPlan& p, hipStream_t stream) {
     uint32_t few = 0, tails = 0; // workgroups of the merge
     if (p.slots > 0) {
         const uint32_t grid = static_cast<uint32_t>(p.slots) * x.c.Hkv;
-        if (p.nt == 1) {
-            hipLaunchKernelGGL((paged_attn_few_kernel<D, BF, 1>), dim3(grid), dim3(kFewThreads), 0, stream, x);
+        if (p.whole) {
+            hipLaunchKernelGGL((paged_attn_few_kernel<D, BF, 1, 8, true>), dim3(grid), dim3(512), 0, stream, x);
+        } else if (p.nt == 1) {
+            hipLaunchKernelGGL((paged_attn_few_kernel<D, BF, 1, 4, false>), dim3(grid), dim3(256), 0, stream, x);
         } else {
-            hipLaunchKernelGGL((paged_attn_few_kernel<D, BF, 2>), dim3(grid), dim3(kFewThreads), 0, stream, x);
+            hipLaunchKernelGGL((paged_attn_few_kernel<D, BF, 2, 4, false>), dim3(grid), dim3(256), 0, stream, x);
         }
         check_launch("paged_attn_few_kernel");
         if (p.merge) { few = static_cast<uint32_t>(p.few_rows) * x.c.Hkv * x.c.B; }
@@ -1677,7 +1713,7 @@ void launch_paged_attention(const PagedAttention& a, const PagedRef& c, void* wo
     char* ws = static_cast<char*>(workspace);
     x.part_o = reinterpret_cast<float*>(ws);
     x.part_ml = reinterpret_cast<float*>(ws + p.ml_offset);
-    x.seq_table = reinterpret_cast<int32_t*>(ws + p.table_offset);
+    x.seq_table = p.merge ? reinterpret_cast<int32_t*>(ws + p.table_offset) : nullptr;
     x.many_o = reinterpret_cast<float*>(ws + p.many_offset);
     x.many_ml = reinterpret_cast<float*>(ws + p.many_ml_offset);
     if (c.D == 128 && !c.bf16) {

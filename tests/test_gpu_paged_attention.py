@@ -55,6 +55,19 @@ def test_ragged_batch(gpu, geo, kv, name):
     _run(PagedCase(RAGGED[name], Hq=Hq, Hkv=Hkv, D=D, kv=kv, page=16, seed=len(name), lead=1, tail=3, page_pad=64))
 
 
+@pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("Hq,Hkv,D,batch", [(40, 8, 128, 32), (40, 8, 128, 25), (24, 4, 256, 64), (8, 1, 128, 250)])
+@pytest.mark.parametrize("rows", [1, 40, 1000])
+@pytest.mark.parametrize("window", [0, 50])
+def test_as_many_short_sequences_as_compute_units(gpu, kv, Hq, Hkv, D, batch, rows, window):
+    """One token each: a workgroup per sequence and head; some sequences without a token, one without pages."""
+    r = np.random.default_rng(batch + rows)
+    seqs = [(int(r.random() < 0.9), int(r.integers(0, rows))) for _ in range(batch)]
+    seqs[3] = (1, rows - 1)
+    seqs[7] = (1, 20)
+    _run(PagedCase(seqs, Hq=Hq, Hkv=Hkv, D=D, kv=kv, page=16, seed=batch, absent={(7, 0), (7, 1)}, window=window, sinks=2 if window else 0))
+
+
 @pytest.mark.parametrize("batch", [65, 200])
 def test_many_sequences(gpu, batch):
     r = np.random.default_rng(batch)
