@@ -109,6 +109,10 @@ __device__ __forceinline__ u2 out_pair(f4 O, float L) {
 // them, and Q follows), and four bytes (INT8; BF16: sixteen) of the V rows 4g .. 4g + 3 of both halves, the keys
 // whose scores the S^T accumulator leaves in this lane; so P needs no exchange between lanes, and V is transposed
 // by byte selects alone. No LDS in the loop.
+//
+// What bounds it: HBM (31 flop a byte with INT8 rows and one row tile); the VALU converts and weighs 64% of the
+// time. Measured on MI355X: 32 single tokens over 535,000 ragged rows at 40/8/128 INT8 213 us (5.3 TB/s), 4 tokens over
+// 131,004 rows at 24/4/256 BF16 99 us (5.4 TB/s).
 
 template <int D, bool BF>
 struct Chunk {
@@ -823,8 +827,12 @@ paged_attn_few_kernel(PagedAttnArgs x) {
 // Operands are FP16 (K and Q of BF16 caches stay BF16): K' = code * scale and V' = code * scale or value, times a
 // power of two that the workgroup takes from its first tile (three bits of room above its largest scale or value),
 // rounded once (2^-11). A tile with a larger, infinite or NaN value or (INT8) a V scale below 2^-18 of the top is left
-// out, and its chunks are walked as the few-row kernel does it afterwards, which has no such range; BF16 values down to 2^-29 of the
-// top are exact.
+// out, and its chunks are walked as the few-row kernel does it afterwards, which has no such range; BF16 values down to
+// 2^-29 of the top are exact.
+//
+// What bounds it: neither matrix cores (40% busy) nor VALU (60%) alone; a SIMD's two waves hardly overlap them, and the
+// registers (256 each) leave no room for more work of one wave in flight. Measured on MI355X, 8,192 first tokens at
+// 40/8/128: INT8 805 us (855 TFLOP/s), BF16 781 us; at 24/4/256 1,162 and 1,082 us; a large library product reaches 1,318.
 
 constexpr int kManyThreads = 512;
 constexpr int kManyMarks = 131072;          // key tiles of a workgroup, at most
@@ -983,9 +991,9 @@ __host__ __device__ constexpr float tile_us(int D, int wk) {
 constexpr float kWorkgroupUs = 8.0f;
 
 // The last `rem` row tiles x heads that do not fill the chip: key splits of each, and the time they take. Parts are
-// written and read at 4 TB/s and cost a launch. Measured at 40/8/128 INT8: 200 tokens over 2,000 rows 39.9 us as it
-// chooses (two waves per row tile, four splits), 38.2 and 48.0 us with one and four waves; 700 over 300 rows 41.0 (two
-// waves, no splits), 51.8 and 58.5 us.
+// written and read at 4 TB/s and cost a launch. Measured at 40/8/128 INT8: 200 tokens over 2,000 rows 39.9 us with
+// two waves per row tile and four splits, 38.2 and 48.0 us with one and four waves; 700 over 300 rows 41.0 (two waves,
+// no splits), 51.8 and 58.5 us.
 struct Tail {
     int splits;
     float us;
@@ -1002,7 +1010,8 @@ __host__ __device__ inline float tail_us(int rem, int ns, int longest, float us_
            static_cast<float>(rem * ns) * static_cast<float>(elements) * 2.0e-6f;
 }
 
-// On the host one after another, on the device a lane each (a loop there took longer than the splits could save).
+// On the host one after another, on the device a lane each (with a loop there 200 tokens over 2,000 rows took 38.8 us
+// instead of 34.2).
 inline Tail tail_of(int rem, int longest, float us_tile, int elements, int parts) {
     Tail best{1, rem > 0 ? tail_us(rem, 1, longest, us_tile, elements, parts) : 0.0f};
     for (int ns = 2; rem > 0 && ns <= kMaxSplits; ++ns) {
@@ -1565,7 +1574,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs x, 
 
 namespace {
 
-// How a call is cut. Few-row slots: two workgroups of the kernel fill a CU.
+// How a call is cut.
 struct PagedPlan {
     int32_t nt = 1;        // 16-row tiles of a few-row workgroup
     int32_t few_rows = 0;
