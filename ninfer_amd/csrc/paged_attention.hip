@@ -825,10 +825,11 @@ paged_attn_few_kernel(PagedAttnArgs x) {
 // reads, V in 32-byte segments for the transposing reads (ds_read_b64_tr_b16), which deliver V^T operands in the key
 // order that the S^T accumulator leaves P in.
 // Operands are FP16 (K and Q of BF16 caches stay BF16): K' = code * scale and V' = code * scale or value, times a
-// power of two that the workgroup takes from its first tile (three bits of room above its largest scale or value),
-// rounded once (2^-11). A tile with a larger, infinite or NaN value or (INT8) a V scale below 2^-18 of the top is left
-// out, and its chunks are walked as the few-row kernel does it afterwards, which has no such range; BF16 values down to
-// 2^-29 of the top are exact.
+// power of two that the workgroup takes from its first tile with a value (three bits of room above its largest scale or
+// value), rounded once (2^-11); BF16 values down to 2^-29 of the top are exact, smaller ones off by at most 2^-19 of the
+// largest of their unit of eight. A tile with a larger, infinite or NaN value, or with an INT8 V scale or a BF16 unit below
+// 2^-18 of the top (other than zero) is left out, and its chunks are walked as the few-row kernel does it afterwards, which
+// has no such range.
 //
 // What bounds it: neither matrix cores (40% busy) nor VALU (60%) alone; a SIMD's two waves hardly overlap them, and the
 // registers (256 each) leave no room for more work of one wave in flight. Measured on MI355X, 8,192 first tokens at
@@ -905,28 +906,38 @@ __device__ __forceinline__ void stage_trim(StageRegs<D, BF>& r, int live, int la
     }
 }
 
-// The largest magnitudes of a thread's part, NaN kept: K's and V's scales, or (BF16) V's values.
+// The largest magnitudes of a thread's part, NaN kept: K's and V's scales, or (BF16) V's values, a pair's as one FP32 number
+// (the upper value's size, off by less than BF16's step, or a number next to zero where only the lower one is not zero).
+// `least` (BF16): the smallest of its units' largest values, zeros aside, as bits less one.
+struct StageSize {
+    float k, v;
+    uint32_t least;
+};
+
 template <int D, bool BF>
-__device__ __forceinline__ void stage_top(const StageRegs<D, BF>& r, float& kt, float& vt) {
-    kt = vt = 0.0f;
+__device__ __forceinline__ StageSize stage_size(const StageRegs<D, BF>& r) {
+    StageSize z{0.0f, 0.0f, 0xffffffffu};
 #pragma unroll
     for (int i = 0; i < StageRegs<D, BF>::U; ++i) {
         if constexpr (BF) {
+            float m = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                vt = fmax_ieee(vt, fmax_ieee(fabsf(__uint_as_float(r.v[i][w] << 16)), fabsf(__uint_as_float(r.v[i][w] & 0xffff0000u))));
-            }
+            for (int w = 0; w < 4; ++w) { m = fmax_ieee(m, fmax_ieee(fabsf(__uint_as_float(r.v[i][w] << 16)), fabsf(__uint_as_float(r.v[i][w])))); }
+            z.v = fmax_ieee(z.v, m);
+            z.least = min(z.least, __float_as_uint(m) - 1u);
         } else {
-            kt = fmax_ieee(kt, fabsf(f16_bits_to_f32(static_cast<uint16_t>(r.ks[i]))));
-            vt = fmax_ieee(vt, fabsf(f16_bits_to_f32(static_cast<uint16_t>(r.vs[i]))));
+            z.k = fmax_ieee(z.k, fabsf(f16_bits_to_f32(static_cast<uint16_t>(r.ks[i]))));
+            z.v = fmax_ieee(z.v, fabsf(f16_bits_to_f32(static_cast<uint16_t>(r.vs[i]))));
         }
     }
+    return z;
 }
 
 // The workgroup's powers of two and the bounds of what they can hold.
 struct ManyScale {
     float k, v;       // factors of K' and V'
     float klim, vlim; // a tile with a larger scale (BF16: value) needs care
+    uint32_t vleast;  // BF16: so does one with a smaller, but not zero, unit, as StageSize::least has it
 };
 
 // INT8: |code| <= 128, so scales below 2^E give K' below 2^15; BF16: values below 2^E.
@@ -944,9 +955,8 @@ __device__ __forceinline__ bool stage_store(const StageRegs<D, BF>& r, const Man
     constexpr int kRow = BF ? 2 * D : D;
     constexpr int PR = kRow / 16;
     char* vp = buf + ManyGeo<D, 1>::kPlane;
-    float kt, vt;
-    stage_top<D, BF>(r, kt, vt);
-    bool small = false; // an INT8 V scale that FP16 would round
+    const StageSize z = stage_size<D, BF>(r);
+    bool small = BF && z.least < sc.vleast; // an INT8 V scale, or a unit of BF16 values, that FP16 would round
 #pragma unroll
     for (int i = 0; i < StageRegs<D, BF>::U; ++i) {
         const int u = lane + 64 * i;
@@ -977,7 +987,7 @@ __device__ __forceinline__ bool stage_store(const StageRegs<D, BF>& r, const Man
             *reinterpret_cast<h8*>(vr + 16) = scale_h8(codes8(r.v[i][2], r.v[i][3]), v2);
         }
     }
-    return small || !(kt <= sc.klim && vt <= sc.vlim); // NaN: care
+    return small || !(z.k <= sc.klim && z.v <= sc.vlim); // NaN: care
 }
 
 constexpr int kCus = 256;
@@ -1157,7 +1167,7 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
         page = __builtin_amdgcn_readlane(ids, i & 63);
         stage_load<D, BF>(x, h, tiles.tile(j) * KT + wave * MG::RW, page, lane, sr);
     };
-    ManyScale sc{1.0f, 1.0f, INFINITY, INFINITY};
+    ManyScale sc{1.0f, 1.0f, INFINITY, INFINITY, 0u};
     const auto trim = [&](int j) {
         const int live = p1 + 1 - (tiles.tile(j) * KT + wave * MG::RW);
         if (live < MG::RW) { stage_trim<D, BF>(sr, live, lane); }
@@ -1179,24 +1189,31 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
     bool cared = false;
     if (j0 < j1) {
         for (int i = threadIdx.x; 32 * i < j1 - j0; i += kManyThreads) { marks[i] = 0u; }
-        trim(j0);
-        float kt, vt;
-        stage_top<D, BF>(sr, kt, vt);
-        kt = wave_max(kt < INFINITY ? kt : 0.0f);
-        vt = wave_max(vt < INFINITY ? vt : 0.0f);
-        if (lane == 0) {
-            tops[0][wave] = kt;
-            tops[1][wave] = vt;
-        }
-        __syncthreads();
-        kt = vt = 0.0f;
+        // the first tile that holds a value tells how large they are: absent pages and zero rows say nothing
+        float kt = 0.0f, vt = 0.0f;
+        int js = j0;
+        for (;; ++js) {
+            if (js > j0) { stage_load<D, BF>(x, h, tiles.tile(js) * KT + wave * MG::RW, __builtin_amdgcn_readfirstlane(pages_from(js)), lane, sr); }
+            trim(js);
+            const StageSize z = stage_size<D, BF>(sr);
+            const float kw = wave_max(z.k < INFINITY ? z.k : 0.0f), vw = wave_max(z.v < INFINITY ? z.v : 0.0f);
+            if (lane == 0) {
+                tops[0][wave] = kw;
+                tops[1][wave] = vw;
+            }
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            kt = fmaxf(kt, tops[0][i]);
-            vt = fmaxf(vt, tops[1][i]);
+            for (int i = 0; i < 8; ++i) {
+                kt = fmaxf(kt, tops[0][i]);
+                vt = fmaxf(vt, tops[1][i]);
+            }
+            if (__any(vt > 0.0f) || js + 1 == j1) { break; }
+            __syncthreads(); // the tops are read
         }
+        if (js > j0) { fetch(j0); }
         pick(kt, 8, sc.k, sc.klim);
         pick(vt, BF ? 15 : 8, sc.v, sc.vlim);
+        sc.vleast = __float_as_uint(0x1p-6f / sc.v) - 1u;
         put(j0);
         if (j0 + 1 < j1) { fetch(j0 + 1); }
         __syncthreads();

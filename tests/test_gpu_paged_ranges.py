@@ -1,0 +1,55 @@
+"""Paged attention where rows differ by many orders of magnitude: keys that a token does not see, or that hardly count,
+cost the others no bits."""
+import numpy as np
+import pytest
+
+from paged_bound import check_bound
+from paged_case import PagedCase, bf16_bits, bf16_values
+
+pytestmark = pytest.mark.gpu
+
+CACHES = ["i8", "bf16"]
+GEO = {"10-2-128": (10, 2, 128), "12-2-256": (12, 2, 256)}
+
+
+def _grow(x, f):
+    x[:] = bf16_bits(bf16_values(x) * np.float32(f))
+
+
+def _run(c):
+    d = c.upload()
+    d.attend()
+    check_bound(c, d.result())
+
+
+@pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("geo", GEO)
+@pytest.mark.parametrize("tokens", [1, 90])
+@pytest.mark.parametrize("size", [1e-4, 1e-6, 1e-7, 1e-8])
+@pytest.mark.parametrize("first", ["absent pages", "zero rows"])
+def test_small_values_behind_an_empty_tile(gpu, kv, geo, tokens, size, first):
+    """The first key tile of a workgroup holds no value that could tell how large the others are."""
+    Hq, Hkv, D = GEO[geo]
+
+    def edit(c):
+        for x in c.v:
+            _grow(x, size * (100 if kv == "i8" else 1))  # an INT8 value is at least its FP16 scale's smallest step
+        if first == "zero rows":
+            c.v[0][:256] = 0
+    absent = {(0, p) for p in range(16)} if first == "absent pages" else ()
+    _run(PagedCase([(tokens, 400), (tokens, 30)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=30, absent=absent, edit=edit))
+
+
+def _small_before_large(kv, geo, small):
+    """First tokens see small values only; the tile that tells the size of the values holds ones of 1e3 too."""
+    Hq, Hkv, D = GEO[geo]
+
+    def edit(c):
+        _grow(c.v[0][:8], small)
+        _grow(c.v[0][8:], 1e3)
+    _run(PagedCase([(100, 0)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=31, edit=edit))
+
+
+@pytest.mark.parametrize("geo", GEO)
+def test_small_bf16_values_before_large_ones(gpu, geo):
+    _small_before_large("bf16", geo, 1e-7)
