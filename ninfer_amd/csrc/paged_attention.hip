@@ -8,9 +8,10 @@
 //
 // Numbers: an INT8 code is exact in FP16, and Q is BF16 made FP16 by a power of two per row, so q . code is exact
 // up to the FP32 sum; the scale of a key's 64-value group multiplies that sum in FP32. The probabilities take the
-// V scales in the same way: w = p * s * 2^-E in FP16 (off by 2^-11 of itself; 2^E tops the scales of the 32 keys
-// at hand, so w neither overflows nor, next to them, vanishes), times codes, times 2^E in FP32. No scale is too
-// large or too small for that. BF16 caches multiply stored values; p goes in as two BF16 terms (16 bits).
+// V scales in the same way: w = p * s * 2^-E in FP16 (off by 2^-11 of itself, 2^-39 of the largest at least), times codes,
+// times 2^E in FP32. 2^E is the row's own: it tops w of the 32 keys at hand, so no scale is too large or too small,
+// and keys that the row does not see or that weigh nothing take no bits from the others. BF16 caches multiply stored
+// values; p goes in as two BF16 terms (16 bits).
 // Maxima, sums and accumulators are FP32.
 #include "attn_math.h"
 #include "common.h"
@@ -400,24 +401,15 @@ __device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const P
     using CK = Chunk<D, BF>;
     const float(&p)[NT][8] = y.p;
     if (!y.whole) {
-        // keys that no row of the wave may see: whatever their rows hold is taken out
+        if constexpr (BF) {
+            // keys that no row of the wave may see: whatever their rows hold is taken out
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bool dead = 32 * tile + 16 * (i >> 2) + 4 * g + (i & 3) > (s.hi | (hv.page[i >> 2] >> 31));
-            if constexpr (BF) {
+            for (int i = 0; i < 8; ++i) {
+                const bool dead = 32 * tile + 16 * (i >> 2) + 4 * g + (i & 3) > (s.hi | (hv.page[i >> 2] >> 31));
 #pragma unroll
                 for (int w = 0; w < CK::VP; ++w) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) { r.v[i][w][e] = dead ? 0u : r.v[i][w][e]; }
-                }
-            } else {
-#pragma unroll
-                for (int w = 0; w < D / 128; ++w) {
-                    if constexpr (D == 128) {
-                        r.vs[i >> 2][0][i & 3] = dead ? 0u : r.vs[i >> 2][0][i & 3];
-                    } else {
-                        r.vs[i >> 2][(i & 3) >> 1][2 * (i & 1) + w] = dead ? 0u : r.vs[i >> 2][(i & 3) >> 1][2 * (i & 1) + w];
-                    }
                 }
             }
         }
@@ -426,27 +418,27 @@ __device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const P
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
             float sc[8];
-            float top = 0.0f; // the largest finite scale of the chunk's keys, in group i
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                sc[k] = scale_of<D>(r.vs[k >> 2], k & 3, i);
-                const float a = fabsf(sc[k]);
-                top = fmaxf(top, a < INFINITY ? a : 0.0f);
-            }
-            top = group4_max(top);
-            // 2^E > top; FP16 scales have exponents of -24 to 15
-            const int E = static_cast<int>(__float_as_uint(top) >> 23) - 126;
-            const float down = top > 0.0f ? __uint_as_float(static_cast<uint32_t>(127 - E) << 23) : 1.0f;
-            const float up = top > 0.0f ? __uint_as_float(static_cast<uint32_t>(127 + E) << 23) : 1.0f;
+            for (int k = 0; k < 8; ++k) { sc[k] = scale_of<D>(r.vs[k >> 2], k & 3, i); }
             h8 w[NT];
+            float up[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
+                float z[8];
+                float top = 0.0f; // the row's largest weight of the chunk in group i
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    float z = p[nt][k] * (sc[k] * down);
-                    if (!y.whole) { z = ((y.seen[nt] >> k) & 1u) ? z : 0.0f; } // an unseen row's scale may be anything
-                    w[nt][k] = static_cast<_Float16>(z);
+                    z[k] = p[nt][k] * sc[k];
+                    if (!y.whole) { z[k] = ((y.seen[nt] >> k) & 1u) ? z[k] : 0.0f; } // an unseen row's scale may be anything
+                    top = fmaxf(top, fabsf(z[k]));
                 }
+                top = group4_max(top);
+                // 2^E > top; next to an infinite scale 2^31, which tops every finite weight (p <= 2^15, FP16 scales)
+                const int E = max(-100, min(31, static_cast<int>(__float_as_uint(top) >> 23) - 126));
+                const float down = __uint_as_float(static_cast<uint32_t>(127 + 15 - E) << 23);
+                up[nt] = __uint_as_float(static_cast<uint32_t>(127 - 15 + E) << 23);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) { w[nt][k] = static_cast<_Float16>(z[k] * down); }
             }
             const auto tile4 = [&](auto byte) {
                 constexpr int Bt = decltype(byte)::value;
@@ -457,7 +449,7 @@ __device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const P
                 for (int nt = 0; nt < NT; ++nt) {
                     const f4 o = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, va), w[nt], f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { s.O[nt][4 * i + Bt][e] = fmaf(o[e], up, s.O[nt][4 * i + Bt][e]); }
+                    for (int e = 0; e < 4; ++e) { s.O[nt][4 * i + Bt][e] = fmaf(o[e], up[nt], s.O[nt][4 * i + Bt][e]); }
                 }
             };
             tile4(std::integral_constant<int, 0>{});

@@ -53,3 +53,53 @@ def _small_before_large(kv, geo, small):
 @pytest.mark.parametrize("geo", GEO)
 def test_small_bf16_values_before_large_ones(gpu, geo):
     _small_before_large("bf16", geo, 1e-7)
+
+
+@pytest.mark.parametrize("geo", GEO)
+def test_small_int8_values_before_large_ones(gpu, geo):
+    _small_before_large("i8", geo, 1e-4)
+
+
+@pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("geo", GEO)
+@pytest.mark.parametrize("tokens", [1, 3, 90])
+@pytest.mark.parametrize("small", [1.0, 1e-3, 1e-5])
+def test_large_values_that_left_the_window(gpu, kv, geo, tokens, small):
+    """Rows right before the window, in the window's first key chunk, hold values of 3e6; those that are seen are small."""
+    Hq, Hkv, D = GEO[geo]
+    h, w = 700, 50
+
+    def edit(c):
+        _grow(c.v[0], small)
+        for r in (h - w, h - w - 1, h - w - 9):
+            c.v[0][r] = bf16_bits(np.full(c.v[0][r].shape, 3e6, np.float32))
+    _run(PagedCase([(tokens, h)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, window=w, sinks=3, seed=32, edit=edit))
+
+
+@pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("geo", GEO)
+@pytest.mark.parametrize("tokens", [3, 90])
+def test_large_values_of_later_tokens(gpu, kv, geo, tokens):
+    """A later token of the chunk brings values of 3e6: earlier ones, whose values are 1e-3, do not see it."""
+    Hq, Hkv, D = GEO[geo]
+
+    def edit(c):
+        _grow(c.v[0], 1e-3)
+        c.v[0][300 + tokens - 1] = bf16_bits(np.full(c.v[0][0].shape, 3e6, np.float32))
+    _run(PagedCase([(tokens, 300)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=33, edit=edit))
+
+
+@pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("geo", GEO)
+@pytest.mark.parametrize("tokens", [1, 90])
+def test_large_values_without_weight(gpu, kv, geo, tokens):
+    """A key that is seen, but counts for less than 1e-20, has values of 3e6; the others have 1e-3."""
+    Hq, Hkv, D = GEO[geo]
+
+    def edit(c):
+        _grow(c.v[0], 1e-3)
+        c.q[:, :, 1] = bf16_bits(np.float32(8.0))
+        c.k[0][:, :, 1] = 0
+        c.k[0][70, :, 1] = bf16_bits(np.float32(-100.0))
+        c.v[0][70] = bf16_bits(np.full(c.v[0][70].shape, 3e6, np.float32))
+    _run(PagedCase([(tokens, 100)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=34, edit=edit))
