@@ -819,7 +819,7 @@ paged_attn_few_kernel(PagedAttnArgs x) {
 // Operands are FP16 (K and Q of BF16 caches stay BF16): K' = code * scale and V' = code * scale or value, times a
 // power of two that the workgroup takes from its first tile with a value (three bits of room above its largest scale or
 // value), rounded once (2^-11); BF16 values down to 2^-29 of the top are exact, smaller ones off by at most 2^-19 of the
-// largest of their unit of eight. A tile with a larger, infinite or NaN value, or with an INT8 V scale or a BF16 unit below
+// largest of their unit of eight. A tile with a larger, infinite or NaN value, or with an INT8 scale or a BF16 unit below
 // 2^-18 of the top (other than zero) is left out, and its chunks are walked as the few-row kernel does it afterwards, which
 // has no such range.
 //
@@ -948,7 +948,7 @@ __device__ __forceinline__ bool stage_store(const StageRegs<D, BF>& r, const Man
     constexpr int PR = kRow / 16;
     char* vp = buf + ManyGeo<D, 1>::kPlane;
     const StageSize z = stage_size<D, BF>(r);
-    bool small = BF && z.least < sc.vleast; // an INT8 V scale, or a unit of BF16 values, that FP16 would round
+    bool small = BF && z.least < sc.vleast; // an INT8 scale, or a unit of BF16 values, that FP16 would round
 #pragma unroll
     for (int i = 0; i < StageRegs<D, BF>::U; ++i) {
         const int u = lane + 64 * i;
@@ -971,7 +971,7 @@ __device__ __forceinline__ bool stage_store(const StageRegs<D, BF>& r, const Man
             const _Float16 k1 = static_cast<_Float16>(f16_bits_to_f32(static_cast<uint16_t>(r.ks[i])) * sc.k);
             const _Float16 v1 = static_cast<_Float16>(f16_bits_to_f32(static_cast<uint16_t>(r.vs[i])) * sc.v);
             const h2 k2 = {k1, k1}, v2 = {v1, v1};
-            small |= r.vs[i] != 0u && fabsf(static_cast<float>(v1)) < 0x1p-14f;
+            small |= (r.ks[i] != 0u && fabsf(static_cast<float>(k1)) < 0x1p-14f) || (r.vs[i] != 0u && fabsf(static_cast<float>(v1)) < 0x1p-14f);
             *reinterpret_cast<h8*>(buf + at + 16 * (p ^ (row & 15))) = scale_h8(codes8(r.k[i][0], r.k[i][1]), k2);
             *reinterpret_cast<h8*>(buf + at + 16 * ((p + 1) ^ (row & 15))) = scale_h8(codes8(r.k[i][2], r.k[i][3]), k2);
             char* vr = vp + at + 32 * ((p >> 1) ^ k7);

@@ -103,3 +103,19 @@ def test_large_values_without_weight(gpu, kv, geo, tokens):
         c.k[0][70, :, 1] = bf16_bits(np.float32(-100.0))
         c.v[0][70] = bf16_bits(np.full(c.v[0][70].shape, 3e6, np.float32))
     _run(PagedCase([(tokens, 100)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=34, edit=edit))
+
+
+@pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("geo", GEO)
+@pytest.mark.parametrize("tokens", [1, 3, 90])
+def test_large_keys_that_left_the_window(gpu, kv, geo, tokens):
+    """As for values: keys of 6e6 that are not seen, next to keys of 1e-3 under queries of 1e3."""
+    Hq, Hkv, D = GEO[geo]
+    h, w = 700, 50
+
+    def edit(c):
+        _grow(c.k[0], 1e-3)
+        _grow(c.q, 1e3)
+        for r in (h - w, h - w - 1, h - w - 9):
+            c.k[0][r] = bf16_bits(np.full(c.k[0][r].shape, 6e6, np.float32))
+    _run(PagedCase([(tokens, h)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, window=w, seed=35, edit=edit))
