@@ -394,8 +394,18 @@ __device__ __forceinline__ void chunk_probs(const PagedAttnArgs& x, int tile, Ha
     }
 }
 
-// O^T += V^T P^T. CARE (BF16): infinite and NaN values reach only the rows that see them; without it they may make any row
-// of the wave NaN.
+// The careful products' weights are p * 2^-kCareShift: a sum of 2^23 of them, each up to 2^15, times BF16's largest value
+// stays finite.
+constexpr int kCareShift = 40;
+
+// The (log2-domain maximum, sum) of a state whose outputs are in the careful products' units.
+__device__ __forceinline__ void care_units(float& M, float& L) {
+    M += static_cast<float>(kCareShift);
+    L = ldexpf(L, -kCareShift);
+}
+
+// O^T += V^T P^T. CARE (BF16): infinite and NaN values reach only the rows that see them, finite ones overflow no sum; without
+// it they may make any row of the wave NaN.
 template <int D, bool BF, int NT, bool CARE>
 __device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const Probs<NT>& y, ChunkV<D, BF>& r, Rows<D, BF, NT>& s) {
     using CK = Chunk<D, BF>;
@@ -463,8 +473,9 @@ __device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const P
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                hi[nt][k] = static_cast<__bf16>(p[nt][k]);
-                lo[nt][k] = static_cast<__bf16>(p[nt][k] - static_cast<float>(hi[nt][k]));
+                const float z = CARE ? ldexpf(p[nt][k], -kCareShift) : p[nt][k];
+                hi[nt][k] = static_cast<__bf16>(z);
+                lo[nt][k] = static_cast<__bf16>(z - static_cast<float>(hi[nt][k]));
             }
         }
         if constexpr (CARE) {
@@ -684,6 +695,7 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
     Rows<D, BF, NT> r;
     const int32_t* table = x.c.table + q.b * x.c.table_row;
     few_walk<D, BF, NT, false>(x, h, s, tiles, table, j0, j1, c, g, r);
+    bool cared = false; // sums from 2^100 up, infinite ones or NaN: again, so that no sum of parts overflows either
     if constexpr (BF) {
         uint32_t top = 0u;
 #pragma unroll
@@ -694,7 +706,8 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
                 for (int e = 0; e < 4; ++e) { top = max(top, __float_as_uint(r.O[nt][t][e]) << 1); }
             }
         }
-        if (__builtin_expect(__any(top >= 0xff000000u), 0)) { few_walk<D, BF, NT, true>(x, h, s, tiles, table, j0, j1, c, g, r); }
+        cared = __any(top >= static_cast<uint32_t>(127 + 100) << 24);
+        if (__builtin_expect(cared, 0)) { few_walk<D, BF, NT, true>(x, h, s, tiles, table, j0, j1, c, g, r); }
     }
     // ---- the waves' states into wave 0's: the upper half into the lower one, again and again
     float M[NT], L[NT];
@@ -702,6 +715,7 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
     for (int nt = 0; nt < NT; ++nt) {
         M[nt] = r.m[nt] == -INFINITY ? -INFINITY : r.m[nt] * r.rowmul[nt];
         L[nt] = group4_sum(r.l[nt]);
+        if (cared) { care_units(M[nt], L[nt]); }
     }
     __syncthreads(); // the last part's states are read
     const auto halve = [&](int half) {
@@ -936,7 +950,7 @@ struct ManyScale {
 __device__ __forceinline__ void pick(float top, int shift, float& factor, float& lim) {
     const uint32_t b = __float_as_uint(top) >> 23;
     // no finite top (or none): factor one
-    const int E = top > 0.0f && b < 255u ? max(-100, min(100, static_cast<int>(b) - 126 + 3)) : shift;
+    const int E = top > 0.0f && b < 255u ? max(-100, min(60, static_cast<int>(b) - 126 + 3)) : shift; // sums stay below 2^100
     factor = __uint_as_float(static_cast<uint32_t>(127 + shift - E) << 23);
     lim = __uint_as_float(static_cast<uint32_t>(127 + E) << 23);
 }
@@ -1407,7 +1421,8 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const float m2 = r.m[nt] == -INFINITY ? -INFINITY : r.m[nt] * r.rowmul[nt], l2 = group4_sum(r.l[nt]);
+            float m2 = r.m[nt] == -INFINITY ? -INFINITY : r.m[nt] * r.rowmul[nt], l2 = group4_sum(r.l[nt]);
+            if constexpr (BF) { care_units(m2, l2); }
             const Weights q = weights(M[nt], L[nt], m2, l2);
             L[nt] = L[nt] * q.a + l2 * q.b;
             M[nt] = q.M;

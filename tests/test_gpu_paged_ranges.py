@@ -119,3 +119,19 @@ def test_large_keys_that_left_the_window(gpu, kv, geo, tokens):
         for r in (h - w, h - w - 1, h - w - 9):
             c.k[0][r] = bf16_bits(np.full(c.k[0][r].shape, 6e6, np.float32))
     _run(PagedCase([(tokens, h)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, window=w, seed=35, edit=edit))
+
+
+@pytest.mark.parametrize("geo", GEO)
+@pytest.mark.parametrize("tokens", [1, 3, 90])
+@pytest.mark.parametrize("size", [1e33, 1e36, 5e37])
+@pytest.mark.parametrize("rows", ["all", "late"])
+def test_values_near_the_top_of_bf16(gpu, geo, tokens, size, rows):
+    """Weighted means of finite values are finite."""
+    Hq, Hkv, D = GEO[geo]
+
+    def edit(c):
+        x = bf16_values(c.v[0]).astype(np.float64)
+        x = np.clip(x * (size / 2), -3e38, 3e38)  # a normal value times 2 in one dimension of 32
+        part = slice(0 if rows == "all" else 350, None)
+        c.v[0][part] = bf16_bits(x[part].astype(np.float32))
+    _run(PagedCase([(tokens, 500), (2, 20)], Hq=Hq, Hkv=Hkv, D=D, kv="bf16", seed=36, edit=edit))
