@@ -225,6 +225,8 @@ __device__ __forceinline__ float scale_of(const u4 (&w)[D / 128], int e, int i) 
     return f16_bits_to_f32(static_cast<uint16_t>((half & 1) ? x >> 16 : x & 0xffffu));
 }
 
+constexpr float kLargest = 3.4028234663852886e38f;
+
 // Online-softmax state of a wave's rows 16 nt + c.
 template <int D, bool BF, int NT>
 struct Rows {
@@ -287,7 +289,7 @@ __device__ __forceinline__ void init_rows(const PagedAttnArgs& x, const Seq& s, 
                     r.q[nt][k][w] = __builtin_bit_cast(uint32_t, p);
                 }
             }
-            r.rowmul[nt] = ldexpf(x.scale_log2, -fexp);
+            r.rowmul[nt] = fminf(ldexpf(x.scale_log2, -fexp), kLargest); // finite: a score of zero stays one
         }
         r.m[nt] = -INFINITY;
         r.l[nt] = 0.0f;
@@ -384,10 +386,11 @@ __device__ __forceinline__ void chunk_probs(const PagedAttnArgs& x, int tile, Ha
             s.l[nt] *= alpha;
             s.m[nt] = mn;
         }
-        const float bias = s.m[nt] == -INFINITY ? 0.0f : fmaf(-s.m[nt], s.rowmul[nt], kPOffset);
+        const float ref = s.m[nt] == -INFINITY ? 0.0f : s.m[nt];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            y.p[nt][i] = __builtin_amdgcn_exp2f(fmaf(sv[nt][i], s.rowmul[nt], bias));
+            // the difference first: -m * rowmul rounded would move every p by up to 2^(score 2^-25)
+            y.p[nt][i] = __builtin_amdgcn_exp2f(fmaf(sv[nt][i] - ref, s.rowmul[nt], kPOffset));
         }
         const float(&p)[8] = y.p[nt];
         s.l[nt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
@@ -1225,8 +1228,18 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
         __syncthreads();
     }
     float mul[NT]; // raw score of the FP16 K' -> log2 domain
+    // The products start from the running maximum's negative: scores come out less it (rounded with it, -m * mul would move
+    // every p by up to 2^(score 2^-25)). BF16 rows of 128 have no registers left for that: there it is added afterwards (8,192
+    // tokens 795 us, 816 with eight registers spilled). `lim`: what moves the maximum; -infinity before the first score.
+    constexpr bool kFromRef = !(BF && D == 128);
+    std::conditional_t<kFromRef, f4, float> ref[NT];
+    float lim[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) { mul[nt] = BF ? r.rowmul[nt] : r.rowmul[nt] / sc.k; }
+    for (int nt = 0; nt < NT; ++nt) {
+        mul[nt] = BF ? r.rowmul[nt] : fminf(r.rowmul[nt] / sc.k, kLargest);
+        ref[nt] = {};
+        lim[nt] = -INFINITY;
+    }
     // the wave's V^T reads: lane (c, g) addresses key 4 g + (c >> 2), dims 4 (c & 3) .. of a 16-dim segment
     const int vkey = 4 * g + (c >> 2);
     const int voff = vkey * 2 * D + 32 * (vkey & 7) + 8 * (c & 3);
@@ -1283,7 +1296,9 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
                     for (int k = 0; k < D / 32; ++k) {
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            const f4 acc = k == 0 ? f4{0.f, 0.f, 0.f, 0.f} : sacc[kt][nt];
+                            f4 acc = {0.f, 0.f, 0.f, 0.f};
+                            if constexpr (kFromRef) { acc = ref[nt]; }
+                            if (k > 0) { acc = sacc[kt][nt]; }
                             if constexpr (BF) {
                                 sacc[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, kf[kt][k]), __builtin_bit_cast(bf8, r.q[nt][k]), acc, 0, 0, 0);
                             } else {
@@ -1309,7 +1324,10 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) { sv[nt][i] = sacc[i >> 2][nt][i & 3]; }
+                    for (int i = 0; i < 8; ++i) {
+                        sv[nt][i] = sacc[i >> 2][nt][i & 3];
+                        if constexpr (!kFromRef) { sv[nt][i] += ref[nt]; }
+                    }
                 }
                 if (!all_seen(x, r.lo, r.hi, c0 >> 5, hv)) {
 #pragma unroll
@@ -1326,26 +1344,28 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     cmax[nt] = score_max(sv[nt]);
-                    any |= (cmax[nt] - r.m[nt]) * mul[nt] > kLazyTau;
+                    any |= cmax[nt] > lim[nt];
                 }
                 if (__any(any)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        const bool need = (cmax[nt] - r.m[nt]) * mul[nt] > kLazyTau;
-                        const float mn = need ? cmax[nt] : r.m[nt];
-                        const float alpha = need ? __builtin_amdgcn_exp2f((r.m[nt] - mn) * mul[nt]) : 1.0f;
+                        const bool need = cmax[nt] > lim[nt];
+                        const float up = need ? cmax[nt] : 0.0f;
+                        const float alpha = lim[nt] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-up * mul[nt]);
 #pragma unroll
                         for (int t = 0; t < D / 16; ++t) { r.O[nt][t] *= alpha; }
                         l[nt] *= alpha;
-                        r.m[nt] = mn;
+                        ref[nt] -= up;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) { sv[nt][i] -= up; }
+                        lim[nt] = need ? kLazyTau / mul[nt] : lim[nt];
                     }
                 }
                 h8 p[NT];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const float bias = r.m[nt] == -INFINITY ? 0.0f : fmaf(-r.m[nt], mul[nt], kPOffset);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) { p[nt][i] = static_cast<_Float16>(__builtin_amdgcn_exp2f(fmaf(sv[nt][i], mul[nt], bias))); }
+                    for (int i = 0; i < 8; ++i) { p[nt][i] = static_cast<_Float16>(__builtin_amdgcn_exp2f(fmaf(sv[nt][i], mul[nt], kPOffset))); }
                 }
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -1370,7 +1390,9 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
     float M[NT], L[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        M[nt] = r.m[nt] == -INFINITY ? -INFINITY : r.m[nt] * mul[nt];
+        float neg;
+        if constexpr (kFromRef) { neg = ref[nt][0]; } else { neg = ref[nt]; }
+        M[nt] = lim[nt] == -INFINITY ? -INFINITY : -neg * mul[nt];
         L[nt] = l[nt][0];
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) { r.O[nt][t] *= unit_v; }

@@ -15,7 +15,7 @@ def bound(case, tokens=None, kv_heads=None, dropped=()):
     it for FP32 sums of up to 256 products, 2^-22 of the scores for the exponent's argument, 2^-11 for P in FP16 and 2^-20
     for the exponential. With weights p' = p e^delta, |delta_j| <= d_j, the output moves by
     sum p_j (e^delta_j - 1) (v_j - o) / sum p_j e^delta_j; the same with every delta_j less the heaviest key's, whose term
-    is then zero. Values: 2^-11 of p_j |v_j| where INT8 rows are rounded; FP32 sums 2^-24 for each 32 keys and 64 more.
+    is then zero; and by 2 max |v| at most. Values: 2^-11 of p_j |v_j| where INT8 rows are rounded; FP32 sums 2^-24 for each 32 keys and 64 more.
     FP16's steps: p is held to 2^-33 of the heaviest, an INT8 weight p_j s_j to 2^-32 of the largest, a BF16 value to 2^-19 of
     the largest of its eight, seen keys only. The result is rounded to BF16, 2^-8 of itself at most."""
     i8 = case.kv == "i8"
@@ -55,8 +55,8 @@ def bound(case, tokens=None, kv_heads=None, dropped=()):
 
             def moved(d):
                 # p (e^d - 1) without p underflowing before e^d grows; |v - o| <= |v| + |o|
-                up = np.where(d < 1, p * np.expm1(np.minimum(d, 1)), np.exp(np.minimum(log_p + d, 700)))
-                return (up @ av + up.sum(-1, keepdims=True) * np.abs(out)) / (p * np.exp(-d)).sum(-1, keepdims=True)
+                up = np.where(d < 1, p * np.expm1(np.minimum(d, 1)), np.exp(np.minimum(log_p + d, 300)))
+                return (up @ av + up.sum(-1, keepdims=True) * np.abs(out)) / np.maximum((p * np.exp(-d)).sum(-1, keepdims=True), 1e-100)
             each = np.arange(G)
             far = d + d[each, heaviest][:, None]
             far[each, heaviest] = 0
@@ -68,7 +68,8 @@ def bound(case, tokens=None, kv_heads=None, dropped=()):
                 fp16 = fp16 + 2.0**-32 * len(rows) * np.repeat(largest, 64, -1)
             else:
                 fp16 = fp16 + 2.0**-19 * np.repeat(p @ av.reshape(len(rows), -1, 8).max(-1), 8, -1)
-            tol = 2.0**-8 * np.abs(out) + np.minimum(moved(d), moved(far)) + fp16 + 1e-38
+            move = np.minimum(np.minimum(moved(d), moved(far)), 2 * av.max(0))
+            tol = 2.0**-8 * np.abs(out) + move + fp16 + 1e-38
             tol += weight * ((2.0**-11 if i8 else 0.0) + 2.0**-24 * (len(rows) / 32 + 64))
             yield n, hh, out, tol
 

@@ -135,3 +135,17 @@ def test_values_near_the_top_of_bf16(gpu, geo, tokens, size, rows):
         part = slice(0 if rows == "all" else 350, None)
         c.v[0][part] = bf16_bits(x[part].astype(np.float32))
     _run(PagedCase([(tokens, 500), (2, 20)], Hq=Hq, Hkv=Hkv, D=D, kv="bf16", seed=36, edit=edit))
+
+
+@pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("geo", GEO)
+@pytest.mark.parametrize("tokens", [1, 3, 90])
+@pytest.mark.parametrize("size", [1e5, 1e6, 1e7, 1e9])
+def test_large_scores(gpu, kv, geo, tokens, size):
+    """Scores of about `size`: one key takes all the weight, and its values are the result."""
+    Hq, Hkv, D = GEO[geo]
+
+    def edit(c):
+        _grow(c.q, size / 1e3)
+        _grow(c.k[0], 1e3)
+    _run(PagedCase([(tokens, 400)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=39, edit=edit))
