@@ -139,6 +139,32 @@ def test_values_near_the_top_of_bf16(gpu, geo, tokens, size, rows):
 
 @pytest.mark.parametrize("kv", CACHES)
 @pytest.mark.parametrize("geo", GEO)
+@pytest.mark.parametrize("tokens", [1, 90])
+@pytest.mark.parametrize("size", [1e-4, 1e3, 3e4, 2e5])
+def test_size_of_values(gpu, kv, geo, tokens, size):
+    Hq, Hkv, D = GEO[geo]
+    _run(PagedCase([(tokens, 400)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=37, edit=lambda c: _grow(c.v[0], size)))
+
+
+@pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("geo", GEO)
+@pytest.mark.parametrize("tokens", [1, 90])
+@pytest.mark.parametrize("size", [1e3, 2e5])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_one_key_outgrows_the_others(gpu, kv, geo, tokens, size, sign):
+    """A key of `size` times the others takes all the weight (or none) of the tokens that see it."""
+    Hq, Hkv, D = GEO[geo]
+
+    def edit(c):
+        c.q[:, :, 1] = bf16_bits(np.float32(16.0 * sign))
+        c.k[0][390] = bf16_bits(np.float32(0.01) * bf16_values(c.k[0][390]))
+        c.k[0][390, :, 1] = bf16_bits(np.float32(1.0))
+        _grow(c.k[0][390], size)
+    _run(PagedCase([(tokens, 400)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=38, edit=edit))
+
+
+@pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("geo", GEO)
 @pytest.mark.parametrize("tokens", [1, 3, 90])
 @pytest.mark.parametrize("size", [1e5, 1e6, 1e7, 1e9])
 def test_large_scores(gpu, kv, geo, tokens, size):
