@@ -915,9 +915,8 @@ __device__ __forceinline__ void stage_trim(StageRegs<D, BF>& r, int live, int la
     }
 }
 
-// The largest magnitudes of a thread's part, NaN kept: K's and V's scales, or (BF16) V's values, a pair's as one FP32 number
-// (the upper value's size, off by less than BF16's step, or a number next to zero where only the lower one is not zero).
-// `least` (BF16): the smallest of its units' largest values, zeros aside, as bits less one.
+// The largest magnitudes of a thread's part, NaN kept: K's and V's scales, or (BF16) V's values. `least` (BF16): the smallest
+// of its units' largest values, zeros aside, as bits less one.
 struct StageSize {
     float k, v;
     uint32_t least;
@@ -931,7 +930,7 @@ __device__ __forceinline__ StageSize stage_size(const StageRegs<D, BF>& r) {
         if constexpr (BF) {
             float m = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) { m = fmax_ieee(m, fmax_ieee(fabsf(__uint_as_float(r.v[i][w] << 16)), fabsf(__uint_as_float(r.v[i][w])))); }
+            for (int w = 0; w < 4; ++w) { m = fmax_ieee(m, fmax_ieee(fabsf(__uint_as_float(r.v[i][w] << 16)), fabsf(__uint_as_float(r.v[i][w] & 0xffff0000u)))); }
             z.v = fmax_ieee(z.v, m);
             z.least = min(z.least, __float_as_uint(m) - 1u);
         } else {

@@ -26,7 +26,7 @@ def _run(c):
 @pytest.mark.parametrize("geo", GEO)
 @pytest.mark.parametrize("tokens", [1, 90])
 @pytest.mark.parametrize("size", [1e-4, 1e-6, 1e-7, 1e-8])
-@pytest.mark.parametrize("first", ["absent pages", "zero rows"])
+@pytest.mark.parametrize("first", ["absent pages", "zero rows", "zero rows of both signs"])
 def test_small_values_behind_an_empty_tile(gpu, kv, geo, tokens, size, first):
     """The first key tile of a workgroup holds no value that could tell how large the others are."""
     Hq, Hkv, D = GEO[geo]
@@ -36,6 +36,8 @@ def test_small_values_behind_an_empty_tile(gpu, kv, geo, tokens, size, first):
             _grow(x, size * (100 if kv == "i8" else 1))  # an INT8 value is at least its FP16 scale's smallest step
         if first == "zero rows":
             c.v[0][:256] = 0
+        if first == "zero rows of both signs":
+            c.v[0][:256] &= 0x8000
     absent = {(0, p) for p in range(16)} if first == "absent pages" else ()
     _run(PagedCase([(tokens, 400), (tokens, 30)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=30, absent=absent, edit=edit))
 
