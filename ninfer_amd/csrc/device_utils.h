@@ -114,6 +114,9 @@ __device__ __forceinline__ float group4_sum(float v) {
 
 // Two signed INT8 codes -> one packed FP16 pair, exactly: byte BYTE of `lo` -> low half, byte BYTE
 // of `hi` -> high half. One SDWA convert per code reads the byte in place (no shifts, no packing).
+// The result (as i8_bytes_to_f16x2's) has to go through another VALU instruction before an MFMA: the compiler keeps the wait
+// state between a partial write in inline asm and a VALU read of it, but an MFMA that read one two instructions later saw
+// stale halves.
 template <int BYTE>
 __device__ __forceinline__ uint32_t i8x2_to_f16x2(uint32_t lo, uint32_t hi) {
     uint32_t r;

@@ -11,8 +11,8 @@
 // V scales in the same way: w = p * s * 2^-E in FP16 (off by 2^-11 of itself, 2^-39 of the largest at least), times codes,
 // times 2^E in FP32. 2^E is the row's own: it tops w of the 32 keys at hand, so no scale is too large or too small,
 // and keys that the row does not see or that weigh nothing take no bits from the others. BF16 caches multiply stored
-// values; p goes in as two BF16 terms (16 bits).
-// Maxima, sums and accumulators are FP32.
+// values; p goes in as two BF16 terms (16 bits). Maxima, sums (of p as it is, before either rounding) and accumulators
+// are FP32. The many-row kernel rounds more, to keep the matrix cores fed; what it rounds stands there.
 #include "attn_math.h"
 #include "common.h"
 #include "device_utils.h"
@@ -111,8 +111,8 @@ __device__ __forceinline__ u2 out_pair(f4 O, float L) {
 // whose scores the S^T accumulator leaves in this lane; so P needs no exchange between lanes, and V is transposed
 // by byte selects alone. No LDS in the loop.
 //
-// What bounds it: HBM (31 flop a byte with INT8 rows and one row tile); the VALU converts and weighs 64% of the
-// time. Measured on MI355X: 32 single tokens over 535,000 ragged rows at 40/8/128 INT8 213 us (5.3 TB/s), 4 tokens over
+// What bounds it: HBM (31 flop a byte with INT8 rows and one row tile); the VALU converts and weighs 60% of the
+// time. Measured on MI355X: 32 single tokens over 535,000 ragged rows at 40/8/128 INT8 208 us (5.4 TB/s), 4 tokens over
 // 131,004 rows at 24/4/256 BF16 99 us (5.4 TB/s).
 
 template <int D, bool BF>
@@ -838,11 +838,12 @@ paged_attn_few_kernel(PagedAttnArgs x) {
 // value), rounded once (2^-11); BF16 values down to 2^-29 of the top are exact, smaller ones off by at most 2^-19 of the
 // largest of their unit of eight. A tile with a larger, infinite or NaN value, or with an INT8 scale or a BF16 unit below
 // 2^-18 of the top (other than zero) is left out, and its chunks are walked as the few-row kernel does it afterwards, which
-// has no such range.
+// has no such range but decodes each key in every wave (with every tile 2,370 instead of 790 us, as below; BF16 4,490).
+// P is FP16, off by 2^-11 of itself and 2^-33 of the row's largest, and its sum is that of the same rounded numbers.
 //
-// What bounds it: neither matrix cores (40% busy) nor VALU (60%) alone; a SIMD's two waves hardly overlap them, and the
+// What bounds it: neither matrix cores (40% busy) nor VALU (57%) alone; a SIMD's two waves hardly overlap them, and the
 // registers (256 each) leave no room for more work of one wave in flight. Measured on MI355X, 8,192 first tokens at
-// 40/8/128: INT8 805 us (855 TFLOP/s), BF16 781 us; at 24/4/256 1,162 and 1,082 us; a large library product reaches 1,318.
+// 40/8/128: INT8 790 us (870 TFLOP/s), BF16 785 us; at 24/4/256 1,167 and 1,097 us; a large library product reaches 1,318.
 
 constexpr int kManyThreads = 512;
 constexpr int kManyMarks = 131072;          // key tiles of a workgroup, at most
@@ -1002,7 +1003,8 @@ constexpr int kCus = 256;
 
 // What the choices below weigh, in us on MI355X: a key tile with WK = 1, 2, 4 waves per row tile (8,192 tokens, every WK
 // forced: 802, 1,054 and 1,574 us at head_dim 128, 1,161 and 1,614 us at 256, INT8), and a workgroup besides its tiles
-// (the batch's plan, the first page, the epilogue).
+// (the batch's plan, the first page, the epilogue). Half empty row tiles of one sequence's verify round fit too: 5 to 8 tokens
+// over 45,000 and 131,000 rows reckoned 49, 103, 65, 151 and 149 us, took 45, 90, 70, 160 and 136.
 __host__ __device__ constexpr float tile_us(int D, int wk) {
     return D == 128 ? (wk == 1 ? 4.9f : wk == 2 ? 3.2f : 2.6f) : (wk == 1 ? 2.95f : 2.05f);
 }
@@ -1229,7 +1231,7 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
     float mul[NT]; // raw score of the FP16 K' -> log2 domain
     // The products start from the running maximum's negative: scores come out less it (rounded with it, -m * mul would move
     // every p by up to 2^(score 2^-25)). BF16 rows of 128 have no registers left for that: there it is added afterwards (8,192
-    // tokens 795 us, 816 with eight registers spilled). `lim`: what moves the maximum; -infinity before the first score.
+    // tokens 785 us, 816 with eight registers spilled). `lim`: what moves the maximum; -infinity before the first score.
     constexpr bool kFromRef = !(BF && D == 128);
     std::conditional_t<kFromRef, f4, float> ref[NT];
     float lim[NT];
