@@ -397,20 +397,38 @@ __device__ __forceinline__ void chunk_probs(const PagedAttnArgs& x, int tile, Ha
     }
 }
 
-// The careful products' weights are p * 2^-kCareShift: a sum of 2^23 of them, each up to 2^15, times BF16's largest value
-// stays finite.
-constexpr int kCareShift = 40;
+// The careful products' weights are p * down. A sum of 2^23 weights, each up to 2^15, times values below 2^80 stays finite; where
+// there are larger ones `down` is 2^-40, which keeps sums of BF16's largest value finite (values below 2^-78 lose bits that way,
+// so not everywhere).
+constexpr uint32_t kCareTop = static_cast<uint32_t>(127 + 80) << 23; // 2^80
+constexpr float kCareDown = 0x1p-40f;
 
-// The (log2-domain maximum, sum) of a state whose outputs are in the careful products' units.
+// The (log2-domain maximum, sum) of a state whose outputs were made by the lower weights.
 __device__ __forceinline__ void care_units(float& M, float& L) {
-    M += static_cast<float>(kCareShift);
-    L = ldexpf(L, -kCareShift);
+    M += 40.0f;
+    L *= kCareDown;
 }
 
+// Tile `tile`'s pages; rows past `last` need none.
+__device__ __forceinline__ Halves halves_of(const PagedAttnArgs& x, const int32_t* table, int tile, int last) {
+    Halves hv;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+        const int key = 32 * tile + 16 * kt;
+        const int pg = key <= last ? table[key >> x.c.page_shift] : -1;
+        hv.page[kt] = __builtin_amdgcn_readfirstlane(pg >= 0 && pg < x.c.pages ? pg : -1);
+    }
+    return hv;
+}
+
+// A word of two BF16 values with zeros for infinite and NaN ones, and the bits of the larger one's magnitude.
+__device__ __forceinline__ uint32_t finite_word(uint32_t x) { return x & ~((nonfinite_bits(x) >> 15) * 0xffffu); }
+__device__ __forceinline__ uint32_t larger_bits(uint32_t x) { return max(x & 0x7fff0000u, (x << 16) & 0x7fff0000u); }
+
 // O^T += V^T P^T. CARE (BF16): infinite and NaN values reach only the rows that see them, finite ones overflow no sum; without
-// it they may make any row of the wave NaN.
+// it they may make any row of the wave NaN. `large`: the bits of the largest finite value so far (CARE).
 template <int D, bool BF, int NT, bool CARE>
-__device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const Probs<NT>& y, ChunkV<D, BF>& r, Rows<D, BF, NT>& s) {
+__device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const Probs<NT>& y, ChunkV<D, BF>& r, Rows<D, BF, NT>& s, float down, uint32_t& large) {
     using CK = Chunk<D, BF>;
     const float(&p)[NT][8] = y.p;
     if (!y.whole) {
@@ -476,7 +494,7 @@ __device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const P
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float z = CARE ? ldexpf(p[nt][k], -kCareShift) : p[nt][k];
+                const float z = CARE ? p[nt][k] * down : p[nt][k];
                 hi[nt][k] = static_cast<__bf16>(z);
                 lo[nt][k] = static_cast<__bf16>(z - static_cast<float>(hi[nt][k]));
             }
@@ -521,7 +539,10 @@ __device__ __forceinline__ void chunk_values(int tile, Halves hv, int g, const P
 #pragma unroll
                 for (int i = 0; i < CK::VP; ++i) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { r.v[k][i][e] &= ~((nonfinite_bits(r.v[k][i][e]) >> 15) * 0xffffu); }
+                    for (int e = 0; e < 4; ++e) {
+                        r.v[k][i][e] = finite_word(r.v[k][i][e]);
+                        large = max(large, larger_bits(r.v[k][i][e]));
+                    }
                 }
             }
         }
@@ -629,7 +650,7 @@ constexpr int few_waves(int D) { return D == 128 ? 2 : 1; }
 // A wave's tiles [j0, j1) of a sequence: the state of its rows.
 template <int D, bool BF, int NT, bool CARE>
 __device__ __forceinline__ void few_walk(const PagedAttnArgs& x, int h, const Seq& s, const Tiles& tiles, const int32_t* table, int j0, int j1, int c, int g,
-                                         Rows<D, BF, NT>& r) {
+                                         Rows<D, BF, NT>& r, float down) {
     const int lane = threadIdx.x & 63;
     const int end = s.history + s.tokens;
     // pages of 64 halves (32 tiles) at a time, one per lane, the next 64 fetched ahead
@@ -655,6 +676,7 @@ __device__ __forceinline__ void few_walk(const PagedAttnArgs& x, int h, const Se
         return hv;
     };
     Probs<NT> pr;
+    uint32_t large = 0u; // known already
     // registers for one chunk: its keys make room for the next ones' as soon as the scores are there, then its values
     ChunkK<D, BF> ka;
     ChunkV<D, BF> va;
@@ -670,7 +692,7 @@ __device__ __forceinline__ void few_walk(const PagedAttnArgs& x, int h, const Se
         __builtin_amdgcn_sched_barrier(0);
         load_keys<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, ka);
         __builtin_amdgcn_sched_barrier(0);
-        chunk_values<D, BF, NT, CARE>(tiles.tile(j), ha, g, pr, va, r);
+        chunk_values<D, BF, NT, CARE>(tiles.tile(j), ha, g, pr, va, r, down, large);
         __builtin_amdgcn_sched_barrier(0);
         load_values<D, BF>(x, h, tiles.tile(j + 1), hb, c, g, va);
         ha = hb;
@@ -697,8 +719,8 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
     }
     Rows<D, BF, NT> r;
     const int32_t* table = x.c.table + q.b * x.c.table_row;
-    few_walk<D, BF, NT, false>(x, h, s, tiles, table, j0, j1, c, g, r);
-    bool cared = false; // sums from 2^100 up, infinite ones or NaN: again, so that no sum of parts overflows either
+    few_walk<D, BF, NT, false>(x, h, s, tiles, table, j0, j1, c, g, r, 1.0f);
+    bool lower = false; // by the lower weights
     if constexpr (BF) {
         uint32_t top = 0u;
 #pragma unroll
@@ -709,8 +731,26 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
                 for (int e = 0; e < 4; ++e) { top = max(top, __float_as_uint(r.O[nt][t][e]) << 1); }
             }
         }
-        cared = __any(top >= static_cast<uint32_t>(127 + 100) << 24);
-        if (__builtin_expect(cared, 0)) { few_walk<D, BF, NT, true>(x, h, s, tiles, table, j0, j1, c, g, r); }
+        // sums from 2^100 up (no sum of parts may overflow either), infinite ones or NaN
+        if (__builtin_expect(__any(top >= static_cast<uint32_t>(127 + 100) << 24), 0)) {
+            uint32_t large = 0u;
+#pragma unroll 1
+            for (int j = j0; j < j1; ++j) {
+                const int tile = tiles.tile(j);
+                ChunkV<D, BF> cv;
+                load_values<D, BF>(x, h, tile, halves_of(x, table, tile, s.history + s.tokens - 1), c, g, cv);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+#pragma unroll
+                    for (int i = 0; i < Chunk<D, BF>::VP; ++i) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) { large = max(large, larger_bits(finite_word(cv.v[k][i][e]))); }
+                    }
+                }
+            }
+            lower = __any(large >= kCareTop);
+            few_walk<D, BF, NT, true>(x, h, s, tiles, table, j0, j1, c, g, r, lower ? kCareDown : 1.0f);
+        }
     }
     // ---- the waves' states into wave 0's: the upper half into the lower one, again and again
     float M[NT], L[NT];
@@ -718,7 +758,7 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
     for (int nt = 0; nt < NT; ++nt) {
         M[nt] = r.m[nt] == -INFINITY ? -INFINITY : r.m[nt] * r.rowmul[nt];
         L[nt] = group4_sum(r.l[nt]);
-        if (cared) { care_units(M[nt], L[nt]); }
+        if (lower) { care_units(M[nt], L[nt]); }
     }
     __syncthreads(); // the last part's states are read
     const auto halve = [&](int half) {
@@ -1404,48 +1444,51 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int t = 0; t < D / 16; ++t) {
-                *reinterpret_cast<f4*>(keep + (16 * nt + c) * D + 16 * t + 4 * g) = r.O[nt][t];
-                r.O[nt][t] = f4{0.f, 0.f, 0.f, 0.f};
-            }
-            r.m[nt] = -INFINITY;
-            r.l[nt] = 0.0f;
+            for (int t = 0; t < D / 16; ++t) { *reinterpret_cast<f4*>(keep + (16 * nt + c) * D + 16 * t + 4 * g) = r.O[nt][t]; }
         }
         __syncthreads();
+        uint32_t large = 0u;
+        bool lower = false;
 #pragma unroll 1
-        for (int base = 0; base < j1 - j0; base += 32) {
-            uint32_t bits = __builtin_amdgcn_readfirstlane(marks[base >> 5]);
-#pragma unroll 1
-            for (; bits != 0u; bits &= bits - 1u) {
-                const int key0 = tiles.tile(j0 + base + __builtin_ctz(bits)) * KT;
-#pragma unroll 1
-                for (int cw = 0; cw < MG::NCH / WK; ++cw) {
-                    const int c0 = key0 + 32 * (cw * WK + wk);
-                    if (c0 > r.hi) { continue; }
-                    Halves hv;
+        for (;;) {
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt) {
-                        const int key = c0 + 16 * kt;
-                        const int pg = key <= p1 ? table[key >> x.c.page_shift] : -1;
-                        hv.page[kt] = __builtin_amdgcn_readfirstlane(pg >= 0 && pg < x.c.pages ? pg : -1);
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) { r.O[nt][t] = f4{0.f, 0.f, 0.f, 0.f}; }
+                r.m[nt] = -INFINITY;
+                r.l[nt] = 0.0f;
+            }
+#pragma unroll 1
+            for (int base = 0; base < j1 - j0; base += 32) {
+                uint32_t bits = __builtin_amdgcn_readfirstlane(marks[base >> 5]);
+#pragma unroll 1
+                for (; bits != 0u; bits &= bits - 1u) {
+                    const int key0 = tiles.tile(j0 + base + __builtin_ctz(bits)) * KT;
+#pragma unroll 1
+                    for (int cw = 0; cw < MG::NCH / WK; ++cw) {
+                        const int tile = (key0 >> 5) + cw * WK + wk;
+                        if (32 * tile > r.hi) { continue; }
+                        const Halves hv = halves_of(x, table, tile, p1);
+                        Probs<NT> pr;
+                        {
+                            ChunkK<D, BF> ck;
+                            load_keys<D, BF>(x, h, tile, hv, c, g, ck);
+                            chunk_probs<D, BF, NT>(x, tile, hv, g, ck, r, pr);
+                        }
+                        __builtin_amdgcn_sched_barrier(0); // the registers hold one plane's rows at a time
+                        ChunkV<D, BF> cv;
+                        load_values<D, BF>(x, h, tile, hv, c, g, cv);
+                        chunk_values<D, BF, NT, BF>(tile, hv, g, pr, cv, r, lower ? kCareDown : 1.0f, large);
                     }
-                    Probs<NT> pr;
-                    {
-                        ChunkK<D, BF> ck;
-                        load_keys<D, BF>(x, h, c0 >> 5, hv, c, g, ck);
-                        chunk_probs<D, BF, NT>(x, c0 >> 5, hv, g, ck, r, pr);
-                    }
-                    __builtin_amdgcn_sched_barrier(0); // the registers hold one plane's rows at a time
-                    ChunkV<D, BF> cv;
-                    load_values<D, BF>(x, h, c0 >> 5, hv, c, g, cv);
-                    chunk_values<D, BF, NT, BF>(c0 >> 5, hv, g, pr, cv, r);
                 }
             }
+            if (!BF || lower || !__any(large >= kCareTop)) { break; }
+            lower = true; // again, by the lower weights
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float m2 = r.m[nt] == -INFINITY ? -INFINITY : r.m[nt] * r.rowmul[nt], l2 = group4_sum(r.l[nt]);
-            if constexpr (BF) { care_units(m2, l2); }
+            if (lower) { care_units(m2, l2); }
             const Weights q = weights(M[nt], L[nt], m2, l2);
             L[nt] = L[nt] * q.a + l2 * q.b;
             M[nt] = q.M;

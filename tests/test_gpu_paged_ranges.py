@@ -177,3 +177,19 @@ def test_large_scores(gpu, kv, geo, tokens, size):
         _grow(c.q, size / 1e3)
         _grow(c.k[0], 1e3)
     _run(PagedCase([(tokens, 400)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=39, edit=edit))
+
+
+@pytest.mark.parametrize("geo", GEO)
+@pytest.mark.parametrize("tokens", [1, 3, 90])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_values_near_the_bottom_of_bf16(gpu, geo, tokens, infinite):
+    """Values of 1e-33 behind larger ones in tiles of their own, with and without an infinite one that no token sees."""
+    Hq, Hkv, D = GEO[geo]
+    h, w = 700, 190
+
+    def edit(c):
+        _grow(c.v[0], 1e-33)
+        _grow(c.v[0][:520], 1e20)
+        if infinite:
+            c.v[0][h - w] = 0x7F80
+    _run(PagedCase([(tokens, h), (2, 20)], Hq=Hq, Hkv=Hkv, D=D, kv="bf16", window=w, seed=29, edit=edit))
