@@ -365,7 +365,7 @@ def _run_own(s, c):
         ops.paged_kv_read(s["cache"], v["starts"], v["history"], v["k_out"], v["v_out"])
         return s["q_out"], s["k_out"], s["v_out"]
     if c["kind"] == "means":
-        ops.paged_block_update(s["cache"], v["starts"], v["history"], s["blocks"])
+        ops.paged_block_update(s["cache"], v["starts"], v["history"], s["n"], s["blocks"])
         return s["codes"] * s["scales"][..., None]
     if c["kind"] == "select":
         ops.paged_block_select(v["q"], v["starts"], v["history"], v["table"], c["page"], s["blocks"], (c["first"], c["local"], c["top"]), s["envelope"],
