@@ -524,12 +524,11 @@ def _free_page(refs, k):
 def _copy_pages(s):
     src, dst = s["src"], s["dst"]
     live = (src >= 0) & (dst >= 0)
-    # a pair without pages copies the first pair's page again
-    src, dst = torch.where(live, src, src[0]).clamp(min=0).long(), torch.where(live, dst, dst[0]).clamp(min=0).long()
-    rows = [x.index_select(0, src) for x in s["pool"]]
-    live = live[:, None, None, None]
-    s["pool"][0][dst] = torch.where(live | live[0], rows[0], s["pool"][0][dst])
-    s["pool"][1][dst] = torch.where(live | live[0], rows[1], s["pool"][1][dst])
+    # a pair without pages copies a live pair's page again (where there is none, page 0 to itself)
+    one = live.to(torch.uint8).argmax(0, keepdim=True)
+    src, dst = (torch.where(live, x, x.index_select(0, one)).clamp(min=0).long() for x in (src, dst))
+    s["pool"][0][dst] = s["pool"][0].index_select(0, src)
+    s["pool"][1][dst] = s["pool"][1].index_select(0, src)
 
 
 def _fork(s, c):
