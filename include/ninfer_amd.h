@@ -120,6 +120,32 @@ typedef struct nmi_attention_window {
     uint32_t sinks;
 } nmi_attention_window;
 
+/* EXTENSION: the mean of every block of block_size key rows of a paged cache, next to its pages (so pages that sequences share
+ * share them): codes I8 [D, page_size / block_size, Hkv, pages], scales FP32 [page_size / block_size, Hkv, pages]; mean = code *
+ * scale. A page is contiguous, nb[3] of the codes any multiple of 16 bytes and nb[2] of the scales any multiple of 4 from a
+ * page's size up. block_size is a power of two from 32 to page_size. */
+typedef struct nmi_paged_block_view {
+    nmi_tensor codes;
+    nmi_tensor scales;
+    int32_t block_size;
+} nmi_paged_block_view;
+
+/* EXTENSION: the blocks that a token selects: the `first` first ones, the `local` (at least one) last ones up to its own, and
+ * of those between the `top` with the highest scores. */
+typedef struct nmi_block_selection {
+    int32_t first;
+    int32_t local;
+    int32_t top;
+} nmi_block_selection;
+
+/* EXTENSION: head norm and rotation: y = x / sqrt(mean(x^2) + eps) * (weight + weight_offset) (an offset of 1 for weights that
+ * are stored around zero), eps from 2^-60 to 1; pairs (y[i], y[i + R/2]) or, interleaved, (y[2i], y[2i+1]) of the first R dims. */
+typedef struct nmi_norm_rope {
+    float eps;
+    float weight_offset;
+    int32_t interleaved; /* 0 or 1 */
+} nmi_norm_rope;
+
 /* include/ninfer/ops/gqa_attention.h:13-16 */
 typedef struct nmi_gqa_envelope {
     uint32_t min_visible_keys;
@@ -279,6 +305,94 @@ int nmi_paged_attention(const nmi_tensor* q, const nmi_tensor* starts, const nmi
                         float scale, nmi_attention_window window, const nmi_paged_kv_layer_view* cache,
                         nmi_paged_envelope envelope, void* workspace, size_t workspace_bytes,
                         nmi_tensor* out, nmi_stream_t stream);
+
+/* ---------------------------------------------------------------- head norms and rotation (EXTENSION) */
+
+/* Every head of q and k normalised and rotated in one pass: pair i of a token at position p turns by p * inv_freq[i]. q/q_out
+ * BF16 [D, Hq, N], k/k_out BF16 [D, Hkv, N], head_dim 128 or 256, strides as for the paged ops (slices of a fused projection);
+ * weights BF16 or FP32 [D], NULL for ones; positions I32 [N]; inv_freq FP32 [R/2], R a multiple of 16 up to D, NULL for no
+ * rotation; dims from R on are normalised only. The angle is taken in 64 bits, the result rounded once. q_out may be q and k_out k
+ * (same data and strides); other overlaps of outputs with anything are not allowed. N at most 2^23. */
+int nmi_qk_norm_rope(const nmi_tensor* q, const nmi_tensor* k, const nmi_tensor* q_weight, const nmi_tensor* k_weight,
+                     const nmi_tensor* positions, const nmi_tensor* inv_freq, nmi_norm_rope norm, nmi_tensor* q_out,
+                     nmi_tensor* k_out, nmi_stream_t stream);
+
+/* The same at positions history[b] + i of packed sequences, with the keys and the values v (BF16 [D, Hkv, N]) appended to the
+ * paged cache in the pass: what nmi_qk_norm_rope and nmi_paged_kv_append leave, to the bit. Tokens of no sequence (or with a
+ * negative history) are left out, rows past the page table or in absent pages dropped (their q_out is written). */
+int nmi_paged_qk_norm_rope_append(const nmi_tensor* q, const nmi_tensor* k, const nmi_tensor* v, const nmi_tensor* q_weight,
+                                  const nmi_tensor* k_weight, const nmi_tensor* starts, const nmi_tensor* history,
+                                  const nmi_tensor* inv_freq, nmi_norm_rope norm, const nmi_paged_kv_layer_view* cache,
+                                  nmi_tensor* q_out, nmi_stream_t stream);
+
+/* ---------------------------------------------------------------- sparse attention over blocks (EXTENSION) */
+
+/* The means of the blocks that hold the new rows (history[b] .. of `tokens` packed tokens; the rows are in the cache already),
+ * each over the block's rows up to the sequence's last one: sums in 64 bits, step = max |sum| / 127 over the head, code = rne(sum *
+ * (1 / step)), scale = FP32(step / rows). A block with an infinite or NaN key gets codes 0 and an infinite scale. Blocks past
+ * the page table or in absent pages are left out. */
+int nmi_paged_block_update(const nmi_paged_kv_layer_view* cache, const nmi_tensor* starts, const nmi_tensor* history,
+                           int32_t tokens, const nmi_paged_block_view* blocks, nmi_stream_t stream);
+
+/* For every token and KV head the blocks to attend over, I32 [first + local + top, Hkv, N], ascending, -1 behind the last. Token
+ * at position p: its own block is o = p / block_size; blocks c < first and c > o - local are always taken, of first <= c <= o -
+ * local (those whose page is there) the `top` highest scores, the lower c of equals. score(c) = FP32(scale_c * <u, codes_c>), with u
+ * the codes (made as the means') of the sum of the group's query heads; a block with an infinite scale comes first. The means of those
+ * blocks have to be up to date. A sequence outside the envelope is left out: its lists stay as they were. At most 1,024 selected
+ * blocks, 2^23 rows and 32,768 blocks of a sequence. Workspace from the query, for the same arguments (it may be 0). */
+size_t nmi_paged_block_select_workspace_bytes(int32_t kv_heads, int32_t head_dim, int32_t tokens, int32_t batch,
+                                              nmi_paged_envelope envelope, int32_t block_size);
+int nmi_paged_block_select(const nmi_tensor* q, const nmi_tensor* starts, const nmi_tensor* history,
+                           const nmi_tensor* page_table, int32_t page_size, const nmi_paged_block_view* blocks,
+                           nmi_block_selection selection, nmi_paged_envelope envelope, void* workspace,
+                           size_t workspace_bytes, nmi_tensor* selected, nmi_stream_t stream);
+
+/* nmi_paged_attention over the rows of selected blocks alone: a token at position p sees the rows j <= p of the blocks that its
+ * list (selected I32 [S, Hkv, N], S at most 1,024) holds for the KV head. Entries that are negative or past the token's own block are no
+ * block, one that stands twice counts twice; any order. A token that sees no row gets zeros. block_size is a power of two from 32
+ * to 4,096, whatever the page_size. A sequence outside the envelope is left out. */
+size_t nmi_paged_sparse_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t tokens,
+                                                  int32_t batch, int32_t selected_blocks, int32_t block_size);
+int nmi_paged_sparse_attention(const nmi_tensor* q, const nmi_tensor* starts, const nmi_tensor* history, float scale,
+                               const nmi_tensor* selected, int32_t block_size, const nmi_paged_kv_layer_view* cache,
+                               nmi_paged_envelope envelope, void* workspace, size_t workspace_bytes, nmi_tensor* out,
+                               nmi_stream_t stream);
+
+/* ---------------------------------------------------------------- pages (EXTENSION) */
+
+/* refs I32 [pages] counts the entries of the page table (or tables) that hold a page; a page without any is free. The ops below keep
+ * the counts, and everything is done on the device, so a scheduler's step can be captured. A pool has at most 2^19 pages here. */
+
+/* Page src[i] to page dst[i] of the cache, bit by bit, with its block means where `blocks` is not NULL. src/dst I32 [n]; a pair with an
+ * entry outside the pool, or twice the same, is left out. No page may be written by two pairs or both written and read. */
+int nmi_paged_kv_copy_pages(const nmi_paged_kv_layer_view* cache, const nmi_paged_block_view* blocks, const nmi_tensor* src,
+                            const nmi_tensor* dst, nmi_stream_t stream);
+
+/* Pages for the new rows history[b] .. of the packed tokens: every absent entry of theirs gets a free page, the lowest first, in
+ * the order of the sequences and their entries. granted I32 [B]: the sequence's new tokens whose rows all have a page now (all of them
+ * unless the pool or the table ends). */
+int nmi_paged_pages_reserve(nmi_tensor* page_table, nmi_tensor* refs, const nmi_tensor* starts, const nmi_tensor* history,
+                            int32_t page_size, nmi_tensor* granted, nmi_stream_t stream);
+
+/* Sequence sequences[i] keeps the pages of its first keep_rows[i] rows and gives the others back (0: all of them). I32 [n], n up to
+ * 65,536; entries that name no sequence or a negative number of rows are left out. */
+int nmi_paged_pages_release(nmi_tensor* page_table, nmi_tensor* refs, const nmi_tensor* sequences, const nmi_tensor* keep_rows,
+                            int32_t page_size, nmi_stream_t stream);
+
+/* Sequence children[i] becomes a copy of parents[i] (I32 [n], n up to 1,024) with history[parent] rows: it shares the whole pages
+ * and gets a page of its own for the rest (the lowest free ones, in order), which nmi_paged_kv_copy_pages(src, dst) fills
+ * in every layer; src/dst I32 [n], -1 where there is nothing to copy. history I32 [B]: the child's becomes the parent's, or, where
+ * no page is left, its whole pages' rows. What the child held before is given back (not for use in the same call). A pair that names no
+ * sequence, whose child is a parent of any pair, or an earlier pair's child, is left out. */
+int nmi_paged_pages_fork(nmi_tensor* page_table, nmi_tensor* refs, const nmi_tensor* parents, const nmi_tensor* children,
+                         nmi_tensor* history, int32_t page_size, nmi_tensor* src, nmi_tensor* dst, nmi_stream_t stream);
+
+/* Moves pages together: the highest page in use to the lowest free one, the next highest to the next, while that lies below it, up
+ * to n moves (src/dst I32 [n], -1 behind the last; moved I32 [1]: how many). The table's entries and the counts follow at once; the
+ * pages' contents move by nmi_paged_kv_copy_pages(src, dst) in every layer. All tables that hold pages of the pool have to be
+ * this one. */
+int nmi_paged_pages_compact(nmi_tensor* page_table, nmi_tensor* refs, nmi_tensor* src, nmi_tensor* dst, nmi_tensor* moved,
+                            nmi_stream_t stream);
 
 /* ---------------------------------------------------------------- acceptance (part b) */
 

@@ -141,6 +141,22 @@ struct PagedKVCacheLayerView {
     }
 };
 
+// Extension: means of blocks of a paged cache's keys (nmi_paged_block_view).
+struct PagedBlockView {
+    Tensor codes, scales;
+    int32_t block_size = 0;
+
+    nmi_paged_block_view c() const {
+        nmi_paged_block_view r{};
+        r.codes = codes.c();
+        r.scales = scales.c();
+        r.block_size = block_size;
+        return r;
+    }
+};
+
+using BlockSelection = nmi_block_selection;
+using NormRope = nmi_norm_rope;
 using PagedExecutionEnvelope = nmi_paged_envelope;
 using AttentionWindow = nmi_attention_window;
 using GqaExecutionEnvelope = nmi_gqa_envelope;
@@ -181,6 +197,16 @@ inline void check(int status) {
     throw std::runtime_error(msg);
 }
 inline nmi_stream_t st(hipStream_t s) { return reinterpret_cast<nmi_stream_t>(s); }
+
+// A tensor that may be left out.
+struct Optional {
+    nmi_tensor t{};
+    bool there = false;
+    explicit Optional(const Tensor* p) : there(p != nullptr) {
+        if (there) { t = p->c(); }
+    }
+    const nmi_tensor* get() const { return there ? &t : nullptr; }
+};
 } // namespace detail
 
 namespace ops {
@@ -416,6 +442,120 @@ inline void paged_attention(const Tensor& q, const Tensor& starts, const Tensor&
     nmi_tensor co = out.c();
     const nmi_paged_kv_layer_view view = cache.c();
     detail::check(nmi_paged_attention(&cq, &cs, &ch, scale, window, &view, envelope, ws, need, &co, detail::st(stream)));
+}
+
+// ---- head norms and rotation (extension) --------------------------------------------------------------
+
+// Every head of q and k normalised, times its weight (null: ones), rotated by positions * inv_freq (null: not) in one pass.
+inline void qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor* q_weight, const Tensor* k_weight, const Tensor& positions,
+                         const Tensor* inv_freq, NormRope norm, Tensor& q_out, Tensor& k_out, hipStream_t stream) {
+    const nmi_tensor cq = q.c(), ck = k.c(), cp = positions.c();
+    const detail::Optional qw(q_weight), kw(k_weight), freq(inv_freq);
+    nmi_tensor cqo = q_out.c(), cko = k_out.c();
+    detail::check(nmi_qk_norm_rope(&cq, &ck, qw.get(), kw.get(), &cp, freq.get(), norm, &cqo, &cko, detail::st(stream)));
+}
+
+// The same at the packed tokens' positions, the keys and values appended to the cache in the pass.
+inline void paged_qk_norm_rope_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor* q_weight, const Tensor* k_weight,
+                                      const Tensor& starts, const Tensor& history, const Tensor* inv_freq, NormRope norm,
+                                      const PagedKVCacheLayerView& cache, Tensor& q_out, hipStream_t stream) {
+    const nmi_tensor cq = q.c(), ck = k.c(), cv = v.c(), cs = starts.c(), ch = history.c();
+    const detail::Optional qw(q_weight), kw(k_weight), freq(inv_freq);
+    const nmi_paged_kv_layer_view view = cache.c();
+    nmi_tensor cqo = q_out.c();
+    detail::check(nmi_paged_qk_norm_rope_append(&cq, &ck, &cv, qw.get(), kw.get(), &cs, &ch, freq.get(), norm, &view, &cqo, detail::st(stream)));
+}
+
+// ---- sparse attention over blocks of a paged cache (extension) -----------------------------------------
+
+// The means of the blocks that hold the rows of the `tokens` packed tokens, which are in the cache already.
+inline void paged_block_update(const PagedKVCacheLayerView& cache, const Tensor& starts, const Tensor& history, int32_t tokens,
+                               const PagedBlockView& blocks, hipStream_t stream) {
+    const nmi_tensor cs = starts.c(), ch = history.c();
+    const nmi_paged_kv_layer_view view = cache.c();
+    const nmi_paged_block_view bv = blocks.c();
+    detail::check(nmi_paged_block_update(&view, &cs, &ch, tokens, &bv, detail::st(stream)));
+}
+
+[[nodiscard]] inline std::size_t paged_block_select_workspace_bytes(int32_t kv_heads, int32_t head_dim, int32_t tokens, int32_t batch,
+                                                                    PagedExecutionEnvelope envelope, int32_t block_size) {
+    return nmi_paged_block_select_workspace_bytes(kv_heads, head_dim, tokens, batch, envelope, block_size);
+}
+
+// For every token and KV head the selection's blocks, ascending, -1 behind them.
+inline void paged_block_select(const Tensor& q, const Tensor& starts, const Tensor& history, const Tensor& page_table, int32_t page_size,
+                               const PagedBlockView& blocks, BlockSelection selection, PagedExecutionEnvelope envelope,
+                               WorkspaceArena& workspace, Tensor& selected, hipStream_t stream) {
+    auto scope = workspace.scope();
+    const nmi_paged_block_view bv = blocks.c();
+    const std::size_t need =
+        paged_block_select_workspace_bytes(bv.codes.ne[2], q.ne[0], q.ne[2], page_table.ne[1], envelope, blocks.block_size);
+    void* ws = need ? workspace.alloc_bytes(need) : nullptr;
+    const nmi_tensor cq = q.c(), cs = starts.c(), ch = history.c(), ct = page_table.c();
+    nmi_tensor co = selected.c();
+    detail::check(nmi_paged_block_select(&cq, &cs, &ch, &ct, page_size, &bv, selection, envelope, ws, need, &co, detail::st(stream)));
+}
+
+[[nodiscard]] inline std::size_t paged_sparse_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t tokens,
+                                                                        int32_t batch, int32_t selected_blocks, int32_t block_size) {
+    return nmi_paged_sparse_attention_workspace_bytes(q_heads, kv_heads, head_dim, tokens, batch, selected_blocks, block_size);
+}
+
+// paged_attention over the rows of the blocks that each token's list holds for the KV head (negative: none).
+inline void paged_sparse_attention(const Tensor& q, const Tensor& starts, const Tensor& history, float scale, const Tensor& selected,
+                                   int32_t block_size, const PagedKVCacheLayerView& cache, PagedExecutionEnvelope envelope,
+                                   WorkspaceArena& workspace, Tensor& out, hipStream_t stream) {
+    auto scope = workspace.scope();
+    const std::size_t need = paged_sparse_attention_workspace_bytes(q.ne[1], cache.num_kv_heads, q.ne[0], q.ne[2], cache.page_table.ne[1],
+                                                                    selected.ne[0], block_size);
+    void* ws = need ? workspace.alloc_bytes(need) : nullptr;
+    const nmi_tensor cq = q.c(), cs = starts.c(), ch = history.c(), cl = selected.c();
+    nmi_tensor co = out.c();
+    const nmi_paged_kv_layer_view view = cache.c();
+    detail::check(
+        nmi_paged_sparse_attention(&cq, &cs, &ch, scale, &cl, block_size, &view, envelope, ws, need, &co, detail::st(stream)));
+}
+
+// ---- pages of a paged cache (extension) ------------------------------------------------------------------
+
+// Page src[i] to page dst[i] (negative: none), with its block means where `blocks` is not null.
+inline void paged_kv_copy_pages(const PagedKVCacheLayerView& cache, const PagedBlockView* blocks, const Tensor& src, const Tensor& dst,
+                                hipStream_t stream) {
+    const nmi_tensor cs = src.c(), cd = dst.c();
+    const nmi_paged_kv_layer_view view = cache.c();
+    nmi_paged_block_view bv{};
+    if (blocks != nullptr) { bv = blocks->c(); }
+    detail::check(nmi_paged_kv_copy_pages(&view, blocks != nullptr ? &bv : nullptr, &cs, &cd, detail::st(stream)));
+}
+
+// Free pages (the lowest first) for the new rows that have none; granted[b]: the new tokens of b that have theirs.
+inline void paged_pages_reserve(Tensor& page_table, Tensor& refs, const Tensor& starts, const Tensor& history, int32_t page_size,
+                                Tensor& granted, hipStream_t stream) {
+    const nmi_tensor cs = starts.c(), ch = history.c();
+    nmi_tensor ct = page_table.c(), cr = refs.c(), cg = granted.c();
+    detail::check(nmi_paged_pages_reserve(&ct, &cr, &cs, &ch, page_size, &cg, detail::st(stream)));
+}
+
+// Sequence sequences[i] gives back the pages past its first keep_rows[i] rows.
+inline void paged_pages_release(Tensor& page_table, Tensor& refs, const Tensor& sequences, const Tensor& keep_rows, int32_t page_size,
+                                hipStream_t stream) {
+    const nmi_tensor cs = sequences.c(), ck = keep_rows.c();
+    nmi_tensor ct = page_table.c(), cr = refs.c();
+    detail::check(nmi_paged_pages_release(&ct, &cr, &cs, &ck, page_size, detail::st(stream)));
+}
+
+// Sequence children[i] as a copy of parents[i]: whole pages shared, the rest in a page of its own that paged_kv_copy_pages fills.
+inline void paged_pages_fork(Tensor& page_table, Tensor& refs, const Tensor& parents, const Tensor& children, Tensor& history,
+                             int32_t page_size, Tensor& src, Tensor& dst, hipStream_t stream) {
+    const nmi_tensor cp = parents.c(), cc = children.c();
+    nmi_tensor ct = page_table.c(), cr = refs.c(), ch = history.c(), cs = src.c(), cd = dst.c();
+    detail::check(nmi_paged_pages_fork(&ct, &cr, &cp, &cc, &ch, page_size, &cs, &cd, detail::st(stream)));
+}
+
+// The highest pages in use to the lowest free ones: table and counts now, contents by paged_kv_copy_pages.
+inline void paged_pages_compact(Tensor& page_table, Tensor& refs, Tensor& src, Tensor& dst, Tensor& moved, hipStream_t stream) {
+    nmi_tensor ct = page_table.c(), cr = refs.c(), cs = src.c(), cd = dst.c(), cm = moved.c();
+    detail::check(nmi_paged_pages_compact(&ct, &cr, &cs, &cd, &cm, detail::st(stream)));
 }
 
 // ---- lm_head ----------------------------------------------------------------------------------------

@@ -9,12 +9,13 @@ Layers:
 from __future__ import annotations
 
 from . import _capi
-from ._capi import (BF16, FP16, FP32, I8, I32, I64, U8, AttentionWindow, CommitEnvelope, CyclicKVLayerView, GeneralConfig,
-                    GqaEnvelope, KVLayerView, PagedEnvelope, PagedKVLayerView, SamplingConfig, Tensor, Weight, lib)
+from ._capi import (BF16, FP16, FP32, I8, I32, I64, U8, AttentionWindow, BlockSelection, CommitEnvelope, CyclicKVLayerView,
+                    GeneralConfig, GqaEnvelope, KVLayerView, NormRope, PagedBlockView, PagedEnvelope, PagedKVLayerView, SamplingConfig,
+                    Tensor, Weight, lib)
 
 __all__ = [
     "BF16", "FP16", "FP32", "I8", "I32", "I64", "Tensor", "KVLayerView", "CyclicKVLayerView", "GqaEnvelope",
-    "Weight", "PagedKVLayerView", "PagedEnvelope", "AttentionWindow",
+    "Weight", "PagedKVLayerView", "PagedEnvelope", "AttentionWindow", "PagedBlockView", "BlockSelection", "NormRope",
     "CommitEnvelope", "SamplingConfig", "GeneralConfig", "lib", "build_info",
 ]
 

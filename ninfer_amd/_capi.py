@@ -130,6 +130,20 @@ class AttentionWindow(C.Structure):
     _fields_ = [("size", C.c_uint32), ("sinks", C.c_uint32)]
 
 
+class PagedBlockView(C.Structure):
+    """nmi_paged_block_view."""
+
+    _fields_ = [("codes", Tensor), ("scales", Tensor), ("block_size", C.c_int32)]
+
+
+class BlockSelection(C.Structure):
+    _fields_ = [("first", C.c_int32), ("local", C.c_int32), ("top", C.c_int32)]
+
+
+class NormRope(C.Structure):
+    _fields_ = [("eps", C.c_float), ("weight_offset", C.c_float), ("interleaved", C.c_int32)]
+
+
 class GqaEnvelope(C.Structure):
     _fields_ = [("min_visible_keys", C.c_uint32), ("max_visible_keys", C.c_uint32)]
 
@@ -179,6 +193,20 @@ _SIGNATURES = {
                                                          AttentionWindow]),
     "nmi_paged_attention": (C.c_int, [_T, _T, _T, C.c_float, AttentionWindow, P(PagedKVLayerView), PagedEnvelope, C.c_void_p,
                                       C.c_size_t, _T, _STREAM]),
+    "nmi_qk_norm_rope": (C.c_int, [_T, _T, _T, _T, _T, _T, NormRope, _T, _T, _STREAM]),
+    "nmi_paged_qk_norm_rope_append": (C.c_int, [_T, _T, _T, _T, _T, _T, _T, _T, NormRope, P(PagedKVLayerView), _T, _STREAM]),
+    "nmi_paged_block_update": (C.c_int, [P(PagedKVLayerView), _T, _T, C.c_int32, P(PagedBlockView), _STREAM]),
+    "nmi_paged_block_select_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, PagedEnvelope, C.c_int32]),
+    "nmi_paged_block_select": (C.c_int, [_T, _T, _T, _T, C.c_int32, P(PagedBlockView), BlockSelection, PagedEnvelope, C.c_void_p, C.c_size_t,
+                                         _T, _STREAM]),
+    "nmi_paged_sparse_attention_workspace_bytes": (C.c_size_t, [C.c_int32] * 7),
+    "nmi_paged_sparse_attention": (C.c_int, [_T, _T, _T, C.c_float, _T, C.c_int32, P(PagedKVLayerView), PagedEnvelope, C.c_void_p,
+                                             C.c_size_t, _T, _STREAM]),
+    "nmi_paged_kv_copy_pages": (C.c_int, [P(PagedKVLayerView), P(PagedBlockView), _T, _T, _STREAM]),
+    "nmi_paged_pages_reserve": (C.c_int, [_T, _T, _T, _T, C.c_int32, _T, _STREAM]),
+    "nmi_paged_pages_release": (C.c_int, [_T, _T, _T, _T, C.c_int32, _STREAM]),
+    "nmi_paged_pages_fork": (C.c_int, [_T, _T, _T, _T, _T, C.c_int32, _T, _T, _STREAM]),
+    "nmi_paged_pages_compact": (C.c_int, [_T, _T, _T, _T, _T, _STREAM]),
     "nmi_argmax": (C.c_int, [_T, _T, C.c_int32, _STREAM]),
     "nmi_sampling_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
     "nmi_speculative_prepare_verify_inputs": (C.c_int, [_T, _T, _T, _T, _T, _STREAM]),

@@ -1,0 +1,217 @@
+// Head norms of queries and keys with the rotation by position in the same pass on gfx950; on its way into a paged KV
+// cache, the keys (and the values) are appended in that pass too.
+//
+// Mathematics: for every head x of a token at position p, y = x / sqrt(mean(x^2) + eps) * (weight + offset); pair i of the
+// rotated dims, (a, b) = (y[i], y[i + half]) or interleaved (y[2i], y[2i + 1]), becomes (a cos t - b sin t, b cos t + a sin t)
+// with t = p * inv_freq[i]; one rounding to BF16 at the end. The append is that of paged_cache.hip, to the bit.
+//
+// Numbers: t in turns is p * (inv_freq / 2 pi) in 64 bits, less its nearest whole number, so a far position loses nothing (in
+// 32 bits a position of 2^23 would be half a radian off); sine and cosine of what is left are FP32, the sum of squares too,
+// scaled down first where it passes FP32's range.
+//
+// What bounds it: HBM for prompts, launch and the chain token -> sequence -> page for decode steps.
+#include "common.h"
+#include "device_utils.h"
+#include "kv_codec.h"
+#include "paged_internal.h"
+
+#include <algorithm>
+
+namespace nmi {
+namespace {
+
+struct NormRopeArgs {
+    NormRope a;
+    PagedRef c;
+};
+
+// The sum over the D / 8 lanes of a head, in every one of them.
+template <int D>
+__device__ __forceinline__ float head_sum(float v) {
+    v += dpp_from<0xB1, 0xf>(v, 0.0f);  // lane ^ 1
+    v += dpp_from<0x4E, 0xf>(v, 0.0f);  // lane ^ 2
+    v += dpp_from<0x141, 0xf>(v, 0.0f); // the other four of eight
+    v += dpp_from<0x140, 0xf>(v, 0.0f); // the other eight of sixteen
+    if constexpr (D == 256) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
+__device__ __forceinline__ float bf16_of(i4 raw, int e) {
+    const uint32_t w = static_cast<uint32_t>(raw[e >> 1]);
+    return __uint_as_float((e & 1) ? w & 0xffff0000u : w << 16);
+}
+
+// Eight weights from dim d on, the offset added.
+__device__ __forceinline__ void load_weights(const void* w, bool f32, float offset, int d, float (&y)[8]) {
+    if (w == nullptr) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { y[e] = 1.0f + offset; }
+    } else if (f32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { y[e] = static_cast<const float*>(w)[d + e] + offset; }
+    } else {
+        const i4 raw = *reinterpret_cast<const i4*>(static_cast<const uint16_t*>(w) + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { y[e] = bf16_of(raw, e) + offset; }
+    }
+}
+
+// A workgroup per token (and share of its heads): D / 8 lanes a head, eight dims a lane.
+template <int D, bool APPEND>
+__global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs x) {
+    constexpr int L = D / 8;       // lanes of a head
+    constexpr int HEADS = 256 / L; // heads of a pass
+    __shared__ float2 turn[D / 2];
+    const NormRope& a = x.a;
+    const int64_t n = blockIdx.x;
+    const int li = threadIdx.x & (L - 1);
+    const int step = HEADS * gridDim.y;
+    const int heads = a.Hq + a.Hkv + (APPEND ? a.Hkv : 0);
+    const auto load = [&](int head) {
+        const PackedRef& src = head < a.Hq ? a.q : head < a.Hq + a.Hkv ? a.k : a.v;
+        const int of = head < a.Hq ? head : head < a.Hq + a.Hkv ? head - a.Hq : head - a.Hq - a.Hkv;
+        return *reinterpret_cast<const i4*>(src.data + n * src.token_stride + (of * D + 8 * li) * 2);
+    };
+    int head = blockIdx.y * HEADS + threadIdx.x / L;
+    i4 raw = {0, 0, 0, 0};
+    if (head < heads) { raw = load(head); }
+
+    int64_t pos;
+    int32_t page = -1, row = 0;
+    if constexpr (APPEND) {
+        // the last sequence that starts at or before the token
+        int count = 0;
+        for (int i = threadIdx.x; i - static_cast<int>(threadIdx.x) < x.c.B; i += 256) { count += __syncthreads_count(i < x.c.B && a.starts[i] <= n); }
+        if (count == 0) { return; }
+        const int b = count - 1;
+        const int32_t start = a.starts[b], end = a.starts[b + 1], history = a.history[b];
+        if (start < 0 || n < start || n >= end || history < 0) { return; } // of no sequence
+        pos = static_cast<int64_t>(history) + (n - start);
+        if ((pos >> x.c.page_shift) < x.c.max_pages) {
+            page = x.c.table[b * x.c.table_row + (pos >> x.c.page_shift)];
+            page = page >= 0 && page < x.c.pages ? page : -1;
+            row = static_cast<int32_t>(pos & ((int64_t{1} << x.c.page_shift) - 1));
+        }
+    } else {
+        pos = a.positions[n];
+    }
+    for (int i = threadIdx.x; i < a.half; i += 256) {
+        double t = static_cast<double>(pos) * (static_cast<double>(a.inv_freq[i]) * 0.15915494309189533577);
+        t -= rint(t);
+        float s, c;
+        sincospif(static_cast<float>(2.0 * t), &s, &c);
+        turn[i] = float2{c, s};
+    }
+    // the lane's dims, its partner's lane, and the weights of both
+    const int lanes = a.half / 8; // lanes of half a rotated part
+    const bool rotated = 8 * li < 2 * a.half;
+    const bool upper = !a.interleaved && li >= lanes; // b of its pairs
+    const int partner = !rotated || a.interleaved ? li : upper ? li - lanes : li + lanes;
+    float qw[8], kw[8], qp[8], kp[8];
+    load_weights(a.q_weight, a.q_weight_f32, a.offset, 8 * li, qw);
+    load_weights(a.k_weight, a.k_weight_f32, a.offset, 8 * li, kw);
+    load_weights(a.q_weight, a.q_weight_f32, a.offset, 8 * partner, qp);
+    load_weights(a.k_weight, a.k_weight_f32, a.offset, 8 * partner, kp);
+    __syncthreads();
+    float cs[8], sn[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        cs[e] = 1.0f;
+        sn[e] = 0.0f;
+        if (rotated) {
+            const float2 z = turn[a.interleaved ? 4 * li + (e >> 1) : 8 * (upper ? li - lanes : li) + e];
+            cs[e] = z.x;
+            sn[e] = a.interleaved ? ((e & 1) ? z.y : -z.y) : upper ? z.y : -z.y;
+        }
+    }
+
+    for (; head < heads; head += step) {
+        i4 next = {0, 0, 0, 0};
+        if (head + step < heads) { next = load(head + step); }
+        const bool key = head >= a.Hq;
+        i4 out = raw;
+        if (!APPEND || head < a.Hq + a.Hkv) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { ss = fmaf(bf16_of(raw, e), bf16_of(raw, e), ss); }
+            ss = head_sum<D>(ss);
+            float r = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
+            if (__builtin_expect(__any(ss > 0x1p120f), 0)) { // beyond FP32's squares: 2^-70 of the values, eps is nothing next to them
+                float s2 = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float z = bf16_of(raw, e) * 0x1p-70f;
+                    s2 = fmaf(z, z, s2);
+                }
+                s2 = head_sum<D>(s2);
+                if (ss > 0x1p120f) { r = 0x1p-70f / sqrtf(s2 * (1.0f / D)); }
+            }
+            i4 other = raw;
+            if (!a.interleaved) {
+                const int from = 4 * ((threadIdx.x & 63 & ~(L - 1)) + partner);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) { other[w] = __builtin_amdgcn_ds_bpermute(from, raw[w]); }
+            }
+            uint32_t bits[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = bf16_of(raw, e) * r * (key ? kw[e] : qw[e]);
+                const int pe = a.interleaved ? e ^ 1 : e;
+                const float w = a.interleaved ? (key ? kw[e ^ 1] : qw[e ^ 1]) : (key ? kp[e] : qp[e]);
+                const float z = (a.interleaved ? bf16_of(raw, e ^ 1) : bf16_of(other, pe)) * r * w;
+                bits[e] = f32_to_bf16_bits(rotated ? y * cs[e] + z * sn[e] : y);
+            }
+#pragma unroll
+            for (int w = 0; w < 4; ++w) { out[w] = static_cast<int>(bits[2 * w] | (bits[2 * w + 1] << 16)); }
+        }
+        if (head < a.Hq) {
+            *reinterpret_cast<i4*>(a.q_out.data + n * a.q_out.token_stride + (head * D + 8 * li) * 2) = out;
+        } else if constexpr (!APPEND) {
+            *reinterpret_cast<i4*>(a.k_out.data + n * a.k_out.token_stride + ((head - a.Hq) * D + 8 * li) * 2) = out;
+        } else if (page >= 0) {
+            const bool value = head >= a.Hq + a.Hkv;
+            const int64_t at = (static_cast<int64_t>(head - a.Hq - (value ? a.Hkv : 0)) << x.c.page_shift) + row;
+            char* dst = value ? x.c.v + page * x.c.v_page : x.c.k + page * x.c.k_page;
+            if (x.c.bf16) {
+                *reinterpret_cast<i4*>(dst + (at * D + 8 * li) * 2) = out;
+            } else {
+                uint16_t scale;
+                const i2 code = quantize_g64(out, scale);
+                *reinterpret_cast<i2*>(dst + at * D + 8 * li) = code;
+                if ((li & 7) == 0) {
+                    char* sdst = value ? x.c.vs + page * x.c.vs_page : x.c.ks + page * x.c.ks_page;
+                    *reinterpret_cast<uint16_t*>(sdst + (at * (D / 64) + (li >> 3)) * 2) = scale;
+                }
+            }
+        }
+        raw = next;
+    }
+}
+
+template <int D, bool APPEND>
+void launch(const NormRopeArgs& x, hipStream_t stream) {
+    const int heads = x.a.Hq + x.a.Hkv * (APPEND ? 2 : 1);
+    const int passes = (heads * (D / 8) + 255) / 256;
+    // one token's heads over several workgroups where the tokens alone leave CUs idle
+    const int shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(passes, 1024 / x.a.tokens)));
+    hipLaunchKernelGGL((norm_rope_kernel<D, APPEND>), dim3(static_cast<uint32_t>(x.a.tokens), shares), dim3(256), 0, stream, x);
+    check_launch("norm_rope_kernel");
+}
+
+} // namespace
+
+void launch_norm_rope(const NormRope& a, const PagedRef* cache, hipStream_t stream) {
+    NormRopeArgs x{};
+    x.a = a;
+    if (cache != nullptr) {
+        x.c = *cache;
+        a.D == 128 ? launch<128, true>(x, stream) : launch<256, true>(x, stream);
+    } else {
+        a.D == 128 ? launch<128, false>(x, stream) : launch<256, false>(x, stream);
+    }
+}
+
+} // namespace nmi

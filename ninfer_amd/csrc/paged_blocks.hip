@@ -1,0 +1,422 @@
+// Blocks of keys of a paged KV cache on gfx950: a mean for each, and the blocks that a token's queries score highest.
+//
+// Mathematics: a block's rows are summed in 64 bits (sums of stored values, exact unless they span more than 2^53), step = max
+// |sum| / 127, code = rne(sum * (1 / step)), scale = FP32(step / rows): code * scale is the mean with 8 bits. A token's query for a
+// KV head is the sum of its group's heads, made codes the same way; a block's score is scale * <codes, codes>, the product of
+// whole numbers exact on the matrix cores (up to 2^22), so it does not depend on any order, and which blocks are
+// selected is defined to the bit. A token always takes the first blocks and the last ones up to its own; of those
+// between it takes the `top` highest scores, the lower index of equals. A block with an infinite or NaN key has an infinite scale
+// and comes first.
+#include "common.h"
+#include "device_utils.h"
+#include "paged_internal.h"
+
+#include <algorithm>
+
+namespace nmi {
+namespace {
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+// Lanes of a wave exchange data through LDS: everything written before is there for the others.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Sequence b's tokens [start, start + tokens), the first at position history; no tokens where the scalars are out of range.
+struct Span {
+    int32_t start;
+    int32_t tokens;
+    int32_t history;
+};
+
+__device__ __forceinline__ Span span_of(const int32_t* starts, const int32_t* history, int b, int64_t total) {
+    Span s{starts[b], 0, history[b]};
+    const int32_t end = starts[b + 1];
+    if (s.start >= 0 && end >= s.start && end <= total && s.history >= 0) { s.tokens = end - s.start; }
+    return s;
+}
+
+// Units of work dealt out by sequence, `units(span)` for each: the sequence that holds unit u and u's place in it (b -1: past the
+// last). For the whole wave, 64 sequences at a time.
+struct Found {
+    int b;
+    int at;
+    Span s;
+};
+
+template <typename F>
+__device__ __forceinline__ Found find_unit(const int32_t* starts, const int32_t* history, int B, int64_t total, int u, int lane, F units) {
+    int sum = 0;
+    for (int base = 0; base < B; base += 64) {
+        Span s{0, 0, 0};
+        int n = 0;
+        if (base + lane < B) {
+            s = span_of(starts, history, base + lane, total);
+            n = units(s);
+        }
+        const int end = sum + wave_inclusive_scan(n);
+        const uint64_t past = __ballot(end > u);
+        if (past != 0u) {
+            const int l = __ffsll(static_cast<long long>(past)) - 1;
+            return Found{base + l, u - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(n, l)),
+                         Span{__builtin_amdgcn_readlane(s.start, l), __builtin_amdgcn_readlane(s.tokens, l), __builtin_amdgcn_readlane(s.history, l)}};
+        }
+        sum = __builtin_amdgcn_readlane(end, 63);
+    }
+    return Found{-1, 0, Span{0, 0, 0}};
+}
+
+// max |x| over the D / 8 lanes of a head in every one of them, infinite where a value is infinite or NaN.
+template <int D>
+__device__ __forceinline__ double head_amax(const double (&x)[8]) {
+    double m = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { m = fabs(x[e]) < INFINITY ? fmax(m, fabs(x[e])) : static_cast<double>(INFINITY); }
+#pragma unroll
+    for (int d = 1; d < D / 8; d *= 2) { m = fmax(m, __shfl_xor(m, d)); }
+    return m;
+}
+
+// Eight codes of x at 1 / step, none where there is nothing to tell (amax zero or infinite).
+__device__ __forceinline__ i2 codes_of(const double (&x)[8], double amax, double step) {
+    uint32_t code[2] = {0u, 0u};
+    if (amax > 0.0 && amax < INFINITY) {
+        const double inv = 1.0 / step;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const double r = fmin(127.0, fmax(-127.0, rint(x[e] * inv)));
+            code[e >> 2] |= (static_cast<uint32_t>(static_cast<int32_t>(r)) & 0xffu) << (8 * (e & 3));
+        }
+    }
+    return i2{static_cast<int>(code[0]), static_cast<int>(code[1])};
+}
+
+// ---- means ---------------------------------------------------------------------------------------
+//
+// A wave per touched block and head: D / 8 lanes a row, eight values a lane, so 512 values (four or two rows) at a time.
+// What bounds it: the reads of the block's rows (HBM), launch for decode steps.
+
+struct UpdateArgs {
+    int64_t tokens;
+    const int32_t* starts;
+    const int32_t* history;
+    PagedRef c;
+    BlocksRef b;
+    int64_t units; // waves
+};
+
+template <int D, bool BF>
+__global__ __launch_bounds__(256) void block_update_kernel(UpdateArgs x) {
+    constexpr int L = D / 8;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+    if (unit >= x.units) { return; }
+    const int h = static_cast<int>(unit % x.c.Hkv);
+    const int bs = x.b.shift;
+    // the blocks that hold new rows
+    const Found f = find_unit(x.starts, x.history, x.c.B, x.tokens, static_cast<int>(unit / x.c.Hkv), lane, [&](const Span& s) {
+        return s.tokens > 0 ? static_cast<int>(((static_cast<int64_t>(s.history) + s.tokens - 1) >> bs) - (s.history >> bs)) + 1 : 0;
+    });
+    if (f.b < 0) { return; }
+    const int64_t row0 = static_cast<int64_t>((f.s.history >> bs) + f.at) << bs;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(1) << bs, f.s.history + static_cast<int64_t>(f.s.tokens) - row0));
+    if ((row0 >> x.c.page_shift) >= x.c.max_pages) { return; }
+    const int32_t page = x.c.table[f.b * x.c.table_row + (row0 >> x.c.page_shift)];
+    if (page < 0 || page >= x.c.pages) { return; }
+    const int in_page = static_cast<int>(row0 & ((int64_t{1} << x.c.page_shift) - 1));
+    const int64_t first = (static_cast<int64_t>(h) << x.c.page_shift) + in_page;
+    const int li = lane & (L - 1), group = lane / L;
+    constexpr int GROUPS = 64 / L;
+    const char* k = x.c.k + page * x.c.k_page + first * (BF ? 2 * D : D) + li * (BF ? 16 : 8);
+    const char* ks = x.c.ks + page * x.c.ks_page + first * (D / 32) + (li >> 3) * 2;
+    double sum[8] = {};
+#pragma unroll 8
+    for (int r = group; r < rows; r += GROUPS) {
+        if constexpr (BF) {
+            const i4 raw = *reinterpret_cast<const i4*>(k + r * (2 * D));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t w = static_cast<uint32_t>(raw[e >> 1]);
+                sum[e] += __uint_as_float((e & 1) ? w & 0xffff0000u : w << 16);
+            }
+        } else {
+            const i2 raw = *reinterpret_cast<const i2*>(k + r * D);
+            const float s = f16_bits_to_f32(*reinterpret_cast<const uint16_t*>(ks + r * (D / 32)));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                sum[e] += static_cast<float>(static_cast<int8_t>(static_cast<uint32_t>(raw[e >> 2]) >> (8 * (e & 3)))) * s;
+            }
+        }
+    }
+#pragma unroll
+    for (int d = L; d < 64; d *= 2) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { sum[e] += __shfl_xor(sum[e], d); }
+    }
+    const double amax = head_amax<D>(sum);
+    const double step = amax / 127.0;
+    const i2 code = codes_of(sum, amax, step);
+    const int64_t slot = (static_cast<int64_t>(h) << (x.c.page_shift - bs)) + (in_page >> bs);
+    if (group == 0) { *reinterpret_cast<i2*>(x.b.codes + page * x.b.code_page + slot * D + 8 * li) = code; }
+    if (lane == 0) { *reinterpret_cast<float*>(x.b.scales + page * x.b.scale_page + slot * 4) = static_cast<float>(step / rows); }
+}
+
+// ---- selection -----------------------------------------------------------------------------------
+//
+// A workgroup per (tile of up to 16 tokens of a sequence, KV head): the tile's query codes, then 16 blocks at a time as
+// 16x16x64 products of whole numbers (rows: tokens, columns: blocks), the scores to LDS as ordered keys; then a wave
+// per token finds the `top`-th largest key by the digits of the keys less their smallest (8 bits a step) and writes the
+// list in order.
+// What bounds it: the means' reads and the walk over the keys in LDS.
+
+struct SelectArgs {
+    BlockSelect a;
+    PagedRef c;
+    BlocksRef b;
+    int32_t G;
+    int32_t tile_shift; // log2(tokens of a tile)
+    int32_t cap;        // keys of a token in LDS
+};
+
+// FP32 as an unsigned number of the same order; zero is left for blocks that are not to choose.
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f); // -0 as +0
+    return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+}
+
+// The keys of one token, `count` of them: those above `than` are chosen, and the first `equal` of those that equal it.
+struct Threshold {
+    uint32_t than;
+    int equal;
+};
+
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_inclusive_scan(v), 63); }
+
+__device__ __forceinline__ Threshold top_keys(const uint32_t* keys, int count, int want, int lane, uint32_t* hist) {
+    uint32_t lo = 0xffffffffu, hi = 0u;
+    int there = 0;
+    for (int i = lane; i < count; i += 64) {
+        const uint32_t k = keys[i];
+        there += k != 0u ? 1 : 0;
+        hi = max(hi, k);
+        lo = min(lo, k - 1u); // zero becomes the largest
+    }
+    there = wave_total(there);
+    if (there <= want) { return Threshold{0u, 0}; }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        hi = max(hi, static_cast<uint32_t>(__shfl_xor(static_cast<int>(hi), d)));
+        lo = min(lo, static_cast<uint32_t>(__shfl_xor(static_cast<int>(lo), d)));
+    }
+    uint32_t base = lo + 1u;       // keys [base, base + span] are undecided, those above are chosen
+    uint32_t span = hi - base;
+    int need = want;
+    while (true) {
+        const int bits = 32 - __clz(static_cast<int>(span));
+        const int shift = max(0, bits - 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { hist[lane + 64 * i] = 0u; }
+        wave_sync();
+        for (int i = lane; i < count; i += 64) {
+            const uint32_t k = keys[i];
+            if (k >= base && k - base <= span) { atomicAdd(&hist[(k - base) >> shift], 1u); }
+        }
+        wave_sync();
+        // lane l: bins 255 - 4 l down to 252 - 4 l
+        int n[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            n[i] = static_cast<int>(hist[255 - 4 * lane - i]);
+            sum += n[i];
+        }
+        const int end = wave_inclusive_scan(sum);
+        const int at = __ffsll(static_cast<long long>(__ballot(end >= need))) - 1;
+        int before = __builtin_amdgcn_readlane(end - sum, at);
+        int bin = 255 - 4 * at, held = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            held = __builtin_amdgcn_readlane(n[i], at);
+            if (before + held >= need) { break; }
+            before += held;
+            --bin;
+        }
+        wave_sync();
+        need -= before; // of this bin
+        base += static_cast<uint32_t>(bin) << shift;
+        if (held == need) { return Threshold{base - 1u, 0}; } // the whole bin; nothing else lies at base - 1 (it would not be chosen)
+        if (shift == 0) { return Threshold{base, need}; }
+        span = (1u << shift) - 1u;
+    }
+}
+
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
+    constexpr int L = D / 8;
+    constexpr int PAD = 16;
+    extern __shared__ uint32_t keys[]; // [tile token][cap]
+    __shared__ __attribute__((aligned(16))) char qcode[16 * (D + PAD)];
+    __shared__ uint32_t hist[NW][256];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = blockIdx.x % x.c.Hkv;
+    const int bs = x.b.shift;
+    const int tt = 1 << x.tile_shift;
+    const Found f = find_unit(x.a.starts, x.a.history, x.c.B, x.a.tokens, blockIdx.x / x.c.Hkv, lane, [&](const Span& s) {
+        // a sequence outside the envelope takes no part
+        return s.tokens <= x.a.max_new && static_cast<int64_t>(s.history) + s.tokens <= x.a.max_keys ? (s.tokens + tt - 1) >> x.tile_shift : 0;
+    });
+    if (f.b < 0) { return; }
+    const int t0 = f.at << x.tile_shift;
+    const int tokens = min(tt, f.s.tokens - t0);
+    const int pos0 = f.s.history + t0;
+    const int first = x.a.first, local = x.a.local;
+    // candidates of the tile's last token: blocks first .. last
+    const int last = ((pos0 + tokens - 1) >> bs) - local;
+
+    // ---- query codes
+    for (int i = threadIdx.x; i < 16 * (D + PAD) / 16; i += 64 * NW) { reinterpret_cast<u4*>(qcode)[i] = u4{0u, 0u, 0u, 0u}; }
+    __syncthreads();
+    for (int i = threadIdx.x; i < tokens * L; i += 64 * NW) {
+        const int t = i / L, li = i & (L - 1);
+        const char* src = x.a.q.data + static_cast<int64_t>(f.s.start + t0 + t) * x.a.q.token_stride + (h * x.G * D + 8 * li) * 2;
+        double sum[8] = {};
+        for (int g = 0; g < x.G; ++g) {
+            const i4 raw = *reinterpret_cast<const i4*>(src + g * (D * 2));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t w = static_cast<uint32_t>(raw[e >> 1]);
+                sum[e] += __uint_as_float((e & 1) ? w & 0xffff0000u : w << 16);
+            }
+        }
+        const double amax = head_amax<D>(sum);
+        *reinterpret_cast<i2*>(qcode + t * (D + PAD) + 8 * li) = codes_of(sum, amax, amax / 127.0);
+    }
+    __syncthreads();
+
+    // ---- scores
+    const int c = lane & 15, g = lane >> 4;
+    const int per = x.c.page_shift - bs; // log2(blocks of a page)
+    const int32_t* table = x.c.table + f.b * x.c.table_row;
+    i4 q[D / 64];
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) { q[i] = *reinterpret_cast<const i4*>(qcode + c * (D + PAD) + 64 * i + 16 * g); }
+    const int from = first & ~15;
+#pragma unroll 4
+    for (int b0 = from + 16 * wave; b0 <= last; b0 += 16 * NW) {
+        const int blk = b0 + c;
+        int32_t page = -1;
+        if (blk >= first && blk <= last && (blk >> per) < x.c.max_pages) { page = table[blk >> per]; }
+        const bool there = page >= 0 && page < x.c.pages;
+        const int64_t slot = (static_cast<int64_t>(h) << per) + (blk & ((1 << per) - 1));
+        i4 k[D / 64];
+        float scale = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) { k[i] = i4{0, 0, 0, 0}; }
+        if (there) {
+            const char* src = x.b.codes + page * x.b.code_page + slot * D + 16 * g;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) { k[i] = *reinterpret_cast<const i4*>(src + 64 * i); }
+            scale = *reinterpret_cast<const float*>(x.b.scales + page * x.b.scale_page + slot * 4);
+        }
+        i4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) { acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[i], k[i], acc, 0, 0, 0); }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) { // token 4 g + r, block c
+            const int t = 4 * g + r;
+            if (t < tt) {
+                const bool open = there && blk <= ((pos0 + t) >> bs) - local;
+                const float score = scale == INFINITY ? INFINITY : scale * static_cast<float>(acc[r]);
+                keys[t * x.cap + blk - from] = open ? ordered(score) : 0u;
+            }
+        }
+    }
+    __syncthreads();
+
+    // ---- lists
+    const int S = first + local + x.a.top;
+    for (int t = wave; t < tokens; t += NW) {
+        const int own = (pos0 + t) >> bs;
+        const int64_t token = f.s.start + t0 + t;
+        int32_t* out = x.a.selected + (token * x.c.Hkv + h) * S;
+        const int heads = min(first, own + 1);                 // the first blocks
+        const int tail = max(heads, own - local + 1);          // the last ones: tail .. own
+        const int count = max(0, own - local - first + 1);     // blocks between
+        const uint32_t* of = keys + t * x.cap + (first - from);
+        for (int i = lane; i < heads; i += 64) { out[i] = i; }
+        int taken = heads;
+        if (x.a.top > 0 && count > 0) {
+            const Threshold y = top_keys(of, count, x.a.top, lane, hist[wave]);
+            int equal = y.equal;
+            for (int i0 = 0; i0 < count; i0 += 64) {
+                const uint32_t k = i0 + lane < count ? of[i0 + lane] : 0u;
+                const uint64_t same = __ballot(k == y.than && k != 0u);
+                const bool take = k > y.than || (k == y.than && k != 0u && __popcll(same & ((uint64_t{1} << lane) - 1)) < equal);
+                const uint64_t all = __ballot(take);
+                if (take) { out[taken + __popcll(all & ((uint64_t{1} << lane) - 1))] = first + i0 + lane; }
+                taken += __popcll(all);
+                equal = max(0, equal - static_cast<int>(__popcll(same)));
+            }
+        }
+        for (int i = tail + lane; i <= own; i += 64) { out[taken + i - tail] = i; }
+        taken += own - tail + 1;
+        for (int i = taken + lane; i < S; i += 64) { out[i] = -1; }
+    }
+}
+
+template <int D>
+void select(const SelectArgs& x, int64_t tiles, hipStream_t stream) {
+    const size_t lds = (static_cast<size_t>(x.cap) << x.tile_shift) * 4;
+    const int64_t grid = tiles * x.c.Hkv;
+    if (grid > 0x3FFFFF) { throw Unsupported("paged block selection: more than 2^22 workgroups are not built"); }
+    // many waves for the blocks of a single token, few for a tile of tokens
+    if (x.tile_shift == 0) {
+        hipLaunchKernelGGL((block_select_kernel<D, 16>), dim3(static_cast<uint32_t>(grid)), dim3(1024), lds, stream, x);
+    } else {
+        hipLaunchKernelGGL((block_select_kernel<D, 4>), dim3(static_cast<uint32_t>(grid)), dim3(256), lds, stream, x);
+    }
+    check_launch("block_select_kernel");
+}
+
+} // namespace
+
+void launch_block_update(int64_t tokens, const int32_t* starts, const int32_t* history, const PagedRef& c, const BlocksRef& b, hipStream_t stream) {
+    // a sequence's new rows touch at most tokens / rows + 2 blocks
+    const int64_t units = ((tokens >> b.shift) + 2 * static_cast<int64_t>(c.B)) * c.Hkv;
+    const UpdateArgs x{tokens, starts, history, c, b, units};
+    const int64_t grid = (units + 3) / 4;
+    if (grid > 0x7FFFFF) { throw Unsupported("paged block update: more than 2^23 workgroups are not built"); }
+    const dim3 blocks(static_cast<uint32_t>(grid));
+    if (c.D == 128 && c.bf16) {
+        hipLaunchKernelGGL((block_update_kernel<128, true>), blocks, dim3(256), 0, stream, x);
+    } else if (c.D == 128) {
+        hipLaunchKernelGGL((block_update_kernel<128, false>), blocks, dim3(256), 0, stream, x);
+    } else if (c.bf16) {
+        hipLaunchKernelGGL((block_update_kernel<256, true>), blocks, dim3(256), 0, stream, x);
+    } else {
+        hipLaunchKernelGGL((block_update_kernel<256, false>), blocks, dim3(256), 0, stream, x);
+    }
+    check_launch("block_update_kernel");
+}
+
+size_t block_select_bytes(int32_t, int32_t, int64_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+
+void launch_block_select(const BlockSelect& a, const PagedRef& c, const BlocksRef& b, void*, hipStream_t stream) {
+    SelectArgs x{};
+    x.a = a;
+    x.c = c;
+    x.b = b;
+    x.G = a.Hq / c.Hkv;
+    const int32_t blocks = ((a.max_keys + (1 << b.shift) - 1) >> b.shift);
+    x.cap = (blocks + 31) & ~15; // a tile's keys begin at a multiple of 16
+    // as many tokens of a tile as its keys leave room for in 128 KiB, no more than a sequence may have
+    x.tile_shift = 4;
+    while (x.tile_shift > 0 && ((static_cast<int64_t>(x.cap) << x.tile_shift) > 32768 || (1 << (x.tile_shift - 1)) >= a.max_new)) { --x.tile_shift; }
+    const int64_t tiles = std::min<int64_t>(a.tokens, (a.tokens >> x.tile_shift) + c.B);
+    c.D == 128 ? select<128>(x, tiles, stream) : select<256>(x, tiles, stream);
+}
+
+} // namespace nmi

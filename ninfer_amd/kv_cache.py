@@ -12,7 +12,7 @@ import ctypes as C
 import numpy as np
 
 from . import _capi
-from ._capi import KVLayerView, PagedKVLayerView, Tensor
+from ._capi import KVLayerView, PagedBlockView, PagedKVLayerView, Tensor
 from .device import DeviceArray
 
 QUANT_GROUP = 64
@@ -98,9 +98,12 @@ class KVCacheLayer:
 
 class PagedKVCacheLayer:
     """Owning pool of pages (INT8-G64 by default, or BF16), the table of `batch` sequences of up to `max_pages` pages
-    (-1: absent, as at first) and the matching nmi_paged_kv_layer_view."""
+    (-1: absent, as at first), the counts of the table's entries per page (`refs`) and the matching nmi_paged_kv_layer_view.
+    `block_size`: means of blocks of so many keys next to the pages (0: none). `table_of`: the layer whose table and counts this one
+    shares, as the layers of a model do."""
 
-    def __init__(self, pages: int, page_size: int, num_kv_heads: int, head_dim: int, batch: int, max_pages: int, dtype: int = _capi.I8):
+    def __init__(self, pages: int, page_size: int, num_kv_heads: int, head_dim: int, batch: int, max_pages: int, dtype: int = _capi.I8,
+                 block_size: int = 0, table_of: "PagedKVCacheLayer | None" = None):
         if page_size < 16 or page_size > 4096 or page_size & (page_size - 1):
             raise ValueError("PagedKVCache page_size must be a power of two in [16, 4096]")
         if pages <= 0 or batch <= 0 or max_pages <= 0:
@@ -109,6 +112,10 @@ class PagedKVCacheLayer:
             raise ValueError("PagedKVCache geometry invalid")
         if dtype not in (_capi.I8, _capi.BF16):
             raise ValueError("PagedKVCache dtype must be I8 or BF16")
+        if block_size and (block_size < 32 or block_size > page_size or block_size & (block_size - 1)):
+            raise ValueError("PagedKVCache block_size must be a power of two from 32 to page_size")
+        if table_of is not None and (table_of.pages, table_of.page_size, table_of.batch, table_of.max_pages) != (pages, page_size, batch, max_pages):
+            raise ValueError("PagedKVCache layers that share a table must have the same pages")
         self.pages, self.page_size, self.num_kv_heads, self.head_dim = pages, page_size, num_kv_heads, head_dim
         self.batch, self.max_pages, self.dtype = batch, max_pages, dtype
         self.k = DeviceArray(dtype, (head_dim, page_size, num_kv_heads, pages))
@@ -117,8 +124,17 @@ class PagedKVCacheLayer:
         if dtype == _capi.I8:
             self.k_scale = DeviceArray(_capi.FP16, (head_dim // QUANT_GROUP, page_size, num_kv_heads, pages))
             self.v_scale = DeviceArray(_capi.FP16, (head_dim // QUANT_GROUP, page_size, num_kv_heads, pages))
-        self.page_table = DeviceArray(_capi.I32, (max_pages, batch))
-        self.set_pages(np.full((batch, max_pages), -1, dtype=np.int32))
+        self.block_size = block_size
+        self.block_codes = self.block_scales = None
+        if block_size:
+            self.block_codes = DeviceArray(_capi.I8, (head_dim, page_size // block_size, num_kv_heads, pages))
+            self.block_scales = DeviceArray(_capi.FP32, (page_size // block_size, num_kv_heads, pages))
+        if table_of is not None:
+            self.page_table, self.refs = table_of.page_table, table_of.refs
+        else:
+            self.page_table = DeviceArray(_capi.I32, (max_pages, batch))
+            self.refs = DeviceArray(_capi.I32, (pages,))
+            self.set_pages(np.full((batch, max_pages), -1, dtype=np.int32))
 
     def _planes(self):
         return [a for a in (self.k, self.v, self.k_scale, self.v_scale) if a is not None]
@@ -128,8 +144,18 @@ class PagedKVCacheLayer:
             a.zero(stream)
 
     def set_pages(self, table) -> None:
-        """The whole page table, int32 [batch, max_pages]."""
-        self.page_table.upload(np.asarray(table, dtype=np.int32).reshape(self.batch, self.max_pages))
+        """The whole page table, int32 [batch, max_pages], and the counts that belong to it."""
+        table = np.asarray(table, dtype=np.int32).reshape(self.batch, self.max_pages)
+        self.page_table.upload(table)
+        held = table[(table >= 0) & (table < self.pages)]
+        self.refs.upload(np.bincount(held, minlength=self.pages).astype(np.int32))
+
+    def blocks(self) -> PagedBlockView:
+        v = PagedBlockView()
+        if self.block_codes is None:
+            raise ValueError("this cache keeps no block means")
+        v.codes, v.scales, v.block_size = self.block_codes.tensor(), self.block_scales.tensor(), self.block_size
+        return v
 
     def view(self) -> PagedKVLayerView:
         v = PagedKVLayerView()

@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _capi
-from ._capi import AttentionWindow, CommitEnvelope, GqaEnvelope, PagedEnvelope, Tensor, check, lib
+from ._capi import AttentionWindow, BlockSelection, CommitEnvelope, GqaEnvelope, NormRope, PagedEnvelope, Tensor, check, lib
 
 
 def _s(stream):
@@ -105,6 +105,84 @@ def paged_attention(q, starts, history, scale, window, cache, envelope, workspac
     ws, nb = _ws(workspace)
     check(lib().nmi_paged_attention(_p(q), _p(starts), _p(history), float(scale), AttentionWindow(*window), C.byref(cache),
                                     PagedEnvelope(*envelope), ws, nb, _p(out), _s(stream)))
+
+
+# ---- head norms and rotation (extension) --------------------------------------------------------
+
+def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, norm, q_out, k_out, stream=None) -> None:
+    """Every head normalised, times its weight, and rotated by positions * inv_freq in one pass. `norm`: (eps, weight_offset,
+    interleaved); a weight may be None (ones), inv_freq None (no rotation)."""
+    check(lib().nmi_qk_norm_rope(_p(q), _p(k), _p(q_weight), _p(k_weight), _p(positions), _p(inv_freq), NormRope(norm[0], norm[1], int(norm[2])),
+                                 _p(q_out), _p(k_out), _s(stream)))
+
+
+def paged_qk_norm_rope_append(q, k, v, q_weight, k_weight, starts, history, inv_freq, norm, cache, q_out, stream=None) -> None:
+    """qk_norm_rope at the tokens' positions and paged_kv_append of the keys and values, in one pass."""
+    check(lib().nmi_paged_qk_norm_rope_append(_p(q), _p(k), _p(v), _p(q_weight), _p(k_weight), _p(starts), _p(history), _p(inv_freq),
+                                              NormRope(norm[0], norm[1], int(norm[2])), C.byref(cache), _p(q_out), _s(stream)))
+
+
+# ---- sparse attention over blocks of a paged cache (extension) ------------------------------------
+#
+# `blocks` is a PagedBlockView (PagedKVCacheLayer(..., block_size=...).blocks()).
+
+def paged_block_update(cache, starts, history, tokens: int, blocks, stream=None) -> None:
+    """The means of the key blocks that hold the rows of the `tokens` packed tokens, which are in the cache already."""
+    check(lib().nmi_paged_block_update(C.byref(cache), _p(starts), _p(history), int(tokens), C.byref(blocks), _s(stream)))
+
+
+def paged_block_select_workspace_bytes(kv_heads: int, head_dim: int, tokens: int, batch: int, envelope, block_size: int) -> int:
+    return int(lib().nmi_paged_block_select_workspace_bytes(kv_heads, head_dim, tokens, batch, PagedEnvelope(*envelope), block_size))
+
+
+def paged_block_select(q, starts, history, page_table, page_size: int, blocks, selection, envelope, workspace, selected, stream=None) -> None:
+    """For every token and KV head the blocks of `selection` (first, local, top): ascending in `selected`, -1 behind them."""
+    ws, nb = _ws(workspace)
+    check(lib().nmi_paged_block_select(_p(q), _p(starts), _p(history), _p(page_table), int(page_size), C.byref(blocks), BlockSelection(*selection),
+                                       PagedEnvelope(*envelope), ws, nb, _p(selected), _s(stream)))
+
+
+def paged_sparse_attention_workspace_bytes(q_heads: int, kv_heads: int, head_dim: int, tokens: int, batch: int, selected_blocks: int,
+                                           block_size: int) -> int:
+    return int(lib().nmi_paged_sparse_attention_workspace_bytes(q_heads, kv_heads, head_dim, tokens, batch, selected_blocks, block_size))
+
+
+def paged_sparse_attention(q, starts, history, scale, selected, block_size: int, cache, envelope, workspace, out, stream=None) -> None:
+    """paged_attention over the rows of the blocks that each token's list holds for the KV head (I32 [S, Hkv, N], negative: none)."""
+    ws, nb = _ws(workspace)
+    check(lib().nmi_paged_sparse_attention(_p(q), _p(starts), _p(history), float(scale), _p(selected), int(block_size), C.byref(cache),
+                                           PagedEnvelope(*envelope), ws, nb, _p(out), _s(stream)))
+
+
+# ---- pages of a paged cache (extension) ------------------------------------------------------------
+#
+# `refs` counts the entries of the page table that hold each page (PagedKVCacheLayer.refs); a page without any is free.
+
+def paged_kv_copy_pages(cache, blocks, src, dst, stream=None) -> None:
+    """Page src[i] to page dst[i] (negative: none), with its block means where `blocks` is not None."""
+    check(lib().nmi_paged_kv_copy_pages(C.byref(cache), C.byref(blocks) if blocks is not None else None, _p(src), _p(dst), _s(stream)))
+
+
+def paged_pages_reserve(page_table, refs, starts, history, page_size: int, granted, stream=None) -> None:
+    """Free pages (the lowest first) for the new rows that have none; granted[b]: the new tokens of b that have theirs."""
+    check(lib().nmi_paged_pages_reserve(_p(page_table), _p(refs), _p(starts), _p(history), int(page_size), _p(granted), _s(stream)))
+
+
+def paged_pages_release(page_table, refs, sequences, keep_rows, page_size: int, stream=None) -> None:
+    """Sequence sequences[i] gives back the pages past its first keep_rows[i] rows."""
+    check(lib().nmi_paged_pages_release(_p(page_table), _p(refs), _p(sequences), _p(keep_rows), int(page_size), _s(stream)))
+
+
+def paged_pages_fork(page_table, refs, parents, children, history, page_size: int, src, dst, stream=None) -> None:
+    """Sequence children[i] as a copy of parents[i]: whole pages shared, the rest in a page of its own that paged_kv_copy_pages(src,
+    dst) fills."""
+    check(lib().nmi_paged_pages_fork(_p(page_table), _p(refs), _p(parents), _p(children), _p(history), int(page_size), _p(src), _p(dst),
+                                     _s(stream)))
+
+
+def paged_pages_compact(page_table, refs, src, dst, moved, stream=None) -> None:
+    """The highest pages in use to the lowest free ones: table and counts now, contents by paged_kv_copy_pages(src, dst)."""
+    check(lib().nmi_paged_pages_compact(_p(page_table), _p(refs), _p(src), _p(dst), _p(moved), _s(stream)))
 
 
 # ---- acceptance (argmax.h, sampling.h, speculative_round.h) ------------------------------------
