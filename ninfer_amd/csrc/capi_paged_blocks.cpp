@@ -105,7 +105,7 @@ size_t nmi_paged_sparse_attention_workspace_bytes(int32_t q_heads, int32_t kv_he
         block_size < 32 || block_size > 4096 || static_cast<int64_t>(tokens) * q_heads > (int64_t{1} << 30)) {
         return 0; // what the op itself refuses
     }
-    return sparse_attention_bytes(q_heads, kv_heads, head_dim, tokens, selected_blocks, log2_of(block_size));
+    return sparse_attention_bytes(q_heads, kv_heads, head_dim, tokens, batch, selected_blocks, log2_of(block_size));
 }
 
 int nmi_paged_sparse_attention(const nmi_tensor* q, const nmi_tensor* starts, const nmi_tensor* history, float scale, const nmi_tensor* selected,
@@ -135,7 +135,7 @@ int nmi_paged_sparse_attention(const nmi_tensor* q, const nmi_tensor* starts, co
         a.max_new = static_cast<int32_t>(envelope.max_new_tokens);
         a.max_keys = static_cast<int32_t>(envelope.max_visible_keys);
         const int32_t shift = log2_of(block_size);
-        validate_workspace(workspace, workspace_bytes, sparse_attention_bytes(a.Hq, c.Hkv, c.D, n, count, shift), op);
+        validate_workspace(workspace, workspace_bytes, sparse_attention_bytes(a.Hq, c.Hkv, c.D, n, c.B, count, shift), op);
         launch_sparse_attention(a, lists, count, shift, c, workspace, reinterpret_cast<hipStream_t>(stream));
     });
 }

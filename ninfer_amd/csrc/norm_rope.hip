@@ -59,25 +59,53 @@ __device__ __forceinline__ void load_weights(const void* w, bool f32, float offs
     }
 }
 
-// A workgroup per token (and share of its heads): D / 8 lanes a head, eight dims a lane.
+// Two FP32 values rounded to BF16, the first in the low half (v_cvt_pk_bf16_f32).
+__device__ __forceinline__ int bf16_pair(float lo, float hi) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(int, b2{static_cast<__bf16>(lo), static_cast<__bf16>(hi)});
+}
+
+// What a lane's eight dims of a head become: x own + y other, x its normalised values and y its partners' (its own ones, times
+// zero, where nothing is rotated).
+struct Turn {
+    float own[8];
+    float other[8];
+};
+
+// A workgroup per token (and share of its heads): D / 8 lanes a head, eight dims a lane, so a wave holds HEADS heads. Queries, keys
+// and values are dealt out in runs of HEADS, so that a wave's heads are of one kind and their weights (times sines and cosines, once
+// per token) come from registers without a choice per value.
 template <int D, bool APPEND>
 __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs x) {
-    constexpr int L = D / 8;       // lanes of a head
-    constexpr int HEADS = 256 / L; // heads of a pass
+    constexpr int L = D / 8;      // lanes of a head
+    constexpr int HEADS = 64 / L; // heads of a wave
     __shared__ float2 turn[D / 2];
     const NormRope& a = x.a;
     const int64_t n = blockIdx.x;
-    const int li = threadIdx.x & (L - 1);
-    const int step = HEADS * gridDim.y;
-    const int heads = a.Hq + a.Hkv + (APPEND ? a.Hkv : 0);
-    const auto load = [&](int head) {
-        const PackedRef& src = head < a.Hq ? a.q : head < a.Hq + a.Hkv ? a.k : a.v;
-        const int of = head < a.Hq ? head : head < a.Hq + a.Hkv ? head - a.Hq : head - a.Hq - a.Hkv;
-        return *reinterpret_cast<const i4*>(src.data + n * src.token_stride + (of * D + 8 * li) * 2);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & (L - 1);
+    const int q_runs = (a.Hq + HEADS - 1) / HEADS, kv_runs = (a.Hkv + HEADS - 1) / HEADS;
+    const int runs = q_runs + kv_runs * (APPEND ? 2 : 1);
+    const int step = 4 * gridDim.y;
+    // run i: its tensor, the lane's head there and whether there is one
+    struct Run {
+        int kind; // 0 queries, 1 keys, 2 values
+        int head;
+        bool live;
     };
-    int head = blockIdx.y * HEADS + threadIdx.x / L;
-    i4 raw = {0, 0, 0, 0};
-    if (head < heads) { raw = load(head); }
+    const auto run_of = [&](int i) {
+        const int kind = i < q_runs ? 0 : i < q_runs + kv_runs ? 1 : 2;
+        const int head = (i - (kind == 0 ? 0 : kind == 1 ? q_runs : q_runs + kv_runs)) * HEADS + lane / L;
+        return Run{kind, head, i < runs && head < (kind == 0 ? a.Hq : a.Hkv)};
+    };
+    const auto load = [&](const Run& r) {
+        const PackedRef& src = r.kind == 0 ? a.q : r.kind == 1 ? a.k : a.v;
+        return r.live ? *reinterpret_cast<const i4*>(src.data + n * src.token_stride + (r.head * D + 8 * li) * 2) : i4{0, 0, 0, 0};
+    };
+    int at = blockIdx.y * 4 + wave;
+    Run run = run_of(at);
+    i4 raw = load(run);
 
     int64_t pos;
     int32_t page = -1, row = 0;
@@ -105,98 +133,122 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs x) {
         sincospif(static_cast<float>(2.0 * t), &s, &c);
         turn[i] = float2{c, s};
     }
-    // the lane's dims, its partner's lane, and the weights of both
+    // the lane's dims and its partner's
     const int lanes = a.half / 8; // lanes of half a rotated part
     const bool rotated = 8 * li < 2 * a.half;
     const bool upper = !a.interleaved && li >= lanes; // b of its pairs
     const int partner = !rotated || a.interleaved ? li : upper ? li - lanes : li + lanes;
-    float qw[8], kw[8], qp[8], kp[8];
-    load_weights(a.q_weight, a.q_weight_f32, a.offset, 8 * li, qw);
-    load_weights(a.k_weight, a.k_weight_f32, a.offset, 8 * li, kw);
-    load_weights(a.q_weight, a.q_weight_f32, a.offset, 8 * partner, qp);
-    load_weights(a.k_weight, a.k_weight_f32, a.offset, 8 * partner, kp);
+    const int from = 4 * ((lane & ~(L - 1)) + partner);
+    Turn q, k;
+    load_weights(a.q_weight, a.q_weight_f32, a.offset, 8 * li, q.own);
+    load_weights(a.k_weight, a.k_weight_f32, a.offset, 8 * li, k.own);
+    load_weights(a.q_weight, a.q_weight_f32, a.offset, 8 * partner, q.other);
+    load_weights(a.k_weight, a.k_weight_f32, a.offset, 8 * partner, k.other);
     __syncthreads();
-    float cs[8], sn[8];
+    if (a.interleaved) { // a dim's partner stands next to it
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        cs[e] = 1.0f;
-        sn[e] = 0.0f;
-        if (rotated) {
-            const float2 z = turn[a.interleaved ? 4 * li + (e >> 1) : 8 * (upper ? li - lanes : li) + e];
-            cs[e] = z.x;
-            sn[e] = a.interleaved ? ((e & 1) ? z.y : -z.y) : upper ? z.y : -z.y;
+        for (int e = 0; e < 8; e += 2) {
+            q.other[e] = q.own[e + 1];
+            q.other[e + 1] = q.own[e];
+            k.other[e] = k.own[e + 1];
+            k.other[e + 1] = k.own[e];
         }
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float c = 1.0f, s = 0.0f;
+        if (rotated) {
+            const float2 z = turn[a.interleaved ? 4 * li + (e >> 1) : 8 * (upper ? li - lanes : li) + e];
+            c = z.x;
+            s = (a.interleaved ? (e & 1) != 0 : upper) ? z.y : -z.y;
+        }
+        q.own[e] *= c;
+        k.own[e] *= c;
+        q.other[e] *= s;
+        k.other[e] *= s;
+    }
 
-    for (; head < heads; head += step) {
-        i4 next = {0, 0, 0, 0};
-        if (head + step < heads) { next = load(head + step); }
-        const bool key = head >= a.Hq;
+    while (at < runs) {
+        at += step;
+        const Run after = run_of(at);
+        const i4 next = load(after);
         i4 out = raw;
-        if (!APPEND || head < a.Hq + a.Hkv) {
+        if (run.kind < 2) {
+            float v[8];
             float ss = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { ss = fmaf(bf16_of(raw, e), bf16_of(raw, e), ss); }
+            for (int e = 0; e < 8; ++e) {
+                v[e] = bf16_of(raw, e);
+                ss = fmaf(v[e], v[e], ss);
+            }
             ss = head_sum<D>(ss);
-            float r = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
+            float r = __builtin_amdgcn_rsqf(fmaf(ss, 1.0f / D, a.eps));
             if (__builtin_expect(__any(ss > 0x1p120f), 0)) { // beyond FP32's squares: 2^-70 of the values, eps is nothing next to them
                 float s2 = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float z = bf16_of(raw, e) * 0x1p-70f;
-                    s2 = fmaf(z, z, s2);
-                }
+                for (int e = 0; e < 8; ++e) { s2 = fmaf(v[e] * 0x1p-70f, v[e] * 0x1p-70f, s2); }
                 s2 = head_sum<D>(s2);
-                if (ss > 0x1p120f) { r = 0x1p-70f / sqrtf(s2 * (1.0f / D)); }
+                if (ss > 0x1p120f) { r = 0x1p-70f * __builtin_amdgcn_rsqf(s2 * (1.0f / D)); }
             }
-            i4 other = raw;
-            if (!a.interleaved) {
-                const int from = 4 * ((threadIdx.x & 63 & ~(L - 1)) + partner);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { v[e] *= r; }
+            float z[8];
+            if (a.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { z[e] = v[e ^ 1]; }
+            } else {
+                i4 other;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) { other[w] = __builtin_amdgcn_ds_bpermute(from, raw[w]); }
-            }
-            uint32_t bits[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float y = bf16_of(raw, e) * r * (key ? kw[e] : qw[e]);
-                const int pe = a.interleaved ? e ^ 1 : e;
-                const float w = a.interleaved ? (key ? kw[e ^ 1] : qw[e ^ 1]) : (key ? kp[e] : qp[e]);
-                const float z = (a.interleaved ? bf16_of(raw, e ^ 1) : bf16_of(other, pe)) * r * w;
-                bits[e] = f32_to_bf16_bits(rotated ? y * cs[e] + z * sn[e] : y);
+                for (int e = 0; e < 8; ++e) { z[e] = bf16_of(other, e) * r; }
             }
+            const auto apply = [&](const Turn& t) {
+                float y[8];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) { out[w] = static_cast<int>(bits[2 * w] | (bits[2 * w + 1] << 16)); }
+                for (int e = 0; e < 8; ++e) { y[e] = fmaf(v[e], t.own[e], z[e] * t.other[e]); }
+#pragma unroll
+                for (int w = 0; w < 4; ++w) { out[w] = bf16_pair(y[2 * w], y[2 * w + 1]); }
+            };
+            if (run.kind == 0) {
+                apply(q);
+            } else {
+                apply(k);
+            }
         }
-        if (head < a.Hq) {
-            *reinterpret_cast<i4*>(a.q_out.data + n * a.q_out.token_stride + (head * D + 8 * li) * 2) = out;
+        if (run.kind == 0) {
+            if (run.live) { *reinterpret_cast<i4*>(a.q_out.data + n * a.q_out.token_stride + (run.head * D + 8 * li) * 2) = out; }
         } else if constexpr (!APPEND) {
-            *reinterpret_cast<i4*>(a.k_out.data + n * a.k_out.token_stride + ((head - a.Hq) * D + 8 * li) * 2) = out;
+            if (run.live) { *reinterpret_cast<i4*>(a.k_out.data + n * a.k_out.token_stride + (run.head * D + 8 * li) * 2) = out; }
         } else if (page >= 0) {
-            const bool value = head >= a.Hq + a.Hkv;
-            const int64_t at = (static_cast<int64_t>(head - a.Hq - (value ? a.Hkv : 0)) << x.c.page_shift) + row;
+            const bool value = run.kind == 2;
+            const int64_t to = (static_cast<int64_t>(run.head) << x.c.page_shift) + row;
             char* dst = value ? x.c.v + page * x.c.v_page : x.c.k + page * x.c.k_page;
             if (x.c.bf16) {
-                *reinterpret_cast<i4*>(dst + (at * D + 8 * li) * 2) = out;
+                if (run.live) { *reinterpret_cast<i4*>(dst + (to * D + 8 * li) * 2) = out; }
             } else {
                 uint16_t scale;
                 const i2 code = quantize_g64(out, scale);
-                *reinterpret_cast<i2*>(dst + at * D + 8 * li) = code;
-                if ((li & 7) == 0) {
-                    char* sdst = value ? x.c.vs + page * x.c.vs_page : x.c.ks + page * x.c.ks_page;
-                    *reinterpret_cast<uint16_t*>(sdst + (at * (D / 64) + (li >> 3)) * 2) = scale;
+                if (run.live) {
+                    *reinterpret_cast<i2*>(dst + to * D + 8 * li) = code;
+                    if ((li & 7) == 0) {
+                        char* sdst = value ? x.c.vs + page * x.c.vs_page : x.c.ks + page * x.c.ks_page;
+                        *reinterpret_cast<uint16_t*>(sdst + (to * (D / 64) + (li >> 3)) * 2) = scale;
+                    }
                 }
             }
         }
+        run = after;
         raw = next;
     }
 }
 
 template <int D, bool APPEND>
 void launch(const NormRopeArgs& x, hipStream_t stream) {
-    const int heads = x.a.Hq + x.a.Hkv * (APPEND ? 2 : 1);
-    const int passes = (heads * (D / 8) + 255) / 256;
+    constexpr int HEADS = 512 / D;
+    const int runs = (x.a.Hq + HEADS - 1) / HEADS + (x.a.Hkv + HEADS - 1) / HEADS * (APPEND ? 2 : 1);
     // one token's heads over several workgroups where the tokens alone leave CUs idle
-    const int shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(passes, 1024 / x.a.tokens)));
+    const int shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((runs + 3) / 4, 1024 / x.a.tokens)));
     hipLaunchKernelGGL((norm_rope_kernel<D, APPEND>), dim3(static_cast<uint32_t>(x.a.tokens), shares), dim3(256), 0, stream, x);
     check_launch("norm_rope_kernel");
 }

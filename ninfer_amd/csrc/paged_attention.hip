@@ -227,7 +227,8 @@ __device__ __forceinline__ void few_part(const PagedAttnArgs& x, int h, const Fe
         if (splits > 1) {
             store_part<D, BF, NT>(x, r, nt, M[nt], L[nt], (static_cast<int64_t>(share + q.rank) * x.c.Hkv + h) * (16 * NT) + row, g);
         } else {
-            store_out<D, BF, NT>(x, s, h, row, r, nt, L[nt], g);
+            const int t = row / x.G;
+            store_out<D, BF, NT>(x, s.start + t, h, row - t * x.G, r, nt, L[nt], g);
         }
     }
 }

@@ -10,6 +10,7 @@
 #include "common.h"
 #include "device_utils.h"
 #include "paged_internal.h"
+#include "paged_place.h"
 
 #include <algorithm>
 
@@ -17,56 +18,6 @@ namespace nmi {
 namespace {
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-
-// Lanes of a wave exchange data through LDS: everything written before is there for the others.
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
-// Sequence b's tokens [start, start + tokens), the first at position history; no tokens where the scalars are out of range.
-struct Span {
-    int32_t start;
-    int32_t tokens;
-    int32_t history;
-};
-
-__device__ __forceinline__ Span span_of(const int32_t* starts, const int32_t* history, int b, int64_t total) {
-    Span s{starts[b], 0, history[b]};
-    const int32_t end = starts[b + 1];
-    if (s.start >= 0 && end >= s.start && end <= total && s.history >= 0) { s.tokens = end - s.start; }
-    return s;
-}
-
-// Units of work dealt out by sequence, `units(span)` for each: the sequence that holds unit u and u's place in it (b -1: past the
-// last). For the whole wave, 64 sequences at a time.
-struct Found {
-    int b;
-    int at;
-    Span s;
-};
-
-template <typename F>
-__device__ __forceinline__ Found find_unit(const int32_t* starts, const int32_t* history, int B, int64_t total, int u, int lane, F units) {
-    int sum = 0;
-    for (int base = 0; base < B; base += 64) {
-        Span s{0, 0, 0};
-        int n = 0;
-        if (base + lane < B) {
-            s = span_of(starts, history, base + lane, total);
-            n = units(s);
-        }
-        const int end = sum + wave_inclusive_scan(n);
-        const uint64_t past = __ballot(end > u);
-        if (past != 0u) {
-            const int l = __ffsll(static_cast<long long>(past)) - 1;
-            return Found{base + l, u - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(n, l)),
-                         Span{__builtin_amdgcn_readlane(s.start, l), __builtin_amdgcn_readlane(s.tokens, l), __builtin_amdgcn_readlane(s.history, l)}};
-        }
-        sum = __builtin_amdgcn_readlane(end, 63);
-    }
-    return Found{-1, 0, Span{0, 0, 0}};
-}
 
 // max |x| over the D / 8 lanes of a head in every one of them, infinite where a value is infinite or NaN.
 template <int D>
@@ -117,7 +68,7 @@ __global__ __launch_bounds__(256) void block_update_kernel(UpdateArgs x) {
     const int h = static_cast<int>(unit % x.c.Hkv);
     const int bs = x.b.shift;
     // the blocks that hold new rows
-    const Found f = find_unit(x.starts, x.history, x.c.B, x.tokens, static_cast<int>(unit / x.c.Hkv), lane, [&](const Span& s) {
+    const Found f = find_unit(x.c.B, static_cast<int>(unit / x.c.Hkv), lane, [&](int b) { return span_of(x.starts, x.history, b, x.tokens); }, [&](const Span& s) {
         return s.tokens > 0 ? static_cast<int>(((static_cast<int64_t>(s.history) + s.tokens - 1) >> bs) - (s.history >> bs)) + 1 : 0;
     });
     if (f.b < 0) { return; }
@@ -167,10 +118,9 @@ __global__ __launch_bounds__(256) void block_update_kernel(UpdateArgs x) {
 // ---- selection -----------------------------------------------------------------------------------
 //
 // A workgroup per (tile of up to 16 tokens of a sequence, KV head): the tile's query codes, then 16 blocks at a time as
-// 16x16x64 products of whole numbers (rows: tokens, columns: blocks), the scores to LDS as ordered keys; then a wave
-// per token finds the `top`-th largest key by the digits of the keys less their smallest (8 bits a step) and writes the
-// list in order.
-// What bounds it: the means' reads and the walk over the keys in LDS.
+// 16x16x64 products of whole numbers (rows: tokens, columns: blocks), the scores to LDS as ordered keys; then the keys of a
+// token, in registers, are counted against a middle that closes in on the `top`-th largest, and the list is written in order.
+// What bounds it: the means' reads, and for prompts the choice (a dozen counts of a token's keys).
 
 struct SelectArgs {
     BlockSelect a;
@@ -187,84 +137,153 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
 
-// The keys of one token, `count` of them: those above `than` are chosen, and the first `equal` of those that equal it.
+// Which of a token's keys are chosen: those above `than`, and the first `equal` of those that equal it.
 struct Threshold {
     uint32_t than;
     int equal;
 };
 
-__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_inclusive_scan(v), 63); }
-
-__device__ __forceinline__ Threshold top_keys(const uint32_t* keys, int count, int want, int lane, uint32_t* hist) {
-    uint32_t lo = 0xffffffffu, hi = 0u;
-    int there = 0;
-    for (int i = lane; i < count; i += 64) {
-        const uint32_t k = keys[i];
-        there += k != 0u ? 1 : 0;
-        hi = max(hi, k);
-        lo = min(lo, k - 1u); // zero becomes the largest
-    }
-    there = wave_total(there);
-    if (there <= want) { return Threshold{0u, 0}; }
+// The `want` largest of the keys that WAVES waves hold, R a lane (zeros are none): the interval of the smallest chosen one is halved
+// until as many keys as are wanted lie at its middle or above, or one value is left. About a dozen steps for scores that
+// differ. `total` sums a count over the waves.
+template <int R, typename F>
+__device__ __forceinline__ Threshold top_keys(const uint32_t (&k)[R], int want, uint32_t lo, uint32_t hi, F total) {
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2 + 1;
+        int n = 0;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        hi = max(hi, static_cast<uint32_t>(__shfl_xor(static_cast<int>(hi), d)));
-        lo = min(lo, static_cast<uint32_t>(__shfl_xor(static_cast<int>(lo), d)));
-    }
-    uint32_t base = lo + 1u;       // keys [base, base + span] are undecided, those above are chosen
-    uint32_t span = hi - base;
-    int need = want;
-    while (true) {
-        const int bits = 32 - __clz(static_cast<int>(span));
-        const int shift = max(0, bits - 8);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { hist[lane + 64 * i] = 0u; }
-        wave_sync();
-        for (int i = lane; i < count; i += 64) {
-            const uint32_t k = keys[i];
-            if (k >= base && k - base <= span) { atomicAdd(&hist[(k - base) >> shift], 1u); }
+        for (int i = 0; i < R; ++i) { n += static_cast<int>(__popcll(__ballot(k[i] >= mid))); }
+        n = total(n);
+        if (n == want) { return Threshold{mid - 1u, 0}; } // (a key of mid - 1 is not chosen: none is counted)
+        if (n > want) {
+            lo = mid;
+        } else {
+            hi = mid - 1u;
         }
-        wave_sync();
-        // lane l: bins 255 - 4 l down to 252 - 4 l
-        int n[4], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            n[i] = static_cast<int>(hist[255 - 4 * lane - i]);
-            sum += n[i];
-        }
-        const int end = wave_inclusive_scan(sum);
-        const int at = __ffsll(static_cast<long long>(__ballot(end >= need))) - 1;
-        int before = __builtin_amdgcn_readlane(end - sum, at);
-        int bin = 255 - 4 * at, held = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            held = __builtin_amdgcn_readlane(n[i], at);
-            if (before + held >= need) { break; }
-            before += held;
-            --bin;
-        }
-        wave_sync();
-        need -= before; // of this bin
-        base += static_cast<uint32_t>(bin) << shift;
-        if (held == need) { return Threshold{base - 1u, 0}; } // the whole bin; nothing else lies at base - 1 (it would not be chosen)
-        if (shift == 0) { return Threshold{base, need}; }
-        span = (1u << shift) - 1u;
     }
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) { above += static_cast<int>(__popcll(__ballot(k[i] > lo))); }
+    return Threshold{lo, want - total(above)};
 }
 
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) { v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), d))); }
+    return v;
+}
+
+// What the waves that choose for one token share.
+struct Shared {
+    int count[2][16]; // by turns: a wave may be a step ahead
+    uint32_t least[16], most[16];
+    int taken[16], equal[16];
+};
+
+// The list of one token from its keys of = [0, count) by WAVES waves, R keys a lane; block `first` + i has key i. Returns how many.
+template <int R, int WAVES>
+__device__ __forceinline__ int choose(const uint32_t* of, int count, int want, int first, int32_t* out, int lane, int wave, Shared& sh) {
+    uint32_t k[R];
+    uint32_t most = 0u, least = 0u; // least as its complement
+    int there = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int at = (wave * R + i) * 64 + lane; // a wave's keys stand together, so lists come out in order
+        k[i] = at < count ? of[at] : 0u;
+        there += static_cast<int>(__popcll(__ballot(k[i] != 0u)));
+        most = max(most, k[i]);
+        least = max(least, k[i] != 0u ? ~k[i] : 0u);
+    }
+    int turn = 0;
+    const auto total = [&](int n) {
+        if constexpr (WAVES == 1) {
+            return n;
+        } else {
+            if (lane == 0) { sh.count[turn][wave] = n; }
+            __syncthreads();
+            int s = 0;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) { s += sh.count[turn][i]; }
+            turn ^= 1;
+            return __builtin_amdgcn_readfirstlane(s);
+        }
+    };
+    most = wave_max_u32(most);
+    least = wave_max_u32(least);
+    if constexpr (WAVES > 1) {
+        if (lane == 0) {
+            sh.most[wave] = most;
+            sh.least[wave] = least;
+        }
+    }
+    there = total(there);
+    if constexpr (WAVES > 1) {
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            most = max(most, sh.most[i]);
+            least = max(least, sh.least[i]);
+        }
+    }
+    Threshold y{0u, 0};
+    if (there > want) { y = top_keys<R>(k, want, __builtin_amdgcn_readfirstlane(~least), __builtin_amdgcn_readfirstlane(most), total); }
+    // what the waves before take, of both kinds
+    int taken = 0, equal = 0;
+    if constexpr (WAVES > 1) {
+        int above = 0, same = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            above += static_cast<int>(__popcll(__ballot(k[i] > y.than)));
+            same += static_cast<int>(__popcll(__ballot(k[i] == y.than && k[i] != 0u)));
+        }
+        if (lane == 0) {
+            sh.taken[wave] = above;
+            sh.equal[wave] = same;
+        }
+        __syncthreads();
+        for (int i = 0; i < wave; ++i) {
+            const int e = min(sh.equal[i], y.equal - equal);
+            taken += sh.taken[i] + e;
+            equal += e;
+        }
+    }
+    int left = y.equal - equal;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const uint64_t below = (uint64_t{1} << lane) - 1;
+        const uint64_t same = __ballot(k[i] == y.than && k[i] != 0u);
+        const bool take = k[i] > y.than || (((same >> lane) & 1u) != 0u && static_cast<int>(__popcll(same & below)) < left);
+        const uint64_t all = __ballot(take);
+        if (take) { out[taken + __popcll(all & below)] = first + (wave * R + i) * 64 + lane; }
+        taken += static_cast<int>(__popcll(all));
+        left = max(0, left - static_cast<int>(__popcll(same)));
+    }
+    return min(there, want);
+}
+
+template <int WAVES>
+__device__ __forceinline__ int choose(const uint32_t* of, int count, int want, int first, int32_t* out, int lane, int wave, Shared& sh) {
+    const int r = (count + 64 * WAVES - 1) / (64 * WAVES);
+    if (r <= 2) { return choose<2, WAVES>(of, count, want, first, out, lane, wave, sh); }
+    if (r <= 4) { return choose<4, WAVES>(of, count, want, first, out, lane, wave, sh); }
+    if (r <= 8) { return choose<8, WAVES>(of, count, want, first, out, lane, wave, sh); }
+    if (r <= 16) { return choose<16, WAVES>(of, count, want, first, out, lane, wave, sh); }
+    return choose<32, WAVES>(of, count, want, first, out, lane, wave, sh);
+}
+
+// NW: 4 for tiles of 16 tokens (a wave chooses for a token, of at most 2,048 keys), 16 for smaller ones (all waves for one).
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
     constexpr int L = D / 8;
     constexpr int PAD = 16;
     extern __shared__ uint32_t keys[]; // [tile token][cap]
     __shared__ __attribute__((aligned(16))) char qcode[16 * (D + PAD)];
-    __shared__ uint32_t hist[NW][256];
+    __shared__ Shared sh;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.x % x.c.Hkv;
     const int bs = x.b.shift;
     const int tt = 1 << x.tile_shift;
-    const Found f = find_unit(x.a.starts, x.a.history, x.c.B, x.a.tokens, blockIdx.x / x.c.Hkv, lane, [&](const Span& s) {
+    const Found f = find_unit(x.c.B, blockIdx.x / x.c.Hkv, lane, [&](int b) { return span_of(x.a.starts, x.a.history, b, x.a.tokens); }, [&](const Span& s) {
         // a sequence outside the envelope takes no part
         return s.tokens <= x.a.max_new && static_cast<int64_t>(s.history) + s.tokens <= x.a.max_keys ? (s.tokens + tt - 1) >> x.tile_shift : 0;
     });
@@ -304,33 +323,47 @@ __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) { q[i] = *reinterpret_cast<const i4*>(qcode + c * (D + PAD) + 64 * i + 16 * g); }
     const int from = first & ~15;
-#pragma unroll 4
-    for (int b0 = from + 16 * wave; b0 <= last; b0 += 16 * NW) {
-        const int blk = b0 + c;
-        int32_t page = -1;
-        if (blk >= first && blk <= last && (blk >> per) < x.c.max_pages) { page = table[blk >> per]; }
-        const bool there = page >= 0 && page < x.c.pages;
-        const int64_t slot = (static_cast<int64_t>(h) << per) + (blk & ((1 << per) - 1));
-        i4 k[D / 64];
-        float scale = 0.0f;
+    constexpr int AHEAD = 4; // sets of 16 blocks on their way
+    for (int b0 = from + 16 * wave; b0 <= last; b0 += 16 * NW * AHEAD) {
+        int32_t page[AHEAD];
+        i4 k[AHEAD][D / 64];
+        float scale[AHEAD];
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) { k[i] = i4{0, 0, 0, 0}; }
-        if (there) {
-            const char* src = x.b.codes + page * x.b.code_page + slot * D + 16 * g;
-#pragma unroll
-            for (int i = 0; i < D / 64; ++i) { k[i] = *reinterpret_cast<const i4*>(src + 64 * i); }
-            scale = *reinterpret_cast<const float*>(x.b.scales + page * x.b.scale_page + slot * 4);
+        for (int u = 0; u < AHEAD; ++u) {
+            const int blk = b0 + 16 * NW * u + c;
+            page[u] = -1;
+            if (blk >= first && blk <= last && (blk >> per) < x.c.max_pages) { page[u] = table[blk >> per]; }
         }
-        i4 acc = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) { acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[i], k[i], acc, 0, 0, 0); }
+        for (int u = 0; u < AHEAD; ++u) {
+            const int blk = b0 + 16 * NW * u + c;
+            page[u] = page[u] >= 0 && page[u] < x.c.pages ? page[u] : -1;
+            const int64_t slot = (static_cast<int64_t>(h) << per) + (blk & ((1 << per) - 1));
+            scale[u] = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) { // token 4 g + r, block c
-            const int t = 4 * g + r;
-            if (t < tt) {
-                const bool open = there && blk <= ((pos0 + t) >> bs) - local;
-                const float score = scale == INFINITY ? INFINITY : scale * static_cast<float>(acc[r]);
-                keys[t * x.cap + blk - from] = open ? ordered(score) : 0u;
+            for (int i = 0; i < D / 64; ++i) { k[u][i] = i4{0, 0, 0, 0}; }
+            if (page[u] >= 0) {
+                const char* src = x.b.codes + page[u] * x.b.code_page + slot * D + 16 * g;
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) { k[u][i] = *reinterpret_cast<const i4*>(src + 64 * i); }
+                scale[u] = *reinterpret_cast<const float*>(x.b.scales + page[u] * x.b.scale_page + slot * 4);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int blk = b0 + 16 * NW * u + c;
+            if (blk - c > last) { continue; }
+            i4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) { acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[i], k[u][i], acc, 0, 0, 0); }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) { // token 4 g + r, block c
+                const int t = 4 * g + r;
+                if (t < tt) {
+                    const bool open = page[u] >= 0 && blk <= ((pos0 + t) >> bs) - local;
+                    const float score = scale[u] == INFINITY ? INFINITY : scale[u] * static_cast<float>(acc[r]);
+                    keys[t * x.cap + blk - from] = open ? ordered(score) : 0u;
+                }
             }
         }
     }
@@ -338,32 +371,24 @@ __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
 
     // ---- lists
     const int S = first + local + x.a.top;
-    for (int t = wave; t < tokens; t += NW) {
+    constexpr int TOGETHER = NW == 4 ? 1 : NW; // waves of a token
+    for (int t = NW == 4 ? wave : 0; t < tokens; t += NW / TOGETHER) {
         const int own = (pos0 + t) >> bs;
         const int64_t token = f.s.start + t0 + t;
         int32_t* out = x.a.selected + (token * x.c.Hkv + h) * S;
-        const int heads = min(first, own + 1);                 // the first blocks
-        const int tail = max(heads, own - local + 1);          // the last ones: tail .. own
-        const int count = max(0, own - local - first + 1);     // blocks between
-        const uint32_t* of = keys + t * x.cap + (first - from);
-        for (int i = lane; i < heads; i += 64) { out[i] = i; }
+        const int part = TOGETHER == 1 ? 0 : wave;
+        const int heads = min(first, own + 1);        // the first blocks
+        const int tail = max(heads, own - local + 1); // the last ones: tail .. own
+        const int count = own - local - first + 1;    // blocks between
         int taken = heads;
         if (x.a.top > 0 && count > 0) {
-            const Threshold y = top_keys(of, count, x.a.top, lane, hist[wave]);
-            int equal = y.equal;
-            for (int i0 = 0; i0 < count; i0 += 64) {
-                const uint32_t k = i0 + lane < count ? of[i0 + lane] : 0u;
-                const uint64_t same = __ballot(k == y.than && k != 0u);
-                const bool take = k > y.than || (k == y.than && k != 0u && __popcll(same & ((uint64_t{1} << lane) - 1)) < equal);
-                const uint64_t all = __ballot(take);
-                if (take) { out[taken + __popcll(all & ((uint64_t{1} << lane) - 1))] = first + i0 + lane; }
-                taken += __popcll(all);
-                equal = max(0, equal - static_cast<int>(__popcll(same)));
-            }
+            taken += choose<TOGETHER>(keys + t * x.cap + (first - from), count, x.a.top, first, out + heads, lane, part, sh);
         }
-        for (int i = tail + lane; i <= own; i += 64) { out[taken + i - tail] = i; }
-        taken += own - tail + 1;
-        for (int i = taken + lane; i < S; i += 64) { out[i] = -1; }
+        if (part == 0) {
+            for (int i = lane; i < heads; i += 64) { out[i] = i; }
+            for (int i = tail + lane; i <= own; i += 64) { out[taken + i - tail] = i; }
+            for (int i = taken + own - tail + 1 + lane; i < S; i += 64) { out[i] = -1; }
+        }
     }
 }
 
@@ -372,11 +397,10 @@ void select(const SelectArgs& x, int64_t tiles, hipStream_t stream) {
     const size_t lds = (static_cast<size_t>(x.cap) << x.tile_shift) * 4;
     const int64_t grid = tiles * x.c.Hkv;
     if (grid > 0x3FFFFF) { throw Unsupported("paged block selection: more than 2^22 workgroups are not built"); }
-    // many waves for the blocks of a single token, few for a tile of tokens
-    if (x.tile_shift == 0) {
-        hipLaunchKernelGGL((block_select_kernel<D, 16>), dim3(static_cast<uint32_t>(grid)), dim3(1024), lds, stream, x);
-    } else {
+    if (x.tile_shift == 4) {
         hipLaunchKernelGGL((block_select_kernel<D, 4>), dim3(static_cast<uint32_t>(grid)), dim3(256), lds, stream, x);
+    } else {
+        hipLaunchKernelGGL((block_select_kernel<D, 16>), dim3(static_cast<uint32_t>(grid)), dim3(1024), lds, stream, x);
     }
     check_launch("block_select_kernel");
 }

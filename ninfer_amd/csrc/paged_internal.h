@@ -130,7 +130,7 @@ struct BlockSelect {
 size_t block_select_bytes(int32_t Hkv, int32_t D, int64_t tokens, int32_t B, int32_t max_new, int32_t max_keys, int32_t block_shift);
 void launch_block_select(const BlockSelect& a, const PagedRef& cache, const BlocksRef& blocks, void* workspace, hipStream_t stream);
 
-size_t sparse_attention_bytes(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t selected, int32_t block_shift);
+size_t sparse_attention_bytes(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t B, int32_t selected, int32_t block_shift);
 void launch_sparse_attention(const PagedAttention& a, const int32_t* selected, int32_t count, int32_t block_shift, const PagedRef& cache,
                              void* workspace, hipStream_t stream);
 

@@ -63,19 +63,19 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 
-// A bit per page in dynamic LDS (kinds of pages: free, or in use), 64 pages a word, and the words' running sums.
+// A bit per page in dynamic LDS, set for the free ones, 64 pages a word, and the words' running sums.
 struct Bits {
     uint64_t* word;
-    int32_t* sum; // bits before the word
+    int32_t* sum; // free pages before the word
     int words;
-    int total;
+    int pages;
+    int total; // free pages
 };
 
-// The bits of pages p with want(refs[p]), for the whole workgroup. `part` is scratch.
-template <typename F>
-__device__ Bits page_bits(const int32_t* refs, int pages, uint64_t* lds, int32_t* part, F want) {
+// For the whole workgroup. `part` is scratch.
+__device__ Bits free_pages(const int32_t* refs, int pages, uint64_t* lds, int32_t* part) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    Bits b{lds, nullptr, (pages + 63) / 64, 0};
+    Bits b{lds, nullptr, (pages + 63) / 64, pages, 0};
     b.sum = reinterpret_cast<int32_t*>(lds + b.words);
     constexpr int kAhead = 16; // words of a wave on their way
     for (int w0 = wave; w0 < b.words; w0 += kAhead * kWaves) {
@@ -85,7 +85,7 @@ __device__ Bits page_bits(const int32_t* refs, int pages, uint64_t* lds, int32_t
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int w = w0 + i * kWaves;
-            const uint64_t m = __ballot(64 * w + lane < pages && want(n[i]));
+            const uint64_t m = __ballot(64 * w + lane < pages && n[i] == 0);
             if (lane == 0 && w < b.words) { b.word[w] = m; }
         }
     }
@@ -111,20 +111,22 @@ __device__ Bits page_bits(const int32_t* refs, int pages, uint64_t* lds, int32_t
     return b;
 }
 
-// The page of the k-th bit (from 0), the lowest first; -1 where there is none.
+// The k-th free page (USED: page in use) from 0, the lowest first; -1 where there is none.
+template <bool USED>
 __device__ int nth_page(const Bits& b, int k) {
-    if (k < 0 || k >= b.total) { return -1; }
-    int lo = 0, hi = b.words; // the last word with at most k bits before it
+    if (k < 0 || k >= (USED ? b.pages - b.total : b.total)) { return -1; }
+    const auto before = [&](int w) { return USED ? 64 * w - b.sum[w] : b.sum[w]; };
+    int lo = 0, hi = b.words; // the last word with at most k of them before it
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (b.sum[mid] <= k) {
+        if (before(mid) <= k) {
             lo = mid;
         } else {
             hi = mid;
         }
     }
-    uint64_t m = b.word[lo];
-    int left = k - b.sum[lo];
+    uint64_t m = USED ? ~b.word[lo] : b.word[lo]; // (pages past the last one stand behind all others)
+    int left = k - before(lo);
     int at = 0;
 #pragma unroll
     for (int half = 32; half > 0; half /= 2) {
@@ -182,13 +184,15 @@ __global__ __launch_bounds__(kThreads) void pages_reserve_kernel(PageTable t, co
     extern __shared__ uint64_t lds[];
     __shared__ int32_t part[kWaves];
     __shared__ int32_t begin[kPagedMaxBatch + 1]; // of a sequence's entries among all
+    __shared__ int32_t first[kPagedMaxBatch];     // entry of its new rows
     __shared__ int32_t lacking[kPagedMaxBatch];   // the first entry that got no page
-    const Bits free = page_bits(t.refs, t.pages, lds, part, [](int32_t n) { return n == 0; });
     const int b0 = threadIdx.x;
     const Entries mine = b0 < t.B ? entries_of(t, starts, history, b0) : Entries{0, 0, 0, 0};
+    const Bits free = free_pages(t.refs, t.pages, lds, part);
     const Sum s = block_sum(mine.count, part);
     if (b0 < t.B) {
         begin[b0] = s.before;
+        first[b0] = mine.first;
         lacking[b0] = 0x7fffffff;
     }
     if (b0 == 0) { begin[t.B] = s.total; }
@@ -208,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void pages_reserve_kernel(PageTable t, co
                 }
             }
             b = lo;
-            entry = (history[b] >> t.shift) + i - begin[b];
+            entry = first[b] + i - begin[b];
             // (starts that descend may promise more entries than whole numbers count)
             if (i >= begin[b] && i < begin[b + 1] && entry >= 0 && entry < t.max_pages) {
                 const int32_t page = t.table[b * t.row + entry];
@@ -217,7 +221,7 @@ __global__ __launch_bounds__(kThreads) void pages_reserve_kernel(PageTable t, co
         }
         const Sum n = block_sum(need, part);
         if (need) {
-            const int page = nth_page(free, handed + n.before);
+            const int page = nth_page<false>(free, handed + n.before);
             if (page >= 0) {
                 t.table[b * t.row + entry] = page;
                 t.refs[page] = 1;
@@ -256,26 +260,32 @@ __global__ __launch_bounds__(kThreads) void pages_fork_kernel(PageTable t, const
     extern __shared__ uint64_t lds[];
     __shared__ int32_t part[kWaves];
     __shared__ int32_t of[kPagedMaxBatch], to[kPagedMaxBatch], rows[kPagedMaxBatch], fresh[kPagedMaxBatch];
+    __shared__ int32_t claim[kPagedMaxBatch]; // of a sequence: the first pair whose child it is, -1 for a parent
     const int i = threadIdx.x;
+    int32_t parent = -1, child = -1, length = 0;
     if (i < n) {
-        of[i] = parents[i];
-        to[i] = children[i];
+        parent = parents[i];
+        child = children[i];
+        if (parent >= 0 && parent < t.B) { length = max(0, history[parent]); }
+        of[i] = parent;
+        to[i] = child;
     }
-    const Bits free = page_bits(t.refs, t.pages, lds, part, [](int32_t r) { return r == 0; }); // before anything is given back
-    bool ok = i < n && of[i] >= 0 && of[i] < t.B && to[i] >= 0 && to[i] < t.B;
-    for (int j = 0; j < n && ok; ++j) {
-        if (to[i] == of[j] || (j < i && to[j] == to[i])) { ok = false; } // a parent, or an earlier pair's child
-    }
-    const int32_t length = ok ? max(0, history[of[i]]) : 0;
+    claim[i] = 0x7fffffff;
+    __syncthreads();
+    // (a pair that names no sequence as its parent claims its child all the same: it is left out for an earlier pair's sake)
+    if (i < n && child >= 0 && child < t.B) { atomicMin(&claim[child], i); }
+    if (i < n && parent >= 0 && parent < t.B) { atomicMin(&claim[parent], -1); }
+    const Bits free = free_pages(t.refs, t.pages, lds, part); // before anything is given back
+    const bool ok = i < n && parent >= 0 && parent < t.B && child >= 0 && child < t.B && claim[child] == i;
     const int whole = min(length >> t.shift, t.max_pages);
     // the last page's rows, where a page holds them
     int32_t last = -1;
     if (ok && whole < t.max_pages && (length & ((1 << t.shift) - 1)) != 0) {
-        last = t.table[of[i] * t.row + whole];
+        last = t.table[parent * t.row + whole];
         last = last >= 0 && last < t.pages ? last : -1;
     }
     const Sum s = block_sum(last >= 0 ? 1 : 0, part);
-    const int page = last >= 0 ? nth_page(free, s.before) : -1;
+    const int page = last >= 0 ? nth_page<false>(free, s.before) : -1;
     if (i < n) {
         rows[i] = ok ? (page >= 0 ? length : whole << t.shift) : -1;
         fresh[i] = page;
@@ -299,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void pages_fork_kernel(PageTable t, const
         if (now >= 0 && now < t.pages) { atomicAdd(&t.refs[now], 1); }
         *at = now;
     }
-    if (ok) { history[to[i]] = rows[i]; }
+    if (ok) { history[child] = rows[i]; }
 }
 
 // ---- moving together -----------------------------------------------------------------------------
@@ -308,25 +318,22 @@ __global__ __launch_bounds__(kThreads) void pages_fork_kernel(PageTable t, const
 __global__ __launch_bounds__(kThreads) void pages_compact_kernel(PageTable t, int32_t* src, int32_t* dst, int n, int32_t* moved) {
     extern __shared__ uint64_t lds[];
     __shared__ int32_t part[kWaves];
-    const Bits free = page_bits(t.refs, t.pages, lds, part, [](int32_t r) { return r == 0; });
-    // pages in use: t.pages - free.total. As many moves as free pages lie below that.
+    const Bits free = free_pages(t.refs, t.pages, lds, part);
+    // as many moves as free pages lie below the number of those in use
     const int used = t.pages - free.total;
     int holes = 0;
-    if (used > 0 && used < t.pages) { holes = free.sum[used / 64] + __popcll(free.word[used / 64] & ((uint64_t{1} << (used & 63)) - 1)); }
+    if (used < t.pages) { holes = free.sum[used / 64] + __popcll(free.word[used / 64] & ((uint64_t{1} << (used & 63)) - 1)); }
     const int count = min(holes, n);
-    // the bits of the pages in use, from here on
-    __syncthreads();
-    for (int k = threadIdx.x; k < n; k += kThreads) { dst[k] = k < count ? nth_page(free, k) : -1; }
-    __syncthreads();
-    const Bits inuse = page_bits(t.refs, t.pages, lds, part, [](int32_t r) { return r != 0; });
     for (int k = threadIdx.x; k < n; k += kThreads) {
-        int32_t from = -1;
+        int32_t from = -1, to = -1;
         if (k < count) {
-            from = nth_page(inuse, used - 1 - k);
-            t.refs[dst[k]] = t.refs[from];
+            to = nth_page<false>(free, k);
+            from = nth_page<true>(free, used - 1 - k);
+            t.refs[to] = t.refs[from];
             t.refs[from] = 0;
         }
         src[k] = from;
+        dst[k] = to;
     }
     if (threadIdx.x == 0) { *moved = count; }
 }

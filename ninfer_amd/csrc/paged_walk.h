@@ -234,6 +234,49 @@ __device__ __forceinline__ constexpr int out_dim(int t, int m) {
     return BF ? 128 * (t >> 3) + 8 * m + (t & 7) : 64 * (t >> 2) + 4 * m + (t & 3);
 }
 
+// Row tile nt's row of the lane: its query from `src` (a row without one: zeros) and its empty state.
+template <int D, bool BF, int NT>
+__device__ __forceinline__ void init_row(const PagedAttnArgs& x, const uint16_t* src, bool valid, int nt, int g, Rows<D, BF, NT>& r) {
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+        // INT8: step 2 i + j holds dims 64 i + 16 g + 8 j ..; BF16: step i dims 32 i + 8 g ..
+        const int dim = BF ? 32 * k + 8 * g : 64 * (k >> 1) + 16 * g + 8 * (k & 1);
+        r.q[nt][k] = valid ? *reinterpret_cast<const u4*>(src + dim) : u4{0u, 0u, 0u, 0u};
+    }
+    if constexpr (BF) {
+        r.rowmul[nt] = x.scale_log2;
+    } else {
+        float amax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(r.q[nt][k][w] << 16)), fabsf(__uint_as_float(r.q[nt][k][w] & 0xffff0000u))));
+            }
+        }
+        amax = group4_max(amax);
+        int fexp = 0; // amax * 2^fexp in [2^14, 2^15): what FP16 then rounds is below 2^-39 of amax
+        if (amax > 0.0f && amax < INFINITY) { fexp = 14 - max(static_cast<int>((__float_as_uint(amax) >> 23) & 0xff) - 127, -46); }
+        const float factor = ldexpf(1.0f, fexp);
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t y = r.q[nt][k][w];
+                const h2 p = {static_cast<_Float16>(__uint_as_float(y << 16) * factor),
+                              static_cast<_Float16>(__uint_as_float(y & 0xffff0000u) * factor)};
+                r.q[nt][k][w] = __builtin_bit_cast(uint32_t, p);
+            }
+        }
+        r.rowmul[nt] = fminf(ldexpf(x.scale_log2, -fexp), kLargest); // finite: a score of zero stays one
+    }
+    r.m[nt] = -INFINITY;
+    r.l[nt] = 0.0f;
+#pragma unroll
+    for (int t16 = 0; t16 < D / 16; ++t16) { r.O[nt][t16] = f4{0.f, 0.f, 0.f, 0.f}; }
+}
+
+// Rows row0 .. of the sequence's, token after token.
 template <int D, bool BF, int NT>
 __device__ __forceinline__ void init_rows(const PagedAttnArgs& x, const Seq& s, int h, int row0, int c, int g, Rows<D, BF, NT>& r) {
     const int rows = s.tokens * x.G;
@@ -246,44 +289,7 @@ __device__ __forceinline__ void init_rows(const PagedAttnArgs& x, const Seq& s, 
         const int t = valid ? row / x.G : 0;
         const int head = h * x.G + (valid ? row - t * x.G : 0);
         r.pos[nt] = valid ? s.history + t : -1;
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(x.a.q.data + (s.start + t) * x.a.q.token_stride) + head * D;
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-            // INT8: step 2 i + j holds dims 64 i + 16 g + 8 j ..; BF16: step i dims 32 i + 8 g ..
-            const int dim = BF ? 32 * k + 8 * g : 64 * (k >> 1) + 16 * g + 8 * (k & 1);
-            r.q[nt][k] = valid ? *reinterpret_cast<const u4*>(src + dim) : u4{0u, 0u, 0u, 0u};
-        }
-        if constexpr (BF) {
-            r.rowmul[nt] = x.scale_log2;
-        } else {
-            float amax = 0.0f;
-#pragma unroll
-            for (int k = 0; k < D / 32; ++k) {
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(r.q[nt][k][w] << 16)), fabsf(__uint_as_float(r.q[nt][k][w] & 0xffff0000u))));
-                }
-            }
-            amax = group4_max(amax);
-            int fexp = 0; // amax * 2^fexp in [2^14, 2^15): what FP16 then rounds is below 2^-39 of amax
-            if (amax > 0.0f && amax < INFINITY) { fexp = 14 - max(static_cast<int>((__float_as_uint(amax) >> 23) & 0xff) - 127, -46); }
-            const float factor = ldexpf(1.0f, fexp);
-#pragma unroll
-            for (int k = 0; k < D / 32; ++k) {
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t y = r.q[nt][k][w];
-                    const h2 p = {static_cast<_Float16>(__uint_as_float(y << 16) * factor),
-                                  static_cast<_Float16>(__uint_as_float(y & 0xffff0000u) * factor)};
-                    r.q[nt][k][w] = __builtin_bit_cast(uint32_t, p);
-                }
-            }
-            r.rowmul[nt] = fminf(ldexpf(x.scale_log2, -fexp), kLargest); // finite: a score of zero stays one
-        }
-        r.m[nt] = -INFINITY;
-        r.l[nt] = 0.0f;
-#pragma unroll
-        for (int t16 = 0; t16 < D / 16; ++t16) { r.O[nt][t16] = f4{0.f, 0.f, 0.f, 0.f}; }
+        init_row<D, BF, NT>(x, reinterpret_cast<const uint16_t*>(x.a.q.data + (s.start + t) * x.a.q.token_stride) + head * D, valid, nt, g, r);
     }
     if (row0 < rows) {
         r.lo = s.history + row0 / x.G;
@@ -616,12 +622,11 @@ __device__ __forceinline__ void store_part(const PagedAttnArgs& x, const Rows<D,
     if (g == 0) { *reinterpret_cast<float2*>(x.part_ml + 2 * at) = float2{M, L}; }
 }
 
-// The same as row `row` of sequence s in the output.
+// The same as token `token`'s head `head` of the group in the output.
 template <int D, bool BF, int NT>
-__device__ __forceinline__ void store_out(const PagedAttnArgs& x, const Seq& s, int h, int row, const Rows<D, BF, NT>& r, int nt, float L, int g) {
+__device__ __forceinline__ void store_out(const PagedAttnArgs& x, int token, int h, int head, const Rows<D, BF, NT>& r, int nt, float L, int g) {
     constexpr int RUN = BF ? 8 : 4;
-    const int t = row / x.G;
-    uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + (s.start + t) * x.a.out.token_stride) + (h * x.G + row - t * x.G) * D;
+    uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + token * x.a.out.token_stride) + (h * x.G + head) * D;
 #pragma unroll
     for (int i = 0; i < D / (16 * RUN); ++i) {
 #pragma unroll
