@@ -143,34 +143,58 @@ struct Threshold {
     int equal;
 };
 
-// The `want` largest of the keys that WAVES waves hold, R a lane (zeros are none): the interval of the smallest chosen one is halved
-// until as many keys as are wanted lie at its middle or above, or one value is left. About a dozen steps for scores that
-// differ. `total` sums a count over the waves.
-template <int R, typename F>
-__device__ __forceinline__ Threshold top_keys(const uint32_t (&k)[R], int want, uint32_t lo, uint32_t hi, F total) {
-    while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo) / 2 + 1;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < R; ++i) { n += static_cast<int>(__popcll(__ballot(k[i] >= mid))); }
-        n = total(n);
+__device__ __forceinline__ float value_of(uint32_t key) {
+    return __uint_as_float(key ^ ((key & 0x80000000u) != 0u ? 0x80000000u : 0xffffffffu));
+}
+
+// The `want` largest of `there` keys from lo to hi (zeros are none); `count_from` says how many there are from a key on. The interval of the
+// smallest chosen key closes in from both sides until as many keys as are wanted lie at its middle or above, or one value is
+// left: first where the counts at its ends put the middle among the scores' values (six to nine steps for scores spread as
+// sums are; halving takes 14), then, for scores that are not, at the keys' own middle.
+template <typename F>
+__device__ __forceinline__ Threshold top_keys(F count_from, int there, int want, uint32_t lo, uint32_t hi) {
+    float over = static_cast<float>(there - want), under = static_cast<float>(want); // keys from lo on that are too many, above hi too few
+    int side = 0;
+#pragma unroll 1
+    for (int step = 0; lo < hi; ++step) {
+        uint32_t mid = lo + (hi - lo) / 2 + 1;
+        if (step < 12) {
+            const float a = value_of(lo), b = value_of(hi);
+            const float share = fminf(0.984375f, fmaxf(0.015625f, over * __builtin_amdgcn_rcpf(over + under)));
+            const float v = a + (b - a) * share;
+            if (v > a && v < b) { mid = __builtin_amdgcn_readfirstlane(max(lo + 1u, min(hi, ordered(v)))); } // (not for infinite ends)
+        }
+        const int n = count_from(mid);
         if (n == want) { return Threshold{mid - 1u, 0}; } // (a key of mid - 1 is not chosen: none is counted)
+        // an end that stays twice counts half: the middle moves towards it
         if (n > want) {
             lo = mid;
+            over = static_cast<float>(n - want);
+            under *= side > 0 ? 0.5f : 1.0f;
+            side = 1;
         } else {
             hi = mid - 1u;
+            under = static_cast<float>(want - n);
+            over *= side < 0 ? 0.5f : 1.0f;
+            side = -1;
         }
     }
-    int above = 0;
-#pragma unroll
-    for (int i = 0; i < R; ++i) { above += static_cast<int>(__popcll(__ballot(k[i] > lo))); }
-    return Threshold{lo, want - total(above)};
+    return Threshold{lo, want - (lo == 0xffffffffu ? 0 : count_from(lo + 1u))};
+}
+
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t max_step(uint32_t v) {
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROW_MASK, 0xf, true)));
 }
 
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) { v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), d))); }
-    return v;
+    v = max_step<0x111, 0xf>(v);
+    v = max_step<0x112, 0xf>(v);
+    v = max_step<0x114, 0xf>(v);
+    v = max_step<0x118, 0xf>(v);
+    v = max_step<0x142, 0xa>(v);
+    v = max_step<0x143, 0xc>(v);
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
 
 // What the waves that choose for one token share.
@@ -225,7 +249,16 @@ __device__ __forceinline__ int choose(const uint32_t* of, int count, int want, i
         }
     }
     Threshold y{0u, 0};
-    if (there > want) { y = top_keys<R>(k, want, __builtin_amdgcn_readfirstlane(~least), __builtin_amdgcn_readfirstlane(most), total); }
+    if (there > want) {
+        y = top_keys(
+            [&](uint32_t from) {
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < R; ++i) { n += static_cast<int>(__popcll(__ballot(k[i] >= from))); }
+                return total(n);
+            },
+            there, want, __builtin_amdgcn_readfirstlane(~least), __builtin_amdgcn_readfirstlane(most));
+    }
     // what the waves before take, of both kinds
     int taken = 0, equal = 0;
     if constexpr (WAVES > 1) {
@@ -247,9 +280,19 @@ __device__ __forceinline__ int choose(const uint32_t* of, int count, int want, i
         }
     }
     int left = y.equal - equal;
+    const uint64_t below = (uint64_t{1} << lane) - 1;
+    if (left == 0) { // no choice among equals
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const bool take = k[i] > y.than;
+            const uint64_t all = __ballot(take);
+            if (take) { out[taken + __popcll(all & below)] = first + (wave * R + i) * 64 + lane; }
+            taken += static_cast<int>(__popcll(all));
+        }
+        return min(there, want);
+    }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const uint64_t below = (uint64_t{1} << lane) - 1;
         const uint64_t same = __ballot(k[i] == y.than && k[i] != 0u);
         const bool take = k[i] > y.than || (((same >> lane) & 1u) != 0u && static_cast<int>(__popcll(same & below)) < left);
         const uint64_t all = __ballot(take);
@@ -263,14 +306,19 @@ __device__ __forceinline__ int choose(const uint32_t* of, int count, int want, i
 template <int WAVES>
 __device__ __forceinline__ int choose(const uint32_t* of, int count, int want, int first, int32_t* out, int lane, int wave, Shared& sh) {
     const int r = (count + 64 * WAVES - 1) / (64 * WAVES);
+    if (r <= 1) { return choose<1, WAVES>(of, count, want, first, out, lane, wave, sh); }
     if (r <= 2) { return choose<2, WAVES>(of, count, want, first, out, lane, wave, sh); }
+    if (r <= 3) { return choose<3, WAVES>(of, count, want, first, out, lane, wave, sh); }
     if (r <= 4) { return choose<4, WAVES>(of, count, want, first, out, lane, wave, sh); }
+    if (r <= 5) { return choose<5, WAVES>(of, count, want, first, out, lane, wave, sh); }
+    if (r <= 6) { return choose<6, WAVES>(of, count, want, first, out, lane, wave, sh); }
     if (r <= 8) { return choose<8, WAVES>(of, count, want, first, out, lane, wave, sh); }
     if (r <= 16) { return choose<16, WAVES>(of, count, want, first, out, lane, wave, sh); }
     return choose<32, WAVES>(of, count, want, first, out, lane, wave, sh);
 }
 
-// NW: 4 for tiles of 16 tokens (a wave chooses for a token, of at most 2,048 keys), 16 for smaller ones (all waves for one).
+// NW: 4 for tiles of 16 tokens (a wave chooses for a token, of at most 2,048 keys), 16 for smaller ones (all waves for one: one wave's walk
+// over 2,048 keys takes longer than the barriers).
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
     constexpr int L = D / 8;
@@ -302,12 +350,18 @@ __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
         const int t = i / L, li = i & (L - 1);
         const char* src = x.a.q.data + static_cast<int64_t>(f.s.start + t0 + t) * x.a.q.token_stride + (h * x.G * D + 8 * li) * 2;
         double sum[8] = {};
-        for (int g = 0; g < x.G; ++g) {
-            const i4 raw = *reinterpret_cast<const i4*>(src + g * (D * 2));
+        for (int g0 = 0; g0 < x.G; g0 += 8) {
+            i4 raw[8]; // eight heads on their way
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t w = static_cast<uint32_t>(raw[e >> 1]);
-                sum[e] += __uint_as_float((e & 1) ? w & 0xffff0000u : w << 16);
+            for (int g = 0; g < 8; ++g) { raw[g] = g0 + g < x.G ? *reinterpret_cast<const i4*>(src + (g0 + g) * (D * 2)) : i4{0, 0, 0, 0}; }
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+                if (g0 + g >= x.G) { break; }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t w = static_cast<uint32_t>(raw[g][e >> 1]);
+                    sum[e] += __uint_as_float((e & 1) ? w & 0xffff0000u : w << 16);
+                }
             }
         }
         const double amax = head_amax<D>(sum);
@@ -323,7 +377,12 @@ __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) { q[i] = *reinterpret_cast<const i4*>(qcode + c * (D + PAD) + 64 * i + 16 * g); }
     const int from = first & ~15;
-    constexpr int AHEAD = 4; // sets of 16 blocks on their way
+    constexpr bool FULL = NW == 4; // tiles of 16 tokens
+    int lasts[4];                  // of tokens 4 g .. 4 g + 3: the last block to choose
+    uint32_t* to = keys + 4 * g * x.cap + c - from;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) { lasts[r] = ((pos0 + 4 * g + r) >> bs) - local; }
+    constexpr int AHEAD = NW == 4 ? 2 : 4; // sets of 16 blocks on their way
     for (int b0 = from + 16 * wave; b0 <= last; b0 += 16 * NW * AHEAD) {
         int32_t page[AHEAD];
         i4 k[AHEAD][D / 64];
@@ -358,12 +417,9 @@ __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
             for (int i = 0; i < D / 64; ++i) { acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[i], k[u][i], acc, 0, 0, 0); }
 #pragma unroll
             for (int r = 0; r < 4; ++r) { // token 4 g + r, block c
-                const int t = 4 * g + r;
-                if (t < tt) {
-                    const bool open = page[u] >= 0 && blk <= ((pos0 + t) >> bs) - local;
-                    const float score = scale[u] == INFINITY ? INFINITY : scale[u] * static_cast<float>(acc[r]);
-                    keys[t * x.cap + blk - from] = open ? ordered(score) : 0u;
-                }
+                const float score = scale[u] * static_cast<float>(acc[r]);
+                const uint32_t key = scale[u] == INFINITY ? 0xff800000u : ordered(score);
+                if (FULL || 4 * g + r < tt) { to[r * x.cap + blk - c] = page[u] >= 0 && blk <= lasts[r] ? key : 0u; }
             }
         }
     }
