@@ -1,20 +1,22 @@
 // Attention of packed new tokens over selected blocks of a paged KV cache on gfx950.
 //
 // Mathematics: token n at position p has for every KV head a list of blocks; it sees the rows j <= p of those blocks whose page
-// exists (an entry that stands twice counts twice), out = sum_j softmax_j(scale * q . K_j) V_j in one pass with a running
+// exists (one that stands twice counts once), out = sum_j softmax_j(scale * q . K_j) V_j in one pass with a running
 // maximum and sum, zero where no row is seen. Numbers as in paged_attention.hip, whose walk over 32 keys at a time this
 // is: the query heads of the token's KV head are the rows of a 16-row tile, K and V go straight from the cache to the matrix
 // cores' operands.
 //
-// Single tokens: a token and KV head for a wave, or four, or several workgroups' waves, where the tokens alone do not fill the
-// chip. Tokens of one sequence next to each other, up to eight: their lists are merged, since neighbours mostly select the same
-// blocks, and a tile of 32 keys is fetched once for all the tokens that take it.
+// Few tokens: a token and KV head for a wave, or four, or several workgroups' waves, where the tokens alone do not fill the
+// chip (sparse_attn_kernel). Prompts: tokens next to each other mostly select the same blocks, so a workgroup of eight waves
+// merges the lists of up to 64 of them and walks the blocks that any of them takes, decoded once (sparse_many_kernel).
 #include "common.h"
 #include "paged_internal.h"
 #include "paged_place.h"
+#include "paged_tile.h"
 #include "paged_walk.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace nmi {
 namespace {
@@ -27,8 +29,8 @@ struct SparseArgs {
     int32_t row_tiles; // of 16 NT query heads
     int32_t parts;     // workgroups of an item
     int64_t items;     // tokens (or groups of tokens) x KV heads x row tiles, at most
-    int32_t tokens;    // of a group (1: none are formed)
-    int32_t per_tile;  // tokens of a 16-row tile of a group
+    int32_t tokens;    // of a group
+    int32_t per_tile;  // of a 16-row tile of a group
 };
 
 // A token, KV head and row tile.
@@ -61,6 +63,27 @@ __device__ __forceinline__ Item item_of(const SparseArgs& y, int64_t id, int row
     return it;
 }
 
+// Which entries of the item's list repeat an earlier one: bit i of lane l for entry 64 i + l. An ascending list has none; in any
+// other every entry is compared with those before it.
+static_assert(kPagedMaxSelected <= 64 * 32);
+__device__ __forceinline__ uint32_t repeats(const int32_t* list, int count, int lane) {
+    bool ascends = true;
+    for (int i = lane; i < count; i += 64) {
+        const int e = list[i], before = i > 0 ? list[i - 1] : 0;
+        ascends &= e < 0 || i == 0 || (before >= 0 && before < e);
+    }
+    uint32_t bits = 0u;
+    if (__builtin_expect(!__all(ascends), 0)) {
+        for (int i = lane; i < count; i += 64) {
+            const int e = list[i];
+            bool again = false;
+            for (int j = 0; j < i && !again; ++j) { again = list[j] == e; }
+            bits |= again ? 1u << (i >> 6) : 0u;
+        }
+    }
+    return bits;
+}
+
 // A half tile of the walk: its first key's tile of 32, and its page.
 struct Half {
     int32_t tile;
@@ -75,13 +98,16 @@ __device__ __forceinline__ void sparse_walk(const SparseArgs& y, const Item& it,
     const int lt = y.block_shift - 5; // log2(tiles of a block)
     const int32_t* list = y.selected + (static_cast<int64_t>(it.token) * x.c.Hkv + it.h) * y.count;
     const int32_t* table = x.c.table + it.b * x.c.table_row;
+    const uint32_t again = repeats(list, y.count, lane);
     // 64 halves (32 tiles) at a time, one per lane, the next 64 fetched ahead
     const auto fetch = [&](int j) {
         const int v = j + (lane >> 1);
+        const int entry = v >> lt;
+        const uint32_t twice = static_cast<uint32_t>(__shfl(static_cast<int>(again), entry & 63)) >> ((entry >> 6) & 31);
         Half f{0, -1};
         if (v < j1) {
-            const int blk = list[v >> lt];
-            if (blk >= 0 && blk <= (it.pos >> y.block_shift)) {
+            const int blk = list[entry];
+            if (blk >= 0 && blk <= (it.pos >> y.block_shift) && (twice & 1u) == 0u) {
                 f.tile = (blk << lt) + (v & ((1 << lt) - 1));
                 const int key = 32 * f.tile + 16 * (lane & 1);
                 if (key <= it.pos && (key >> x.c.page_shift) < x.c.max_pages) {
@@ -233,119 +259,41 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 
     }
 }
 
-// ---- groups of tokens ------------------------------------------------------------------------------
+// The parts of an item's rows, one after another: D / 4 threads a row, `rows` rows an item.
+template <int D>
+__global__ __launch_bounds__(256) void sparse_merge_kernel(SparseArgs y, int rows) {
+    const PagedAttnArgs& x = y.x;
+    constexpr int TPR = D / 4, RPB = 256 / TPR;
+    const int64_t id = blockIdx.x / (rows / RPB);
+    const int row = static_cast<int>(blockIdx.x % (rows / RPB)) * RPB + threadIdx.x / TPR;
+    const Item it = item_of(y, id, rows, threadIdx.x & 63);
+    if (it.b < 0 || it.row0 + row >= x.G) { return; }
+    const int d = 4 * (threadIdx.x % TPR);
+    Merge m;
+#pragma unroll 4
+    for (int k = 0; k < y.parts; ++k) {
+        const int64_t at = (id * rows + row) * y.parts + k;
+        const float2 ml = *reinterpret_cast<const float2*>(x.part_ml + 2 * at);
+        m.add(ml.x, ml.y, *reinterpret_cast<const f4*>(x.part_o + at * D + d));
+    }
+    uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + it.token * x.a.out.token_stride) + (it.h * x.G + it.row0 + row) * D + d;
+    *reinterpret_cast<u2*>(out) = out_pair(m.O, m.L);
+}
+
+// ---- prompts: groups of tokens over blocks that a workgroup decodes once ----------------------------
 //
-// The rows of a wave: per_tile tokens' heads in each of NT 16-row tiles (token t of the group: tile t / per_tile, its head q row
-// (t % per_tile) G + q). The group's lists become one list of (block, tokens that take it) in LDS, through a bit field
-// of the blocks; a tile of keys is multiplied for the row tiles that take it, and a row whose token does not sees none of it.
-// Lists with an entry twice are not merged: their entries stand one after another, for one token each.
-// A wave stages 32 keys in LDS, whole rows by DMA: straight from the cache, as single tokens do it, every 16-byte piece of K
-// is a cache access of its own, and those bounded it (2,048 tokens over 16 blocks of 64 at 24/4/256 BF16 807 us, the
-// caches busy 70% of that). K makes room for the next tile's as soon as it is in registers, then V; DMAs land in order.
+// A workgroup of eight waves: 8 / WK of them have NT row tiles of per_tile whole tokens each, times WK waves that take
+// different chunks of 32 keys. The lists of its tokens become one, ascending, of (block, tokens that take it) in LDS, through a bit
+// field per block; its chunks are walked in tiles as the many-row kernel of paged_attention.hip does it (decoding, ranges of the
+// FP16 operands and the apart walk of tiles beyond them stand there). A wave skips the chunks that none of its tokens takes,
+// and a row whose token does not take a chunk sees none of it.
+// What bounds it: the waves of a workgroup wait for each other at every tile, whichever of them have work there.
 
-constexpr int kListMost = 512;  // entries of a group's lists
-constexpr int kGroupMost = 8;   // tokens of a group: bits above a block's number
-constexpr int kBlockBits = 24;
-static_assert(kPagedMaxKeys / 32 <= (1 << kBlockBits));
-
-template <int D, bool BF>
-struct Stage {
-    static constexpr int kRow = BF ? 2 * D : D;
-    static constexpr int kPlane = 32 * kRow;
-    static constexpr int kBytes = 2 * kPlane;
-    static constexpr int kHalfDma = 16 * kRow / 1024; // 1 KiB DMAs of a plane's half tile
-    static constexpr int kOps = 2 * kHalfDma + (BF ? 0 : 2 * (D / 128)); // loads of a plane's tile, its scales included
-    static constexpr int kRowsPerDma = 1024 / kRow;
-    static constexpr int kVariants = 8 / kRowsPerDma;
-    static constexpr int kTable = kBytes / 4 < 2048 ? kBytes / 4 : 2048; // blocks of a pass over the lists
-};
-
-// s_waitcnt with at most n vector loads outstanding, and with no LDS operation.
-constexpr int waitcnt_vm(int n) { return (n & 0xf) | ((n >> 4) << 14) | (0x7 << 4) | (0xf << 8); }
-constexpr int kWaitLgkm0 = 0xc07f;
-
-// The 16-byte piece p of LDS row r holds piece p ^ (r & 7) of the cache's row: eight rows' same pieces lie in different banks.
-template <int D, bool BF>
-__device__ __forceinline__ void dma_plane(const PagedAttnArgs& x, const char* plane, int64_t page_stride, int h, int tile, Halves hv, NMI_AS3 char* to, int lane) {
-    using ST = Stage<D, BF>;
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-        const __amdgpu_buffer_rsrc_t rows = half_rows(x, plane, page_stride, ST::kRow, h, tile, kt, hv);
-#pragma unroll
-        for (int q = 0; q < ST::kHalfDma; ++q) {
-            const int in_row = 16 * lane % ST::kRow, row = ST::kRowsPerDma * (q % ST::kVariants) + 16 * lane / ST::kRow;
-            dma16(rows, to + (kt * ST::kHalfDma + q) * 1024, (16 * lane - in_row) + (in_row ^ ((row & 7) * 16)), q * 1024);
-        }
-    }
-}
-
-template <int D, bool BF>
-__device__ __forceinline__ void stage_keys(const PagedAttnArgs& x, int h, int tile, Halves hv, NMI_AS3 char* st, int lane, int g, ChunkK<D, BF>& r) {
-    if constexpr (!BF) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            const __amdgpu_buffer_rsrc_t ksb = half_rows(x, x.c.ks, x.c.ks_page, D / 32, h, tile, kt, hv);
-#pragma unroll
-            for (int w = 0; w < D / 128; ++w) {
-                r.ks[kt][w] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(ksb, 4 * g * (D / 32) + 16 * w, 0, 0));
-            }
-        }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    dma_plane<D, BF>(x, x.c.k, x.c.k_page, h, tile, hv, st, lane);
-    __builtin_amdgcn_sched_barrier(0);
-}
-
-template <int D, bool BF>
-__device__ __forceinline__ void stage_values(const PagedAttnArgs& x, int h, int tile, Halves hv, NMI_AS3 char* st, int lane, int g, ChunkV<D, BF>& r) {
-    if constexpr (!BF) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            const __amdgpu_buffer_rsrc_t vsb = half_rows(x, x.c.vs, x.c.vs_page, D / 32, h, tile, kt, hv);
-#pragma unroll
-            for (int w = 0; w < D / 128; ++w) {
-                r.vs[kt][w] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(vsb, 4 * g * (D / 32) + 16 * w, 0, 0));
-            }
-        }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    dma_plane<D, BF>(x, x.c.v, x.c.v_page, h, tile, hv, st + Stage<D, BF>::kPlane, lane);
-    __builtin_amdgcn_sched_barrier(0);
-}
-
-template <int D, bool BF>
-__device__ __forceinline__ void read_keys(const NMI_AS3 char* st, int c, int g, ChunkK<D, BF>& r) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-        for (int i = 0; i < Chunk<D, BF>::KP; ++i) {
-            r.k[kt][i] = *reinterpret_cast<const NMI_AS3 u4*>(st + (16 * kt + c) * Stage<D, BF>::kRow + (((4 * i + g) ^ (c & 7)) * 16));
-        }
-    }
-}
-
-template <int D, bool BF>
-__device__ __forceinline__ void read_values(const NMI_AS3 char* st, int c, int g, ChunkV<D, BF>& r) {
-    st += Stage<D, BF>::kPlane;
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = 4 * g + j;
-#pragma unroll
-            for (int i = 0; i < Chunk<D, BF>::VP; ++i) {
-                const NMI_AS3 char* at = st + (16 * kt + row) * Stage<D, BF>::kRow;
-                if constexpr (BF) {
-                    const u4 w = *reinterpret_cast<const NMI_AS3 u4*>(at + (((16 * i + c) ^ (row & 7)) * 16));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { r.v[4 * kt + j][i][e] = w[e]; }
-                } else {
-                    r.v[4 * kt + j][i][0] = *reinterpret_cast<const NMI_AS3 uint32_t*>(at + (((4 * i + (c >> 2)) ^ (row & 7)) * 16) + 4 * (c & 3));
-                }
-            }
-        }
-    }
-}
+constexpr int kListMost = 2048;               // blocks of a workgroup's list
+constexpr int kGroupMost = 64;                // tokens of a workgroup: bits
+constexpr int kManyBlock = 256;               // rows of a block, at most: bounds the tiles of a list
+constexpr int kManyTiles = kListMost * (kManyBlock / 32) / 2;
+constexpr int kTableBlocks = 16384;           // blocks of a pass over the lists
 
 // Tokens token .. token + count - 1 of sequence b, the first at position pos, and a KV head.
 struct Group {
@@ -375,327 +323,380 @@ __device__ __forceinline__ Group group_of(const SparseArgs& y, int64_t id, int l
     return q;
 }
 
-// The group's blocks, each with the tokens that take it, in `list`; how many. `table`: scratch of `most` words.
-__device__ __forceinline__ int merge_lists(const SparseArgs& y, const Group& q, uint32_t* list, uint32_t* table, int most, int lane) {
+// The merged list in LDS.
+struct List {
+    uint64_t tokens[kListMost];
+    int32_t block[kListMost];
+    int count;
+};
+
+// For the whole workgroup; `table`: scratch of kTableBlocks words.
+__device__ __forceinline__ void merge_lists(const SparseArgs& y, const Group& q, List& list, uint64_t* table) {
     const int32_t* from = y.selected + (static_cast<int64_t>(q.token) * y.x.c.Hkv + q.h) * y.count;
     const int64_t next = static_cast<int64_t>(y.x.c.Hkv) * y.count;
     const int entries = q.count * y.count;
     const int blocks = ((q.pos + q.count - 1) >> y.block_shift) + 1;
-    bool twice = false;
-    int n = 0;
-    for (int b0 = 0; b0 < blocks; b0 += most) {
-        const int some = min(most, blocks - b0);
-        for (int i = lane; i < some; i += 64) { table[i] = 0u; }
-        wave_sync();
-        for (int e = lane; e < entries; e += 64) {
+    const int lane = threadIdx.x & 63;
+    int n = 0; // of the first wave
+    for (int b0 = 0; b0 < blocks; b0 += kTableBlocks) {
+        const int some = min(kTableBlocks, blocks - b0);
+        for (int i = threadIdx.x; i < some; i += kManyThreads) { table[i] = 0u; }
+        __syncthreads();
+        for (int e = threadIdx.x; e < entries; e += kManyThreads) {
             const int t = e / y.count;
             const int blk = from[t * next + (e - t * y.count)];
-            if (blk >= b0 && blk < b0 + some && blk <= ((q.pos + t) >> y.block_shift)) { twice |= ((atomicOr(&table[blk - b0], 1u << t) >> t) & 1u) != 0u; }
-        }
-        wave_sync();
-        for (int i0 = 0; i0 < some; i0 += 64) {
-            const uint32_t m = i0 + lane < some ? table[i0 + lane] : 0u;
-            const uint64_t all = __ballot(m != 0u);
-            if (m != 0u) { list[n + __popcll(all & ((uint64_t{1} << lane) - 1))] = static_cast<uint32_t>(b0 + i0 + lane) | (m << kBlockBits); }
-            n += __popcll(all);
-        }
-        wave_sync();
-    }
-    if (__any(twice)) {
-        n = entries;
-        for (int e = lane; e < entries; e += 64) {
-            const int t = e / y.count;
-            const int blk = from[t * next + (e - t * y.count)];
-            list[e] = blk >= 0 && blk <= ((q.pos + t) >> y.block_shift) ? static_cast<uint32_t>(blk) | (1u << (kBlockBits + t)) : 0u;
-        }
-        wave_sync();
-    }
-    return n;
-}
-
-// The lane's rows of the group.
-template <int D, bool BF, int NT>
-struct GroupRows {
-    Rows<D, BF, NT> r;
-    int pos[NT];       // the row's position, -1: no row
-    uint32_t bit[NT];  // its token's bit
-    int head[NT];
-    uint32_t tokens;   // all rows' bits
-};
-
-// Row tiles nt0 .. of the group.
-template <int D, bool BF, int NT>
-__device__ __forceinline__ void init_group(const SparseArgs& y, const Group& q, int nt0, int c, int g, GroupRows<D, BF, NT>& z) {
-    const PagedAttnArgs& x = y.x;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int in = c / x.G, before = (nt0 + nt) * y.per_tile, t = before + in;
-        const bool valid = in < y.per_tile && t < q.count;
-        z.head[nt] = c - in * x.G;
-        z.pos[nt] = valid ? q.pos + t : -1;
-        z.bit[nt] = valid ? 1u << t : 0u;
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(x.a.q.data + static_cast<int64_t>(q.token + (valid ? t : 0)) * x.a.q.token_stride) +
-                              (q.h * x.G + (valid ? z.head[nt] : 0)) * D;
-        init_row<D, BF, NT>(x, src, valid, nt, g, z.r);
-    }
-    z.tokens = ((1u << min(q.count, (nt0 + NT) * y.per_tile)) - 1u) & ~((1u << min(q.count, nt0 * y.per_tile)) - 1u);
-    z.r.hi = q.pos + q.count - 1;
-}
-
-// Tiles [j0, j1) of the merged list, for the row tiles nt0 ..
-template <int D, bool BF, int NT, bool CARE>
-__device__ __forceinline__ void group_walk(const SparseArgs& y, const Group& q, const uint32_t* list, int j0, int j1, NMI_AS3 char* st, int nt0, int lane,
-                                           int c, int g, GroupRows<D, BF, NT>& z, float down) {
-    using ST = Stage<D, BF>;
-    const PagedAttnArgs& x = y.x;
-    const int lt = y.block_shift - 5;
-    const int32_t* table = x.c.table + q.b * x.c.table_row;
-    const int last = q.pos + q.count - 1;
-    struct Half {
-        int tile, page;
-        uint32_t mask;
-    };
-    const auto fetch = [&](int j) {
-        const int v = j + (lane >> 1);
-        Half f{0, -1, 0u};
-        if (v < j1) {
-            const uint32_t e = list[v >> lt];
-            f.mask = e >> kBlockBits;
-            f.tile = static_cast<int>((e & ((1u << kBlockBits) - 1u)) << lt) + (v & ((1 << lt) - 1));
-            const int key = 32 * f.tile + 16 * (lane & 1);
-            if (f.mask != 0u && key <= last && (key >> x.c.page_shift) < x.c.max_pages) {
-                const int page = table[key >> x.c.page_shift];
-                f.page = page >= 0 && page < x.c.pages ? page : -1;
+            if (blk >= b0 && blk < b0 + some && blk <= ((q.pos + t) >> y.block_shift)) {
+                atomicOr(reinterpret_cast<unsigned long long*>(&table[blk - b0]), 1ull << t);
             }
         }
-        return f;
-    };
-    Half ids = fetch(j0), next_ids = fetch(j0 + 32);
-    const auto refill = [&](int j) {
-        if (((j - j0) & 63) == 30) { ids = fetch(j + 34); }
-        if (((j - j0) & 63) == 62) { next_ids = fetch(j + 34); }
-    };
-    struct Tile {
-        int tile;
-        Halves hv;
-        uint32_t mask;
-    };
-    const auto tile_at = [&](int j) { // past the end no page
-        const int i = 2 * (j - j0);
-        const bool now = (i & 127) < 64;
-        Tile t;
-        t.tile = __builtin_amdgcn_readlane(now ? ids.tile : next_ids.tile, i & 63);
-        t.mask = __builtin_amdgcn_readlane(now ? ids.mask : next_ids.mask, i & 63);
-        t.hv.page[0] = __builtin_amdgcn_readlane(now ? ids.page : next_ids.page, i & 63);
-        t.hv.page[1] = __builtin_amdgcn_readlane(now ? ids.page : next_ids.page, (i & 63) + 1);
-        return t;
-    };
-    Probs<NT> pr;
-    uint32_t large = 0u; // known already
-    ChunkK<D, BF> ka;
-    ChunkV<D, BF> va;
-    init_group<D, BF, NT>(y, q, nt0, c, g, z);
-    Tile ta = tile_at(j0);
-    stage_keys<D, BF>(x, q.h, ta.tile, ta.hv, st, lane, g, ka);
-    stage_values<D, BF>(x, q.h, ta.tile, ta.hv, st, lane, g, va);
-#pragma unroll 1
-    for (int j = j0; j < j1; ++j) {
-        const bool some = (ta.hv.page[0] & ta.hv.page[1]) >= 0 && (ta.mask & z.tokens) != 0u; // otherwise the tile adds nothing
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) { z.r.pos[nt] = (ta.mask & z.bit[nt]) != 0u ? z.pos[nt] : -1; }
-        z.r.lo = (ta.mask & z.tokens) == z.tokens ? q.pos : -1;
-        const Tile tb = tile_at(j + 1); // before the refill: tile 31 of a fetch is still in it
-        __builtin_amdgcn_s_waitcnt(waitcnt_vm(ST::kOps)); // the keys have landed
-        read_keys<D, BF>(st, c, g, ka);
-        __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-        ChunkK<D, BF> kb;
-        stage_keys<D, BF>(x, q.h, tb.tile, tb.hv, st, lane, g, kb);
-        if (some) { chunk_probs<D, BF, NT>(x, ta.tile, ta.hv, g, ka, z.r, pr); }
-        if constexpr (!BF) { __builtin_memcpy(ka.ks, kb.ks, sizeof(ka.ks)); }
-        __builtin_amdgcn_s_waitcnt(waitcnt_vm(ST::kOps)); // the values have landed
-        read_values<D, BF>(st, c, g, va);
-        __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-        ChunkV<D, BF> vb;
-        stage_values<D, BF>(x, q.h, tb.tile, tb.hv, st, lane, g, vb);
-        if (some) { chunk_values<D, BF, NT, CARE>(ta.tile, ta.hv, g, pr, va, z.r, down, large); }
-        if constexpr (!BF) { __builtin_memcpy(va.vs, vb.vs, sizeof(va.vs)); }
-        if (((j - j0) & 1) == 0) { refill(j); }
-        ta = tb;
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            for (int i0 = 0; i0 < some; i0 += 64) {
+                const uint64_t m = i0 + lane < some ? table[i0 + lane] : 0u;
+                const uint64_t all = __ballot(m != 0u);
+                const int at = n + __popcll(all & ((uint64_t{1} << lane) - 1));
+                if (m != 0u && at < kListMost) { // (as many blocks or entries as the host allows fit)
+                    list.block[at] = b0 + i0 + lane;
+                    list.tokens[at] = m;
+                }
+                n += __popcll(all);
+            }
+        }
+        __syncthreads();
     }
-    __builtin_amdgcn_s_waitcnt(0); // no DMA may land after this point
+    if (threadIdx.x == 0) { list.count = min(n, kListMost); }
+    __syncthreads();
 }
 
-// WAVES: a wave per group; otherwise four waves share one, and `parts` workgroups may.
-template <int D, bool BF, int NT, bool WAVES>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : 1, D == 128 ? 2 : 1))) void sparse_group_kernel(SparseArgs y) {
-    using ST = Stage<D, BF>;
-    static_assert(2 * NT * (D / 16) * 64 * 16 <= 4 * ST::kBytes, "the join exceeds the stages");
-    __shared__ __attribute__((aligned(1024))) char smem[4 * ST::kBytes];
-    __shared__ uint32_t lists[4][kListMost];
-    __shared__ float2 xm[2][NT * 64];
+template <int D, bool BF, int WK>
+__global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void sparse_many_kernel(SparseArgs y) {
+    using MG = ManyGeo<D, WK>;
+    constexpr int NT = MG::NT, NCH = MG::NCH;
+    constexpr int WPC = 32 / MG::RW; // waves that stage a chunk's rows
+    __shared__ __attribute__((aligned(256))) char smem[2 * MG::kBuf];
+    __shared__ List list;
+    __shared__ uint32_t marks[kManyTiles / 32]; // tiles that need care
+    __shared__ uint32_t state[2][8];            // per buffer and wave: bit 0 its page exists, bit 1 care
+    __shared__ float tops[2][8];
+    static_assert(kTableBlocks * 8 <= 2 * MG::kBuf);
     const PagedAttnArgs& x = y.x;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
-    int64_t id;
-    int part = 0;
-    if constexpr (WAVES) {
-        // neighbouring waves: neighbouring groups of one head, whose lists are much alike
-        id = (static_cast<int64_t>(blockIdx.x / x.c.Hkv) * 4 + wave) * x.c.Hkv + blockIdx.x % x.c.Hkv;
-        if (id >= y.items) { return; }
-    } else {
-        id = blockIdx.x % y.items;
-        part = static_cast<int>(blockIdx.x / y.items);
-    }
-    const Group q = group_of(y, id, lane);
+    const int wr = wave / WK, wk = wave % WK;
+    const Group q = group_of(y, blockIdx.x, lane);
     if (q.b < 0) { return; }
-    char* own = smem + wave * ST::kBytes;
-    const int entries = merge_lists(y, q, lists[wave], reinterpret_cast<uint32_t*>(own), ST::kTable, lane);
-    const int tiles = entries << (y.block_shift - 5);
-    int j0 = 0, j1 = tiles;
-    if constexpr (!WAVES) {
-        const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * part / y.parts), t1 = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / y.parts);
-        j0 = t0 + (t1 - t0) * wave / 4;
-        j1 = t0 + (t1 - t0) * (wave + 1) / 4;
-    }
-    NMI_AS3 char* st = (NMI_AS3 char*)own;
-    GroupRows<D, BF, NT> z;
-    group_walk<D, BF, NT, false>(y, q, lists[wave], j0, j1, st, 0, lane, c, g, z, 1.0f);
-    bool lower = false;
-    if constexpr (BF) {
-        uint32_t top = 0u;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int t = 0; t < D / 16; ++t) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { top = max(top, __float_as_uint(z.r.O[nt][t][e]) << 1); }
+    merge_lists(y, q, list, reinterpret_cast<uint64_t*>(smem));
+    const int lt = y.block_shift - 5; // log2(chunks of a block)
+    const int chunks = list.count << lt;
+    const int tiles = (chunks + NCH - 1) / NCH;
+    const int p1 = q.pos + q.count - 1;
+
+    // the first key and the page of the wave's rows, 64 tiles at a time
+    const int32_t* table = x.c.table + q.b * x.c.table_row;
+    struct Place {
+        int key, page;
+    };
+    const auto chunk_key = [&](int v) { return ((list.block[v >> lt] << lt) + (v & ((1 << lt) - 1))) * 32; };
+    const auto places_from = [&](int j) {
+        const int v = (j + lane) * NCH + wave / WPC;
+        Place p{0, -1};
+        if (v < chunks) {
+            p.key = chunk_key(v) + wave % WPC * MG::RW;
+            if (p.key <= p1 && (p.key >> x.c.page_shift) < x.c.max_pages) {
+                const int page = table[p.key >> x.c.page_shift];
+                p.page = page >= 0 && page < x.c.pages ? page : -1;
             }
         }
-        // sums from 2^100 up, infinite ones or NaN: the careful walk
-        if (__builtin_expect(__any(top >= static_cast<uint32_t>(127 + 100) << 24), 0)) {
-            uint32_t large = 0u;
-            const int lt = y.block_shift - 5;
-            const int32_t* table = x.c.table + q.b * x.c.table_row;
+        return p;
+    };
+    Place ids = places_from(0), next_ids = places_from(64);
+    StageRegs<D, BF> sr;
+    int key = 0, page = -1; // of the rows in `sr`
+    const auto fetch = [&](int j) {
+        if ((j & 63) == 0 && j > 0) { // a new 64: they were fetched 64 tiles ago
+            ids = next_ids;
+            next_ids = places_from(j + 64);
+        }
+        key = __builtin_amdgcn_readlane(ids.key, j & 63);
+        page = __builtin_amdgcn_readlane(ids.page, j & 63);
+        stage_load<D, BF>(x, q.h, key, page, lane, sr);
+    };
+    ManyScale sc{1.0f, 1.0f, INFINITY, INFINITY, 0u};
+    const auto trim = [&] {
+        const int live = p1 + 1 - key;
+        if (live < MG::RW) { stage_trim<D, BF>(sr, live, lane); }
+    };
+    const auto put = [&](int j) {
+        trim();
+        const bool care = stage_store<D, BF>(sr, sc, smem + (j & 1) * MG::kBuf, wave * MG::RW, lane);
+        const uint32_t st = (page >= 0 ? 1u : 0u) | (__any(care) ? 2u : 0u);
+        if (lane == 0) { state[j & 1][wave] = st; }
+    };
+
+    if (tiles > 0) { fetch(0); }
+    Rows<D, BF, NT> r;
+    int pos[NT];       // the row's position, -1: no row
+    uint32_t bit[NT];  // its token's bit among the wave's
+    const int first = wr * NT * y.per_tile; // the wave's first token
+    const int mine = max(0, min(NT * y.per_tile, q.count - first));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int in = c / x.G, t = nt * y.per_tile + in;
+        const bool valid = in < y.per_tile && t < mine;
+        pos[nt] = valid ? q.pos + first + t : -1;
+        bit[nt] = valid ? 1u << t : 0u;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(x.a.q.data + static_cast<int64_t>(q.token + (valid ? first + t : 0)) * x.a.q.token_stride) +
+                              (q.h * x.G + (valid ? c - in * x.G : 0)) * D;
+        init_row<D, BF, NT>(x, src, valid, nt, g, r);
+    }
+    const uint32_t every = (1u << mine) - 1u;
+    r.hi = q.pos + first + mine - 1;
+    // the wave's tokens that take chunk v; sets what its rows see of it
+    const auto takes = [&](int v) {
+        const uint64_t all = list.tokens[v >> lt];
+        const uint32_t m = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(all >> first)) & every;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) { r.pos[nt] = (m & bit[nt]) != 0u ? pos[nt] : -1; }
+        r.lo = m == every ? q.pos + first : -1;
+        return m != 0u;
+    };
+    bool cared = false;
+    if (tiles > 0) {
+        for (int i = threadIdx.x; 32 * i < tiles; i += kManyThreads) { marks[i] = 0u; }
+        // the first tile that holds a value tells how large they are: absent pages and zero rows say nothing
+        float kt = 0.0f, vt = 0.0f;
+        int js = 0;
+        for (;; ++js) {
+            if (js > 0) {
+                const Place p = places_from(js);
+                key = __builtin_amdgcn_readfirstlane(p.key);
+                stage_load<D, BF>(x, q.h, key, __builtin_amdgcn_readfirstlane(p.page), lane, sr);
+            }
+            trim();
+            const StageSize z = stage_size<D, BF>(sr);
+            const float kw = wave_max(z.k < INFINITY ? z.k : 0.0f), vw = wave_max(z.v < INFINITY ? z.v : 0.0f);
+            if (lane == 0) {
+                tops[0][wave] = kw;
+                tops[1][wave] = vw;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                kt = fmaxf(kt, tops[0][i]);
+                vt = fmaxf(vt, tops[1][i]);
+            }
+            if (__any(vt > 0.0f) || js + 1 == tiles) { break; }
+            __syncthreads(); // the tops are read
+        }
+        if (js > 0) { fetch(0); }
+        pick(kt, 8, sc.k, sc.klim);
+        pick(vt, BF ? 15 : 8, sc.v, sc.vlim);
+        sc.vleast = __float_as_uint(0x1p-6f / sc.v) - 1u;
+        put(0);
+        if (tiles > 1) { fetch(1); }
+        __syncthreads();
+    }
+    ManyState<D, BF, NT> ms;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        ms.mul[nt] = BF ? r.rowmul[nt] : fminf(r.rowmul[nt] / sc.k, kLargest);
+        ms.ref[nt] = {};
+        ms.lim[nt] = -INFINITY;
+        ms.l[nt] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    // the wave's V^T reads: lane (c, g) addresses key 4 g + (c >> 2), dims 4 (c & 3) .. of a 16-dim segment
+    const int vkey = 4 * g + (c >> 2);
+    const int voff = vkey * 2 * D + 32 * (vkey & 7) + 8 * (c & 3);
+    // waves w and w + 4 share a SIMD: one decodes the next tile before its products, one after them
+    const bool early = wave < 4;
 #pragma unroll 1
-            for (int j = j0; j < j1; ++j) {
-                const uint32_t e = __builtin_amdgcn_readfirstlane(lists[wave][j >> lt]);
-                if ((e >> kBlockBits) == 0u) { continue; }
-                const int tile = static_cast<int>((e & ((1u << kBlockBits) - 1u)) << lt) + (j & ((1 << lt) - 1));
-                ChunkV<D, BF> cv;
-                load_values<D, BF>(x, q.h, tile, halves_of(x, table, tile, q.pos + q.count - 1), c, g, cv);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-#pragma unroll
-                    for (int i = 0; i < Chunk<D, BF>::VP; ++i) {
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) { large = max(large, larger_bits(finite_word(cv.v[k][i][w]))); }
-                    }
-                }
+    for (int j = 0; j < tiles; ++j) {
+        const char* buf = smem + (j & 1) * MG::kBuf;
+        const uint32_t st = lane < 8 ? state[j & 1][lane] : 0u;
+        const uint32_t here = static_cast<uint32_t>(__ballot((st & 1u) != 0u));
+        const bool care = __any((st & 2u) != 0u);
+        const auto stage = [&] {
+            if (j + 1 < tiles) {
+                put(j + 1);
+                if (j + 2 < tiles) { fetch(j + 2); }
             }
-            lower = __any(large >= kCareTop);
-            // a row tile at a time: two and the care do not fit the registers
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                GroupRows<D, BF, 1> one;
-                group_walk<D, BF, 1, true>(y, q, lists[wave], j0, j1, st, nt, lane, c, g, one, lower ? kCareDown : 1.0f);
-                z.r.m[nt] = one.r.m[0];
-                z.r.l[nt] = one.r.l[0];
-#pragma unroll
-                for (int t = 0; t < D / 16; ++t) { z.r.O[nt][t] = one.r.O[0][t]; }
+        };
+        if (early) { stage(); }
+        if (care) {
+            cared = true;
+            if (threadIdx.x == 0) { marks[j >> 5] |= 1u << (j & 31); }
+        } else {
+#pragma unroll 1
+            for (int cw = 0; cw < NCH / WK; ++cw) {
+                const int ci = cw * WK + wk;
+                const int v = j * NCH + ci;
+                // the halves' pages: two waves' rows each at head_dim 256
+                const uint32_t bits = D == 128 ? here >> (2 * ci) : (here >> (4 * ci) & 1u) | (here >> (4 * ci + 1) & 2u);
+                // by arithmetic: hipcc 7.2 inverted a select on a bit of a scalar here (s_bitcmp0 for s_bitcmp1)
+                const Halves hv{{static_cast<int>(bits & 1u) - 1, static_cast<int>((bits >> 1) & 1u) - 1}};
+                if (v >= chunks || (hv.page[0] & hv.page[1]) < 0 || !takes(v)) { continue; }
+                const int c0 = __builtin_amdgcn_readfirstlane(chunk_key(v));
+                if (c0 > r.hi) { continue; }
+                many_chunk<D, BF, NT>(x, buf, ci, c0, hv, c, g, voff, r, ms);
             }
         }
+        if (!early) { stage(); }
+        __syncthreads(); // this buffer is free, the next tile is in place
     }
+    const float unit_v = 1.0f / sc.v; // an exact power of two
     float M[NT], L[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        M[nt] = z.r.m[nt] == -INFINITY ? -INFINITY : z.r.m[nt] * z.r.rowmul[nt];
-        L[nt] = group4_sum(z.r.l[nt]);
-        if (lower) { care_units(M[nt], L[nt]); }
+        float neg;
+        if constexpr (kFromRef<D, BF>) { neg = ms.ref[nt][0]; } else { neg = ms.ref[nt]; }
+        M[nt] = ms.lim[nt] == -INFINITY ? -INFINITY : -neg * ms.mul[nt];
+        L[nt] = ms.l[nt][0];
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) { r.O[nt][t] *= unit_v; }
     }
-    if constexpr (!WAVES) {
-        __syncthreads(); // every wave's stage is done with
-        join_waves<D, BF, NT, 4>(z.r, M, L, wave, lane, *reinterpret_cast<f4(*)[2][NT * (D / 16) * 64]>(smem), xm);
-        if (wave != 0) { return; }
+    if (__builtin_expect(cared, 0)) {
+        // the state so far to LDS (each wave its own part), then the marked tiles with a new one
+        float* keep = reinterpret_cast<float*>(smem) + wave * (16 * NT * D);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) { *reinterpret_cast<f4*>(keep + (16 * nt + c) * D + 16 * t + 4 * g) = r.O[nt][t]; }
+        }
+        __syncthreads();
+        uint32_t large = 0u;
+        bool lower = false;
+#pragma unroll 1
+        for (;;) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) { r.O[nt][t] = f4{0.f, 0.f, 0.f, 0.f}; }
+                r.m[nt] = -INFINITY;
+                r.l[nt] = 0.0f;
+            }
+#pragma unroll 1
+            for (int base = 0; base < tiles; base += 32) {
+                uint32_t bits = __builtin_amdgcn_readfirstlane(marks[base >> 5]);
+#pragma unroll 1
+                for (; bits != 0u; bits &= bits - 1u) {
+                    const int v0 = (base + __builtin_ctz(bits)) * NCH;
+#pragma unroll 1
+                    for (int cw = 0; cw < NCH / WK; ++cw) {
+                        const int v = v0 + cw * WK + wk;
+                        if (v >= chunks || !takes(v)) { continue; }
+                        const int tile = __builtin_amdgcn_readfirstlane(chunk_key(v)) >> 5;
+                        if (32 * tile > r.hi || ((32 * tile + 16) >> x.c.page_shift) >= x.c.max_pages) { continue; }
+                        const Halves hv = halves_of(x, table, tile, p1);
+                        Probs<NT> pr;
+                        {
+                            ChunkK<D, BF> ck;
+                            load_keys<D, BF>(x, q.h, tile, hv, c, g, ck);
+                            chunk_probs<D, BF, NT>(x, tile, hv, g, ck, r, pr);
+                        }
+                        __builtin_amdgcn_sched_barrier(0); // the registers hold one plane's rows at a time
+                        ChunkV<D, BF> cv;
+                        load_values<D, BF>(x, q.h, tile, hv, c, g, cv);
+                        chunk_values<D, BF, NT, BF>(tile, hv, g, pr, cv, r, lower ? kCareDown : 1.0f, large);
+                    }
+                }
+            }
+            if (!BF || lower || !__any(large >= kCareTop)) { break; }
+            lower = true; // again, by the lower weights
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float m2 = r.m[nt] == -INFINITY ? -INFINITY : r.m[nt] * r.rowmul[nt], l2 = group4_sum(r.l[nt]);
+            if (lower) { care_units(m2, l2); }
+            const Weights w = weights(M[nt], L[nt], m2, l2);
+            L[nt] = L[nt] * w.a + l2 * w.b;
+            M[nt] = w.M;
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { // back in the first walk's order of dims, so that what follows is the same
+                    float* o = keep + (16 * nt + c) * D + out_dim<BF>(t, 4 * g + e);
+                    *o = (w.a == 0.0f ? 0.0f : *o * w.a) + (w.b == 0.0f ? 0.0f : r.O[nt][t][e] * w.b);
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) { r.O[nt][t] = *reinterpret_cast<const f4*>(keep + (16 * nt + c) * D + 16 * t + 4 * g); }
+        }
+        __syncthreads();
+    }
+    // ---- the WK key waves of a row tile through LDS
+    if constexpr (WK > 1) {
+        f4* xo = reinterpret_cast<f4*>(smem);
+        constexpr int kPer = NT * (D / 16) * 64;
+        static_assert((WK - 1) * MG::WR * kPer * 16 + (WK - 1) * MG::WR * NT * 64 * 8 <= 2 * MG::kBuf, "merge exceeds the buffers");
+        float2* xm = reinterpret_cast<float2*>(smem + (WK - 1) * MG::WR * kPer * 16);
+        if (wk > 0) {
+            const int at = (wk - 1) * MG::WR + wr;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) { xo[at * kPer + (nt * (D / 16) + t) * 64 + lane] = r.O[nt][t]; }
+                xm[(at * NT + nt) * 64 + lane] = float2{M[nt], L[nt]};
+            }
+        }
+        __syncthreads();
+        if (wk > 0) { return; }
+#pragma unroll
+        for (int i = 0; i < WK - 1; ++i) {
+            const int at = i * MG::WR + wr;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float2 o = xm[(at * NT + nt) * 64 + lane];
+                const Weights w = weights(M[nt], L[nt], o.x, o.y);
+                L[nt] = L[nt] * w.a + o.y * w.b;
+                M[nt] = w.M;
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) {
+                    const f4 z = xo[at * kPer + (nt * (D / 16) + t) * 64 + lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { r.O[nt][t][e] = (w.a == 0.0f ? 0.0f : r.O[nt][t][e] * w.a) + (w.b == 0.0f ? 0.0f : z[e] * w.b); }
+                }
+            }
+        }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        if (z.pos[nt] < 0) { continue; }
-        if (!WAVES && y.parts > 1) {
-            store_part<D, BF, NT>(x, z.r, nt, M[nt], L[nt], (id * (16 * NT) + 16 * nt + c) * y.parts + part, g);
-        } else {
-            store_out<D, BF, NT>(x, q.token + z.pos[nt] - q.pos, q.h, z.head[nt], z.r, nt, L[nt], g);
-        }
+        if (pos[nt] < 0) { continue; }
+        uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + static_cast<int64_t>(q.token + pos[nt] - q.pos) * x.a.out.token_stride) +
+                        (q.h * x.G + c % x.G) * D + 4 * g;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) { *reinterpret_cast<u2*>(out + 16 * t) = out_pair(r.O[nt][t], L[nt]); }
     }
-}
-
-// The parts of an item's rows, one after another: D / 4 threads a row, 16 nt rows an item.
-template <int D>
-__global__ __launch_bounds__(256) void sparse_merge_kernel(SparseArgs y, int rows) {
-    const PagedAttnArgs& x = y.x;
-    constexpr int TPR = D / 4, RPB = 256 / TPR;
-    const int lane = threadIdx.x & 63;
-    const int64_t id = blockIdx.x / (rows / RPB);
-    const int row = static_cast<int>(blockIdx.x % (rows / RPB)) * RPB + threadIdx.x / TPR;
-    int64_t token;
-    int head;
-    if (y.tokens > 1) {
-        const Group q = group_of(y, id, lane);
-        const int in = (row & 15) / x.G, t = (row >> 4) * y.per_tile + in;
-        if (q.b < 0 || in >= y.per_tile || t >= q.count) { return; }
-        token = q.token + t;
-        head = q.h * x.G + (row & 15) - in * x.G;
-    } else {
-        const Item it = item_of(y, id, rows, lane);
-        if (it.b < 0 || it.row0 + row >= x.G) { return; }
-        token = it.token;
-        head = it.h * x.G + it.row0 + row;
-    }
-    const int d = 4 * (threadIdx.x % TPR);
-    Merge m;
-#pragma unroll 4
-    for (int k = 0; k < y.parts; ++k) {
-        const int64_t at = (id * rows + row) * y.parts + k;
-        const float2 ml = *reinterpret_cast<const float2*>(x.part_ml + 2 * at);
-        m.add(ml.x, ml.y, *reinterpret_cast<const f4*>(x.part_o + at * D + d));
-    }
-    uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + token * x.a.out.token_stride) + head * D + d;
-    *reinterpret_cast<u2*>(out) = out_pair(m.O, m.L);
 }
 
 // How a call is cut.
 struct SparsePlan {
     int32_t nt = 1;
     int32_t row_tiles = 1;
-    int32_t tokens = 1;   // of a group
-    int32_t per_tile = 1;
     int64_t items = 0;
     bool waves = false; // a wave per item
     int32_t parts = 1;  // workgroups per item
+    int32_t wk = 0;     // groups of tokens, waves of a row tile over the keys (0: none are formed)
+    int32_t tokens = 1; // of a group
+    int32_t per_tile = 1;
     size_t ml_offset = 0;
     size_t bytes = 0;
 };
 
 constexpr int kCus = 256;
 
-SparsePlan plan_sparse(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t B, int32_t max_new, int32_t selected, int32_t block_shift) {
+SparsePlan plan_sparse(int32_t Hq, int32_t Hkv, int32_t D, bool bf16, int64_t tokens, int32_t B, int32_t max_new, int32_t max_keys, int32_t selected,
+                       int32_t block_shift) {
     SparsePlan p;
     const int32_t G = Hq / Hkv;
+    p.nt = G <= 16 ? 1 : 2;
+    p.row_tiles = (G + 16 * p.nt - 1) / (16 * p.nt);
+    p.items = tokens * Hkv * p.row_tiles;
     const int64_t tiles = static_cast<int64_t>(selected) << (block_shift - 5);
-    if (G <= 16) {
-        // one or two row tiles of whole tokens, as many as the lists leave room for
-        p.per_tile = std::min(16 / G, G <= 2 ? 8 : 4);
-        p.tokens = std::min({p.per_tile * (G <= 2 ? 1 : 2), max_new, kListMost / selected});
-    }
-    if (p.tokens > 1) {
-        p.nt = p.tokens > p.per_tile ? 2 : 1;
-        p.items = (tokens + static_cast<int64_t>(B) * (p.tokens - 1)) / p.tokens * Hkv;
-    } else {
-        p.tokens = 1;
-        p.nt = G <= 16 ? 1 : 2;
-        p.row_tiles = (G + 16 * p.nt - 1) / (16 * p.nt);
-        p.items = tokens * Hkv * p.row_tiles;
-    }
     const int64_t slots = kCus * (D == 128 ? 2 : 1); // workgroups of four waves at a time
     p.waves = p.items >= 4 * slots || tiles < 4;
     if (!p.waves) {
@@ -707,6 +708,34 @@ SparsePlan plan_sparse(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32
         p.ml_offset = (rows * D * sizeof(float) + 255) & ~size_t{255};
         p.bytes = p.ml_offset + rows * 2 * sizeof(float);
     }
+    // Groups, where they are estimated to be faster.
+    const int64_t blocks = ((static_cast<int64_t>(max_keys) - 1) >> block_shift) + 1;
+    if (G > 16 || max_new < 2 || (1 << block_shift) > kManyBlock) { return p; }
+    const int32_t nt = D == 128 ? 2 : 1;
+    const int32_t per_tile = std::min(16 / G, 8 / nt);
+    // us: a chunk of 32 keys for one token and KV head, all SIMDs busy; a key tile of the groups
+    const double chunk_us = D == 128 ? (bf16 ? 1.4e-3 : 1.04e-3) : (bf16 ? 3.1e-3 : 2.55e-3);
+    double best = 6.0 + static_cast<double>(p.items * tiles) * chunk_us;
+    for (int32_t wk = 1; wk <= (D == 128 ? 4 : 2); wk *= 2) {
+        const int32_t most = std::min(8 / wk * nt * per_tile, kGroupMost);
+        const int32_t t = std::min(most, max_new);
+        if (std::min<int64_t>(blocks, static_cast<int64_t>(t) * selected) > kListMost) { continue; }
+        const int64_t groups = (tokens + static_cast<int64_t>(B) * (most - 1)) / most * Hkv;
+        // tokens next to each other mostly take the same blocks: 2 of them 1.5 times as many as one, 16 3.2 times
+        const double merged = std::min<double>(static_cast<double>(blocks), selected * std::pow(static_cast<double>(t), 0.42));
+        const double us_tile = D == 128 ? (wk == 1 ? 3.4 : wk == 2 ? 2.4 : 2.0) : (wk == 1 ? 2.2 : 1.6);
+        const double us = static_cast<double>((groups + kCus - 1) / kCus) * (10.0 + merged * (1 << block_shift) / (16384 / D) * us_tile);
+        if (us < best) {
+            best = us;
+            p.wk = wk;
+            p.tokens = most;
+            p.per_tile = per_tile;
+        }
+    }
+    if (p.wk > 0) {
+        p.items = (tokens + static_cast<int64_t>(B) * (p.tokens - 1)) / p.tokens * Hkv;
+        p.parts = 1;
+    }
     return p;
 }
 
@@ -716,21 +745,12 @@ void launch(const SparseArgs& y, const SparsePlan& p, hipStream_t stream) {
     const int64_t grid = p.waves ? (p.items / per + 3) / 4 * per : p.items * p.parts;
     if (grid > 0x7FFFFF) { throw Unsupported("paged sparse attention: more than 2^23 workgroups are not built"); }
     const dim3 blocks(static_cast<uint32_t>(grid));
-    if (p.tokens > 1) {
-        if (p.waves) {
-            hipLaunchKernelGGL((sparse_group_kernel<D, BF, NT, true>), blocks, dim3(256), 0, stream, y);
-        } else {
-            hipLaunchKernelGGL((sparse_group_kernel<D, BF, NT, false>), blocks, dim3(256), 0, stream, y);
-        }
-        check_launch("sparse_group_kernel");
+    if (p.waves) {
+        hipLaunchKernelGGL((sparse_attn_kernel<D, BF, NT, true>), blocks, dim3(256), 0, stream, y);
     } else {
-        if (p.waves) {
-            hipLaunchKernelGGL((sparse_attn_kernel<D, BF, NT, true>), blocks, dim3(256), 0, stream, y);
-        } else {
-            hipLaunchKernelGGL((sparse_attn_kernel<D, BF, NT, false>), blocks, dim3(256), 0, stream, y);
-        }
-        check_launch("sparse_attn_kernel");
+        hipLaunchKernelGGL((sparse_attn_kernel<D, BF, NT, false>), blocks, dim3(256), 0, stream, y);
     }
+    check_launch("sparse_attn_kernel");
     if (p.parts > 1) {
         const uint32_t groups = static_cast<uint32_t>(p.items * (16 * NT / (1024 / D)));
         hipLaunchKernelGGL((sparse_merge_kernel<D>), dim3(groups), dim3(256), 0, stream, y, 16 * NT);
@@ -738,19 +758,29 @@ void launch(const SparseArgs& y, const SparsePlan& p, hipStream_t stream) {
     }
 }
 
+template <int D, bool BF>
+void launch_groups(const SparseArgs& y, const SparsePlan& p, hipStream_t stream) {
+    if (p.items > 0x3FFFFF) { throw Unsupported("paged sparse attention: more than 2^22 workgroups are not built"); }
+    const dim3 blocks(static_cast<uint32_t>(p.items));
+    if (p.wk == 1) {
+        hipLaunchKernelGGL((sparse_many_kernel<D, BF, 1>), blocks, dim3(kManyThreads), 0, stream, y);
+    } else if (p.wk == 2) {
+        hipLaunchKernelGGL((sparse_many_kernel<D, BF, 2>), blocks, dim3(kManyThreads), 0, stream, y);
+    } else if constexpr (D == 128) {
+        hipLaunchKernelGGL((sparse_many_kernel<D, BF, 4>), blocks, dim3(kManyThreads), 0, stream, y);
+    }
+    check_launch("sparse_many_kernel");
+}
+
 } // namespace
 
 size_t sparse_attention_bytes(int32_t Hq, int32_t Hkv, int32_t D, int64_t tokens, int32_t B, int32_t selected, int32_t block_shift) {
-    size_t most = 0; // over every envelope
-    for (int32_t max_new = 1; max_new <= kGroupMost; ++max_new) {
-        most = std::max(most, plan_sparse(Hq, Hkv, D, tokens, B, max_new, selected, block_shift).bytes);
-    }
-    return most;
+    return plan_sparse(Hq, Hkv, D, false, tokens, B, 1, 1, selected, block_shift).bytes; // groups take none
 }
 
 void launch_sparse_attention(const PagedAttention& a, const int32_t* selected, int32_t count, int32_t block_shift, const PagedRef& c,
                              void* workspace, hipStream_t stream) {
-    const SparsePlan p = plan_sparse(a.Hq, c.Hkv, c.D, a.tokens, c.B, a.max_new, count, block_shift);
+    const SparsePlan p = plan_sparse(a.Hq, c.Hkv, c.D, c.bf16, a.tokens, c.B, a.max_new, a.max_keys, count, block_shift);
     SparseArgs y{};
     y.x.a = a;
     y.x.a.window = 0x7FFFFFFF; // every row of a listed block up to the token's own
@@ -770,7 +800,11 @@ void launch_sparse_attention(const PagedAttention& a, const int32_t* selected, i
     const auto pick = [&](auto d, auto bf) {
         constexpr int D = decltype(d)::value;
         constexpr bool BF = decltype(bf)::value;
-        p.nt == 1 ? launch<D, BF, 1>(y, p, stream) : launch<D, BF, 2>(y, p, stream);
+        if (p.wk > 0) {
+            launch_groups<D, BF>(y, p, stream);
+        } else {
+            p.nt == 1 ? launch<D, BF, 1>(y, p, stream) : launch<D, BF, 2>(y, p, stream);
+        }
     };
     const auto cache = [&](auto d) { c.bf16 ? pick(d, std::true_type{}) : pick(d, std::false_type{}); };
     c.D == 128 ? cache(std::integral_constant<int, 128>{}) : cache(std::integral_constant<int, 256>{});
