@@ -328,8 +328,8 @@ int nmi_paged_qk_norm_rope_append(const nmi_tensor* q, const nmi_tensor* k, cons
 /* ---------------------------------------------------------------- sparse attention over blocks (EXTENSION) */
 
 /* The means of the blocks that hold the new rows (history[b] .. of `tokens` packed tokens; the rows are in the cache already),
- * each over the block's rows up to the sequence's last one: sums in 64 bits, step = max |sum| / 127 over the head, code = rne(sum *
- * (1 / step)), scale = FP32(step / rows). A block with an infinite or NaN key gets codes 0 and an infinite scale. Blocks past
+ * each over the block's rows up to the sequence's last one: sums in 64 bits, step = max |sum| * FP64(1 / 127) over the head,
+ * code = rne(sum * (1 / step)), scale = FP32(step / rows). A block with an infinite or NaN key gets codes 0 and an infinite scale. Blocks past
  * the page table or in absent pages are left out. */
 int nmi_paged_block_update(const nmi_paged_kv_layer_view* cache, const nmi_tensor* starts, const nmi_tensor* history,
                            int32_t tokens, const nmi_paged_block_view* blocks, nmi_stream_t stream);

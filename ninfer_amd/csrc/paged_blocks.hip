@@ -1,7 +1,7 @@
 // Blocks of keys of a paged KV cache on gfx950: a mean for each, and the blocks that a token's queries score highest.
 //
 // Mathematics: a block's rows are summed in 64 bits (sums of stored values, exact unless they span more than 2^53), step = max
-// |sum| / 127, code = rne(sum * (1 / step)), scale = FP32(step / rows): code * scale is the mean with 8 bits. A token's query for a
+// |sum| * FP64(1 / 127), code = rne(sum * (1 / step)), scale = FP32(step / rows): code * scale is the mean with 8 bits. A token's query for a
 // KV head is the sum of its group's heads, made codes the same way; a block's score is scale * <codes, codes>, the product of
 // whole numbers exact on the matrix cores (up to 2^22), so it does not depend on any order, and which blocks are
 // selected is defined to the bit. A token always takes the first blocks and the last ones up to its own; of those
@@ -18,6 +18,8 @@ namespace nmi {
 namespace {
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr double kStep = 1.0 / 127.0; // a product, not a quotient: part of the definition, since it decides ties of codes
 
 // max |x| over the D / 8 lanes of a head in every one of them, infinite where a value is infinite or NaN.
 template <int D>
@@ -108,7 +110,7 @@ __global__ __launch_bounds__(256) void block_update_kernel(UpdateArgs x) {
         for (int e = 0; e < 8; ++e) { sum[e] += __shfl_xor(sum[e], d); }
     }
     const double amax = head_amax<D>(sum);
-    const double step = amax / 127.0;
+    const double step = amax * kStep;
     const i2 code = codes_of(sum, amax, step);
     const int64_t slot = (static_cast<int64_t>(h) << (x.c.page_shift - bs)) + (in_page >> bs);
     if (group == 0) { *reinterpret_cast<i2*>(x.b.codes + page * x.b.code_page + slot * D + 8 * li) = code; }
@@ -199,9 +201,9 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 
 // What the waves that choose for one token share.
 struct Shared {
-    int count[2][16]; // by turns: a wave may be a step ahead
-    uint32_t least[16], most[16];
-    int taken[16], equal[16];
+    int count[2][8]; // by turns: a wave may be a step ahead
+    uint32_t least[8], most[8];
+    int taken[8], equal[8];
 };
 
 // The list of one token from its keys of = [0, count) by WAVES waves, R keys a lane; block `first` + i has key i. Returns how many.
@@ -314,11 +316,12 @@ __device__ __forceinline__ int choose(const uint32_t* of, int count, int want, i
     if (r <= 6) { return choose<6, WAVES>(of, count, want, first, out, lane, wave, sh); }
     if (r <= 8) { return choose<8, WAVES>(of, count, want, first, out, lane, wave, sh); }
     if (r <= 16) { return choose<16, WAVES>(of, count, want, first, out, lane, wave, sh); }
-    return choose<32, WAVES>(of, count, want, first, out, lane, wave, sh);
+    if (WAVES == 1 || r <= 32) { return choose<32, WAVES>(of, count, want, first, out, lane, wave, sh); }
+    return choose<64, WAVES>(of, count, want, first, out, lane, wave, sh);
 }
 
-// NW: 4 for tiles of 16 tokens (a wave chooses for a token, of at most 2,048 keys), 16 for smaller ones (all waves for one: one wave's walk
-// over 2,048 keys takes longer than the barriers).
+// NW: 4 for tiles of 16 tokens (a wave chooses for a token, of at most 2,048 keys), 8 for smaller ones (all waves for one). 32 single
+// tokens over up to 2,001 blocks: 24.3 us; with 16 waves 27.4 (barriers), with one wave choosing 39.7.
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
     constexpr int L = D / 8;
@@ -365,7 +368,7 @@ __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
             }
         }
         const double amax = head_amax<D>(sum);
-        *reinterpret_cast<i2*>(qcode + t * (D + PAD) + 8 * li) = codes_of(sum, amax, amax / 127.0);
+        *reinterpret_cast<i2*>(qcode + t * (D + PAD) + 8 * li) = codes_of(sum, amax, amax * kStep);
     }
     __syncthreads();
 
@@ -456,7 +459,7 @@ void select(const SelectArgs& x, int64_t tiles, hipStream_t stream) {
     if (x.tile_shift == 4) {
         hipLaunchKernelGGL((block_select_kernel<D, 4>), dim3(static_cast<uint32_t>(grid)), dim3(256), lds, stream, x);
     } else {
-        hipLaunchKernelGGL((block_select_kernel<D, 16>), dim3(static_cast<uint32_t>(grid)), dim3(1024), lds, stream, x);
+        hipLaunchKernelGGL((block_select_kernel<D, 8>), dim3(static_cast<uint32_t>(grid)), dim3(512), lds, stream, x);
     }
     check_launch("block_select_kernel");
 }

@@ -713,17 +713,21 @@ SparsePlan plan_sparse(int32_t Hq, int32_t Hkv, int32_t D, bool bf16, int64_t to
     if (G > 16 || max_new < 2 || (1 << block_shift) > kManyBlock) { return p; }
     const int32_t nt = D == 128 ? 2 : 1;
     const int32_t per_tile = std::min(16 / G, 8 / nt);
-    // us: a chunk of 32 keys for one token and KV head, all SIMDs busy; a key tile of the groups
-    const double chunk_us = D == 128 ? (bf16 ? 1.4e-3 : 1.04e-3) : (bf16 ? 3.1e-3 : 2.55e-3);
-    double best = 6.0 + static_cast<double>(p.items * tiles) * chunk_us;
+    // In us on MI355X. A chunk of 32 keys for one token and KV head (2,048 tokens over 16 blocks of 64), a third more where the tokens
+    // do not fill the chip: 100 and 300 tokens at 40/8/128 INT8 reckoned 48 and 120, took 51 and 114; at 24/4/256 BF16 66 and 172, 65 and
+    // 176; 24 verify rounds of 4 tokens over 43 blocks 105, 101.
+    const double chunk_us = (D == 128 ? (bf16 ? 1.4e-3 : 1.04e-3) : (bf16 ? 3.1e-3 : 2.55e-3)) * (p.waves ? 1.0 : 1.35);
+    double best = 12.0 + static_cast<double>(p.items * tiles) * chunk_us;
     for (int32_t wk = 1; wk <= (D == 128 ? 4 : 2); wk *= 2) {
         const int32_t most = std::min(8 / wk * nt * per_tile, kGroupMost);
         const int32_t t = std::min(most, max_new);
         if (std::min<int64_t>(blocks, static_cast<int64_t>(t) * selected) > kListMost) { continue; }
         const int64_t groups = (tokens + static_cast<int64_t>(B) * (most - 1)) / most * Hkv;
-        // tokens next to each other mostly take the same blocks: 2 of them 1.5 times as many as one, 16 3.2 times
+        // Tokens next to each other mostly take the same blocks: reckoned as if 2 of them took 1.34 times as many as one, 16 3.2 times (where
+        // they agree less the tiles are more, up to as many as there are blocks). A round of workgroups with WK = 1, 2, 4 at 40/8/128 INT8
+        // over 16 blocks each: 190, 111 and 76 us; at 24/4/256 BF16 165 and 98.
         const double merged = std::min<double>(static_cast<double>(blocks), selected * std::pow(static_cast<double>(t), 0.42));
-        const double us_tile = D == 128 ? (wk == 1 ? 3.4 : wk == 2 ? 2.4 : 2.0) : (wk == 1 ? 2.2 : 1.6);
+        const double us_tile = D == 128 ? (wk == 1 ? 4.4 : wk == 2 ? 3.35 : 2.95) : (wk == 1 ? 3.05 : 2.35);
         const double us = static_cast<double>((groups + kCus - 1) / kCus) * (10.0 + merged * (1 << block_shift) / (16384 / D) * us_tile);
         if (us < best) {
             best = us;

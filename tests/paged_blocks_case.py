@@ -33,7 +33,7 @@ def mean_codes(total, rows):
     """INT8 codes and FP32 scale of 64-bit sums [..., D] over `rows` rows."""
     with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
         amax = np.where(np.isfinite(total).all(-1), np.abs(total).max(-1), np.inf)
-        step = amax / 127.0
+        step = amax * (1.0 / 127.0)
         tell = (amax > 0) & np.isfinite(amax)
         inv = np.where(tell, 1.0 / step, 0.0)
         codes = np.where(tell[..., None], np.clip(np.rint(np.where(np.isfinite(total), total, 0) * inv[..., None]), -127, 127), 0)

@@ -196,6 +196,17 @@ def test_scores_of_any_size(gpu, tokens):
 
 
 @pytest.mark.parametrize("tokens", [1, 40])
+def test_codes_at_ties(gpu, tokens):
+    """Queries with values at half, quarter and odd 254ths of the largest: which way a code rounds is part of the definition."""
+    def queries(c, codes, scales):
+        r = np.random.default_rng(8)
+        top = np.float32(2.0) ** r.integers(-3, 4, (c.N, c.Hq, 1)).astype(np.float32) * r.integers(1, 255, (c.N, 1, 1)).astype(np.float32)
+        c.q[:] = bf16_bits(np.where(r.random(c.q.shape) < 0.5, top / 2, top * r.choice(np.array([1, 0.25, 0.5, 0.75], np.float32), c.q.shape)))
+        scales[:] = 1.0
+    _select(PagedCase([(tokens, 4000)], Hq=4, Hkv=2, page=32, seed=12), 32, (0, 1, 12), edit=queries)
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
 def test_selection_leaves_absent_pages_out(gpu, tokens):
     _select(PagedCase([(tokens, 900), (1, 500)], Hq=4, Hkv=2, page=32, seed=7, absent={(0, p) for p in range(3, 20)} | {(1, 2)}), 32, (1, 1, 12))
 
