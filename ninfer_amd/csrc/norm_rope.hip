@@ -75,8 +75,23 @@ struct Turn {
 // A workgroup per token (and share of its heads): D / 8 lanes a head, eight dims a lane, so a wave holds HEADS heads. Queries, keys
 // and values are dealt out in runs of HEADS, so that a wave's heads are of one kind and their weights (times sines and cosines, once
 // per token) come from registers without a choice per value.
-template <int D, bool APPEND>
-__global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs x) {
+//
+// Two waves a workgroup: more waves wait for the token's sines and cosines together (8,192 tokens at 24/4/256 with one, two, four and
+// eight waves 65.8, 56.5, 61.9 and 72.2 us).
+constexpr int kWaves = 2;
+constexpr int kThreads = 64 * kWaves;
+
+template <bool STREAM, typename T>
+__device__ __forceinline__ void put(char* to, T v) {
+    if constexpr (STREAM) {
+        __builtin_nontemporal_store(v, reinterpret_cast<T*>(to));
+    } else {
+        *reinterpret_cast<T*>(to) = v;
+    }
+}
+
+template <int D, bool APPEND, bool STREAM>
+__global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs x) {
     constexpr int L = D / 8;      // lanes of a head
     constexpr int HEADS = 64 / L; // heads of a wave
     __shared__ float2 turn[D / 2];
@@ -87,7 +102,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs x) {
     const int li = lane & (L - 1);
     const int q_runs = (a.Hq + HEADS - 1) / HEADS, kv_runs = (a.Hkv + HEADS - 1) / HEADS;
     const int runs = q_runs + kv_runs * (APPEND ? 2 : 1);
-    const int step = 4 * gridDim.y;
+    const int step = kWaves * gridDim.y;
     // run i: its tensor, the lane's head there and whether there is one
     struct Run {
         int kind; // 0 queries, 1 keys, 2 values
@@ -103,7 +118,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs x) {
         const PackedRef& src = r.kind == 0 ? a.q : r.kind == 1 ? a.k : a.v;
         return r.live ? *reinterpret_cast<const i4*>(src.data + n * src.token_stride + (r.head * D + 8 * li) * 2) : i4{0, 0, 0, 0};
     };
-    int at = blockIdx.y * 4 + wave;
+    int at = blockIdx.y * kWaves + wave;
     Run run = run_of(at);
     i4 raw = load(run);
 
@@ -112,7 +127,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs x) {
     if constexpr (APPEND) {
         // the last sequence that starts at or before the token
         int count = 0;
-        for (int i = threadIdx.x; i - static_cast<int>(threadIdx.x) < x.c.B; i += 256) { count += __syncthreads_count(i < x.c.B && a.starts[i] <= n); }
+        for (int i = threadIdx.x; i - static_cast<int>(threadIdx.x) < x.c.B; i += kThreads) { count += __syncthreads_count(i < x.c.B && a.starts[i] <= n); }
         if (count == 0) { return; }
         const int b = count - 1;
         const int32_t start = a.starts[b], end = a.starts[b + 1], history = a.history[b];
@@ -126,7 +141,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs x) {
     } else {
         pos = a.positions[n];
     }
-    for (int i = threadIdx.x; i < a.half; i += 256) {
+    for (int i = threadIdx.x; i < a.half; i += kThreads) {
         double t = static_cast<double>(pos) * (static_cast<double>(a.inv_freq[i]) * 0.15915494309189533577);
         t -= rint(t);
         float s, c;
@@ -217,20 +232,20 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs x) {
             }
         }
         if (run.kind == 0) {
-            if (run.live) { *reinterpret_cast<i4*>(a.q_out.data + n * a.q_out.token_stride + (run.head * D + 8 * li) * 2) = out; }
+            if (run.live) { put<STREAM>(a.q_out.data + n * a.q_out.token_stride + (run.head * D + 8 * li) * 2, out); }
         } else if constexpr (!APPEND) {
-            if (run.live) { *reinterpret_cast<i4*>(a.k_out.data + n * a.k_out.token_stride + (run.head * D + 8 * li) * 2) = out; }
+            if (run.live) { put<STREAM>(a.k_out.data + n * a.k_out.token_stride + (run.head * D + 8 * li) * 2, out); }
         } else if (page >= 0) {
             const bool value = run.kind == 2;
             const int64_t to = (static_cast<int64_t>(run.head) << x.c.page_shift) + row;
             char* dst = value ? x.c.v + page * x.c.v_page : x.c.k + page * x.c.k_page;
             if (x.c.bf16) {
-                if (run.live) { *reinterpret_cast<i4*>(dst + (to * D + 8 * li) * 2) = out; }
+                if (run.live) { put<STREAM>(dst + (to * D + 8 * li) * 2, out); }
             } else {
                 uint16_t scale;
                 const i2 code = quantize_g64(out, scale);
                 if (run.live) {
-                    *reinterpret_cast<i2*>(dst + to * D + 8 * li) = code;
+                    put<STREAM>(dst + to * D + 8 * li, code);
                     if ((li & 7) == 0) {
                         char* sdst = value ? x.c.vs + page * x.c.vs_page : x.c.ks + page * x.c.ks_page;
                         *reinterpret_cast<uint16_t*>(sdst + (to * (D / 64) + (li >> 3)) * 2) = scale;
@@ -243,13 +258,22 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs x) {
     }
 }
 
+// Outputs of more than 64 MiB are written past the caches: together with a kernel that reads the queries right after, 8,192 tokens at
+// 24/4/256 (112 MiB) take 91.7 us so and 99.7 us through the caches, 4,096 (56 MiB) 51.6 and 47.9, 1,024 (14 MiB) 16.8 and 16.1.
+constexpr int64_t kCached = 64 << 20;
+
 template <int D, bool APPEND>
 void launch(const NormRopeArgs& x, hipStream_t stream) {
     constexpr int HEADS = 512 / D;
     const int runs = (x.a.Hq + HEADS - 1) / HEADS + (x.a.Hkv + HEADS - 1) / HEADS * (APPEND ? 2 : 1);
     // one token's heads over several workgroups where the tokens alone leave CUs idle
-    const int shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((runs + 3) / 4, 1024 / x.a.tokens)));
-    hipLaunchKernelGGL((norm_rope_kernel<D, APPEND>), dim3(static_cast<uint32_t>(x.a.tokens), shares), dim3(256), 0, stream, x);
+    const int shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((runs + kWaves - 1) / kWaves, 1024 / x.a.tokens)));
+    const dim3 grid(static_cast<uint32_t>(x.a.tokens), shares);
+    if (x.a.tokens * (x.a.Hq + (APPEND ? 2 : 1) * x.a.Hkv) * D * 2 > kCached) {
+        hipLaunchKernelGGL((norm_rope_kernel<D, APPEND, true>), grid, dim3(kThreads), 0, stream, x);
+    } else {
+        hipLaunchKernelGGL((norm_rope_kernel<D, APPEND, false>), grid, dim3(kThreads), 0, stream, x);
+    }
     check_launch("norm_rope_kernel");
 }
 

@@ -103,7 +103,7 @@ def test_size_of_the_values(gpu, value, eps):
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
 def test_infinite_and_nan_values_stay_in_their_head(gpu, value):
     def edit(c):
-        c.q[1, 2, 40] = bf16_bits(np.float32(value))
+        c.q[1, 2, 40] = bf16_bits(np.full(1, value, np.float32))[0]
     c, d = RopeCase(2, 5, 2, 128, 32, [5, 6], edit=edit, seed=3), RopeCase(2, 5, 2, 128, 32, [5, 6], seed=3)
     c.call()
     d.call()
@@ -184,6 +184,42 @@ def test_append_of_a_large_batch(gpu):
     two.k = r.outs[1]
     two.append()
     q_out = Strided(na.BF16, (128, 2, c.N), 64)
+    qw, kw, _, freq, norm = r.args()
+    ops.paged_qk_norm_rope_append(r.d_q.t, r.d_k.t, one.v.t, qw, kw, one.starts.tensor(), one.history.tensor(), freq, norm, one.view, q_out.t)
+    synchronize()
+    for a, b in zip(one.pool(), two.pool()):
+        assert (a == b).all()
+    assert (q_out.numpy(np.uint16) == r.outs[0].numpy(np.uint16)).all()
+
+
+def test_large_outputs_are_the_small_ones(gpu):
+    """More than 64 MiB of heads in one call: the same bits as two calls with half the tokens each."""
+    c = RopeCase(1900, 64, 8, 256, 32, np.arange(1900) + 5, seed=10)
+    c.call()
+    synchronize()
+    whole = [o.numpy(np.uint16).reshape(1900, -1).copy() for o in c.outs]
+    for lo, hi in ((0, 950), (950, 1900)):
+        h = RopeCase(1900, 64, 8, 256, 32, np.arange(1900) + 5, seed=10)
+        qw, kw, _, freq, norm = h.args()
+        h.d_q, h.d_k = (Strided(na.BF16, (256, x.shape[1], hi - lo), 64).upload(x[lo:hi]) for x in (c.q, c.k))
+        h.d_pos = DeviceArray.from_numpy(na.I32, c.positions[lo:hi])
+        h.outs = [Strided(na.BF16, (256, n, hi - lo), 64) for n in (64, 8)]
+        h.call()
+        synchronize()
+        for o, w in zip(h.outs, whole):
+            assert (o.numpy(np.uint16).reshape(hi - lo, -1) == w[lo:hi]).all()
+
+
+@pytest.mark.parametrize("kv", ["i8", "bf16"])
+def test_large_append_is_the_two_calls(gpu, kv):
+    seqs = [(1001, 30), (800, 0), (1, 99)]
+    c = PagedCase(seqs, Hq=64, Hkv=8, D=256, kv=kv, page=64, seed=11, absent={(1, 2)})
+    r = RopeCase(c.N, 64, 8, 256, 128, np.concatenate([np.arange(h, h + t) for t, h in seqs]), interleaved=True, seed=12)
+    one, two = c.upload(c.planes(new_rows=False)), c.upload(c.planes(new_rows=False))
+    r.call()
+    two.k = r.outs[1]
+    two.append()
+    q_out = Strided(na.BF16, (256, 64, c.N), 64)
     qw, kw, _, freq, norm = r.args()
     ops.paged_qk_norm_rope_append(r.d_q.t, r.d_k.t, one.v.t, qw, kw, one.starts.tensor(), one.history.tensor(), freq, norm, one.view, q_out.t)
     synchronize()
