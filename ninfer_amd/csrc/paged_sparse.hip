@@ -43,45 +43,71 @@ struct Item {
 };
 
 // KV heads next to each other: workgroups go round the XCDs in turn, so with eight heads each L2 serves one.
-__device__ __forceinline__ Item item_of(const SparseArgs& y, int64_t id, int rows, int lane) {
-    const PagedAttnArgs& x = y.x;
-    Item it{0, static_cast<int32_t>(id % x.c.Hkv), 0, -1, 0};
-    const int64_t rest = id / x.c.Hkv;
+__device__ __forceinline__ Item item_of(const SparseArgs& y, int64_t id, int rows) {
+    Item it{0, static_cast<int32_t>(id % y.x.c.Hkv), 0, -1, 0};
+    const int64_t rest = id / y.x.c.Hkv;
     it.row0 = static_cast<int32_t>(rest % y.row_tiles) * rows;
     it.token = static_cast<int32_t>(rest / y.row_tiles);
-    int before = 0; // sequences that start at or before the token
-    for (int base = 0; base < x.c.B; base += 64) {
-        const bool in = base + lane < x.c.B && x.a.starts[base + lane] <= it.token;
-        before += __popcll(__ballot(in));
-    }
-    if (before == 0) { return it; }
-    const Seq s = sequence(x, before - 1);
-    if (it.token - s.start < s.tokens) {
-        it.b = before - 1;
-        it.pos = s.history + it.token - s.start;
-    }
     return it;
 }
 
-// Which entries of the item's list repeat an earlier one: bit i of lane l for entry 64 i + l. An ascending list has none; in any
-// other every entry is compared with those before it.
-static_assert(kPagedMaxSelected <= 64 * 32);
-__device__ __forceinline__ uint32_t repeats(const int32_t* list, int count, int lane) {
-    bool ascends = true;
-    for (int i = lane; i < count; i += 64) {
-        const int e = list[i], before = i > 0 ? list[i - 1] : 0;
-        ascends &= e < 0 || i == 0 || (before >= 0 && before < e);
+// Lane l: sequence base + l, loaded and not looked at yet.
+struct Loaded {
+    int32_t start;
+    int32_t end;
+    int32_t history;
+};
+
+__device__ __forceinline__ Loaded load_sequences(const PagedAttnArgs& x, int base, int lane) {
+    Loaded l{0x7fffffff, 0, 0};
+    if (base + lane < x.c.B) { l = Loaded{x.a.starts[base + lane], x.a.starts[base + lane + 1], x.a.history[base + lane]}; }
+    return l;
+}
+
+// The item's sequence, the last that starts at or before its token, and position; `l` holds the first 64 sequences. Every lane of
+// the wave is there.
+__device__ __forceinline__ void place(const PagedAttnArgs& x, Loaded l, Item& it, int lane) {
+    for (int base = 0; base < x.c.B; base += 64) {
+        if (base > 0) { l = load_sequences(x, base, lane); }
+        const int before = __popcll(__ballot(base + lane < x.c.B && l.start <= it.token));
+        if (before == 0) { continue; }
+        const Seq s = lane_seq(checked(x, l.start, l.end, l.history), before - 1);
+        const bool has = s.start <= it.token && it.token - s.start < s.tokens;
+        it.b = has ? base + before - 1 : -1;
+        it.pos = has ? s.history + it.token - s.start : 0;
     }
-    uint32_t bits = 0u;
+}
+
+// An item's list: lane l of the wave that walks it holds entry l, and in bit i whether entry 64 i + l repeats an earlier one.
+struct Listed {
+    const int32_t* at;
+    int32_t entry;
+    uint32_t again;
+};
+
+__device__ __forceinline__ Listed list_of(const SparseArgs& y, const Item& it, int lane) {
+    Listed l{y.selected + (static_cast<int64_t>(it.token) * y.x.c.Hkv + it.h) * y.count, -1, 0u};
+    if (lane < y.count) { l.entry = l.at[lane]; }
+    return l;
+}
+
+// Which entries repeat an earlier one. An ascending list has none; in any other every entry is compared with those before it.
+static_assert(kPagedMaxSelected <= 64 * 32);
+__device__ __forceinline__ void find_repeats(Listed& l, int count, int lane) {
+    const int first = __shfl_up(l.entry, 1);
+    bool ascends = lane == 0 || l.entry < 0 || (first >= 0 && first < l.entry); // no entry in the lane: -1
+    for (int i = 64 + lane; i < count; i += 64) {
+        const int e = l.at[i], before = l.at[i - 1];
+        ascends &= e < 0 || (before >= 0 && before < e);
+    }
     if (__builtin_expect(!__all(ascends), 0)) {
         for (int i = lane; i < count; i += 64) {
-            const int e = list[i];
+            const int e = l.at[i];
             bool again = false;
-            for (int j = 0; j < i && !again; ++j) { again = list[j] == e; }
-            bits |= again ? 1u << (i >> 6) : 0u;
+            for (int j = 0; j < i && !again; ++j) { again = l.at[j] == e; }
+            l.again |= again ? 1u << (i >> 6) : 0u;
         }
     }
-    return bits;
 }
 
 // A half tile of the walk: its first key's tile of 32, and its page.
@@ -92,21 +118,20 @@ struct Half {
 
 // Tiles [j0, j1) of the item's list, 32 keys each.
 template <int D, bool BF, int NT, bool CARE>
-__device__ __forceinline__ void sparse_walk(const SparseArgs& y, const Item& it, int j0, int j1, int c, int g, Rows<D, BF, NT>& r, float down) {
+__device__ __forceinline__ void sparse_walk(const SparseArgs& y, const Item& it, const Listed& l, int j0, int j1, int c, int g, Rows<D, BF, NT>& r, float down) {
     const PagedAttnArgs& x = y.x;
     const int lane = threadIdx.x & 63;
     const int lt = y.block_shift - 5; // log2(tiles of a block)
-    const int32_t* list = y.selected + (static_cast<int64_t>(it.token) * x.c.Hkv + it.h) * y.count;
     const int32_t* table = x.c.table + it.b * x.c.table_row;
-    const uint32_t again = repeats(list, y.count, lane);
     // 64 halves (32 tiles) at a time, one per lane, the next 64 fetched ahead
     const auto fetch = [&](int j) {
         const int v = j + (lane >> 1);
         const int entry = v >> lt;
-        const uint32_t twice = static_cast<uint32_t>(__shfl(static_cast<int>(again), entry & 63)) >> ((entry >> 6) & 31);
+        const uint32_t twice = static_cast<uint32_t>(__shfl(static_cast<int>(l.again), entry & 63)) >> ((entry >> 6) & 31);
+        const int early = __shfl(l.entry, entry & 63);
         Half f{0, -1};
         if (v < j1) {
-            const int blk = list[entry];
+            const int blk = entry < 64 ? early : l.at[entry];
             if (blk >= 0 && blk <= (it.pos >> y.block_shift) && (twice & 1u) == 0u) {
                 f.tile = (blk << lt) + (v & ((1 << lt) - 1));
                 const int key = 32 * f.tile + 16 * (lane & 1);
@@ -163,10 +188,10 @@ __device__ __forceinline__ void sparse_walk(const SparseArgs& y, const Item& it,
 // The walk, and for BF16 caches the careful one after it where a sum passed 2^100 or is not finite. M, L: the rows' log2-domain
 // maxima and sums.
 template <int D, bool BF, int NT>
-__device__ __forceinline__ void walk_rows(const SparseArgs& y, const Item& it, int j0, int j1, int c, int g, Rows<D, BF, NT>& r, float (&M)[NT],
+__device__ __forceinline__ void walk_rows(const SparseArgs& y, const Item& it, const Listed& l, int j0, int j1, int c, int g, Rows<D, BF, NT>& r, float (&M)[NT],
                                           float (&L)[NT]) {
     const PagedAttnArgs& x = y.x;
-    sparse_walk<D, BF, NT, false>(y, it, j0, j1, c, g, r, 1.0f);
+    sparse_walk<D, BF, NT, false>(y, it, l, j0, j1, c, g, r, 1.0f);
     bool lower = false;
     if constexpr (BF) {
         uint32_t top = 0u;
@@ -181,11 +206,10 @@ __device__ __forceinline__ void walk_rows(const SparseArgs& y, const Item& it, i
         if (__builtin_expect(__any(top >= static_cast<uint32_t>(127 + 100) << 24), 0)) {
             uint32_t large = 0u;
             const int lt = y.block_shift - 5;
-            const int32_t* list = y.selected + (static_cast<int64_t>(it.token) * x.c.Hkv + it.h) * y.count;
             const int32_t* table = x.c.table + it.b * x.c.table_row;
 #pragma unroll 1
             for (int j = j0; j < j1; ++j) {
-                const int blk = __builtin_amdgcn_readfirstlane(list[j >> lt]);
+                const int blk = __builtin_amdgcn_readfirstlane(l.at[j >> lt]);
                 if (blk < 0 || blk > (it.pos >> y.block_shift)) { continue; }
                 const int tile = (blk << lt) + (j & ((1 << lt) - 1));
                 ChunkV<D, BF> cv;
@@ -200,7 +224,7 @@ __device__ __forceinline__ void walk_rows(const SparseArgs& y, const Item& it, i
                 }
             }
             lower = __any(large >= kCareTop);
-            sparse_walk<D, BF, NT, true>(y, it, j0, j1, c, g, r, lower ? kCareDown : 1.0f);
+            sparse_walk<D, BF, NT, true>(y, it, l, j0, j1, c, g, r, lower ? kCareDown : 1.0f);
         }
     }
 #pragma unroll
@@ -226,9 +250,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 
         const int64_t group = blockIdx.x / x.c.Hkv, per = x.c.Hkv;
         const int64_t id = (group * 4 + wave) * per + blockIdx.x % x.c.Hkv;
         if (id >= y.items) { return; }
-        const Item it = item_of(y, id, 16 * NT, lane);
+        Item it = item_of(y, id, 16 * NT);
+        const Loaded first = load_sequences(x, 0, lane);
+        Listed l = list_of(y, it, lane);
+        place(x, first, it, lane);
         if (it.b < 0) { return; }
-        walk_rows<D, BF, NT>(y, it, 0, tiles, c, g, r, M, L);
+        find_repeats(l, y.count, lane);
+        walk_rows<D, BF, NT>(y, it, l, 0, tiles, c, g, r, M, L);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int row = it.row0 + 16 * nt + c;
@@ -239,11 +267,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 
         __shared__ float2 xm[2][NT * 64];
         const int64_t id = blockIdx.x % y.items;
         const int part = static_cast<int>(blockIdx.x / y.items);
-        const Item it = item_of(y, id, 16 * NT, lane);
+        Item it = item_of(y, id, 16 * NT);
+        const Loaded first = load_sequences(x, 0, lane);
+        Listed l = list_of(y, it, lane);
+        place(x, first, it, lane);
         if (it.b < 0) { return; }
+        find_repeats(l, y.count, lane);
         const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * part / y.parts), t1 = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / y.parts);
         const int j0 = t0 + (t1 - t0) * wave / 4, j1 = t0 + (t1 - t0) * (wave + 1) / 4;
-        walk_rows<D, BF, NT>(y, it, j0, j1, c, g, r, M, L);
+        walk_rows<D, BF, NT>(y, it, l, j0, j1, c, g, r, M, L);
         join_waves<D, BF, NT, 4>(r, M, L, wave, lane, xo, xm);
         if (wave != 0) { return; }
 #pragma unroll
@@ -266,16 +298,19 @@ __global__ __launch_bounds__(256) void sparse_merge_kernel(SparseArgs y, int row
     constexpr int TPR = D / 4, RPB = 256 / TPR;
     const int64_t id = blockIdx.x / (rows / RPB);
     const int row = static_cast<int>(blockIdx.x % (rows / RPB)) * RPB + threadIdx.x / TPR;
-    const Item it = item_of(y, id, rows, threadIdx.x & 63);
-    if (it.b < 0 || it.row0 + row >= x.G) { return; }
+    Item it = item_of(y, id, rows);
+    const Loaded first = load_sequences(x, 0, threadIdx.x & 63); // looked at behind the parts' loads
+    const bool there = it.row0 + row < x.G;
     const int d = 4 * (threadIdx.x % TPR);
     Merge m;
 #pragma unroll 4
-    for (int k = 0; k < y.parts; ++k) {
+    for (int k = 0; k < (there ? y.parts : 0); ++k) {
         const int64_t at = (id * rows + row) * y.parts + k;
         const float2 ml = *reinterpret_cast<const float2*>(x.part_ml + 2 * at);
         m.add(ml.x, ml.y, *reinterpret_cast<const f4*>(x.part_o + at * D + d));
     }
+    place(x, first, it, threadIdx.x & 63);
+    if (it.b < 0 || !there) { return; }
     uint16_t* out = reinterpret_cast<uint16_t*>(x.a.out.data + it.token * x.a.out.token_stride) + (it.h * x.G + it.row0 + row) * D + d;
     *reinterpret_cast<u2*>(out) = out_pair(m.O, m.L);
 }

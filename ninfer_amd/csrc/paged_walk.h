@@ -38,14 +38,13 @@ struct Seq {
     int32_t history;
 };
 
-__device__ __forceinline__ Seq sequence(const PagedAttnArgs& x, int b) {
-    Seq s{x.a.starts[b], 0, x.a.history[b]};
-    const int32_t end = x.a.starts[b + 1];
-    const bool ok = s.start >= 0 && end >= s.start && end <= x.a.tokens && end - s.start <= x.a.max_new && s.history >= 0 &&
-                    static_cast<int64_t>(s.history) + (end - s.start) <= x.a.max_keys;
-    s.tokens = ok ? end - s.start : 0;
-    return s;
+__device__ __forceinline__ Seq checked(const PagedAttnArgs& x, int32_t start, int32_t end, int32_t history) {
+    const bool ok = start >= 0 && end >= start && end <= x.a.tokens && end - start <= x.a.max_new && history >= 0 &&
+                    static_cast<int64_t>(history) + (end - start) <= x.a.max_keys;
+    return Seq{start, ok ? end - start : 0, history};
 }
+
+__device__ __forceinline__ Seq sequence(const PagedAttnArgs& x, int b) { return checked(x, x.a.starts[b], x.a.starts[b + 1], x.a.history[b]); }
 
 // Lane `at`'s sequence, for the whole wave.
 __device__ __forceinline__ Seq lane_seq(const Seq& s, int at) {
