@@ -346,6 +346,54 @@ __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
     // candidates of the tile's last token: blocks first .. last
     const int last = ((pos0 + tokens - 1) >> bs) - local;
 
+    // ---- the first blocks' codes, on their way while the query's are made
+    const int c = lane & 15, g = lane >> 4;
+    const int per = x.c.page_shift - bs; // log2(blocks of a page)
+    const int32_t* table = x.c.table + f.b * x.c.table_row;
+    const int from = first & ~15;
+    constexpr int AHEAD = NW == 4 ? 2 : 4; // sets of 16 blocks on their way
+    constexpr int STEP = 16 * NW * AHEAD;
+    struct Pages {
+        int32_t page[AHEAD];
+    };
+    struct Codes {
+        int32_t page[AHEAD];
+        i4 k[AHEAD][D / 64];
+        float scale[AHEAD];
+    };
+    const auto load_pages = [&](int b0, Pages& p) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int blk = b0 + 16 * NW * u + c;
+            p.page[u] = -1;
+            if (blk >= first && blk <= last && (blk >> per) < x.c.max_pages) { p.page[u] = table[blk >> per]; }
+        }
+    };
+    const auto load_codes = [&](int b0, const Pages& p, Codes& y) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int blk = b0 + 16 * NW * u + c;
+            const int32_t page = p.page[u] >= 0 && p.page[u] < x.c.pages ? p.page[u] : -1;
+            const int64_t slot = (static_cast<int64_t>(h) << per) + (blk & ((1 << per) - 1));
+            y.page[u] = page;
+            y.scale[u] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) { y.k[u][i] = i4{0, 0, 0, 0}; }
+            if (page >= 0) {
+                const char* src = x.b.codes + page * x.b.code_page + slot * D + 16 * g;
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) { y.k[u][i] = *reinterpret_cast<const i4*>(src + 64 * i); }
+                y.scale[u] = *reinterpret_cast<const float*>(x.b.scales + page * x.b.scale_page + slot * 4);
+            }
+        }
+    };
+    int b0 = from + 16 * wave;
+    Pages ids;
+    Codes now, then;
+    load_pages(b0, ids);
+    load_codes(b0, ids, now);
+    load_pages(b0 + STEP, ids);
+
     // ---- query codes
     for (int i = threadIdx.x; i < 16 * (D + PAD) / 16; i += 64 * NW) { reinterpret_cast<u4*>(qcode)[i] = u4{0u, 0u, 0u, 0u}; }
     __syncthreads();
@@ -373,58 +421,33 @@ __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
     __syncthreads();
 
     // ---- scores
-    const int c = lane & 15, g = lane >> 4;
-    const int per = x.c.page_shift - bs; // log2(blocks of a page)
-    const int32_t* table = x.c.table + f.b * x.c.table_row;
     i4 q[D / 64];
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) { q[i] = *reinterpret_cast<const i4*>(qcode + c * (D + PAD) + 64 * i + 16 * g); }
-    const int from = first & ~15;
     constexpr bool FULL = NW == 4; // tiles of 16 tokens
     int lasts[4];                  // of tokens 4 g .. 4 g + 3: the last block to choose
     uint32_t* to = keys + 4 * g * x.cap + c - from;
 #pragma unroll
     for (int r = 0; r < 4; ++r) { lasts[r] = ((pos0 + 4 * g + r) >> bs) - local; }
-    constexpr int AHEAD = NW == 4 ? 2 : 4; // sets of 16 blocks on their way
-    for (int b0 = from + 16 * wave; b0 <= last; b0 += 16 * NW * AHEAD) {
-        int32_t page[AHEAD];
-        i4 k[AHEAD][D / 64];
-        float scale[AHEAD];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int blk = b0 + 16 * NW * u + c;
-            page[u] = -1;
-            if (blk >= first && blk <= last && (blk >> per) < x.c.max_pages) { page[u] = table[blk >> per]; }
-        }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int blk = b0 + 16 * NW * u + c;
-            page[u] = page[u] >= 0 && page[u] < x.c.pages ? page[u] : -1;
-            const int64_t slot = (static_cast<int64_t>(h) << per) + (blk & ((1 << per) - 1));
-            scale[u] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < D / 64; ++i) { k[u][i] = i4{0, 0, 0, 0}; }
-            if (page[u] >= 0) {
-                const char* src = x.b.codes + page[u] * x.b.code_page + slot * D + 16 * g;
-#pragma unroll
-                for (int i = 0; i < D / 64; ++i) { k[u][i] = *reinterpret_cast<const i4*>(src + 64 * i); }
-                scale[u] = *reinterpret_cast<const float*>(x.b.scales + page[u] * x.b.scale_page + slot * 4);
-            }
-        }
+#pragma unroll 1
+    for (; b0 <= last; b0 += STEP) {
+        load_codes(b0 + STEP, ids, then);
+        load_pages(b0 + 2 * STEP, ids);
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int blk = b0 + 16 * NW * u + c;
             if (blk - c > last) { continue; }
             i4 acc = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) { acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[i], k[u][i], acc, 0, 0, 0); }
+            for (int i = 0; i < D / 64; ++i) { acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[i], now.k[u][i], acc, 0, 0, 0); }
 #pragma unroll
             for (int r = 0; r < 4; ++r) { // token 4 g + r, block c
-                const float score = scale[u] * static_cast<float>(acc[r]);
-                const uint32_t key = scale[u] == INFINITY ? 0xff800000u : ordered(score);
-                if (FULL || 4 * g + r < tt) { to[r * x.cap + blk - c] = page[u] >= 0 && blk <= lasts[r] ? key : 0u; }
+                const float score = now.scale[u] * static_cast<float>(acc[r]);
+                const uint32_t key = now.scale[u] == INFINITY ? 0xff800000u : ordered(score);
+                if (FULL || 4 * g + r < tt) { to[r * x.cap + blk - c] = now.page[u] >= 0 && blk <= lasts[r] ? key : 0u; }
             }
         }
+        now = then;
     }
     __syncthreads();
 
