@@ -308,20 +308,135 @@ __device__ __forceinline__ int choose(const uint32_t* of, int count, int want, i
 template <int WAVES>
 __device__ __forceinline__ int choose(const uint32_t* of, int count, int want, int first, int32_t* out, int lane, int wave, Shared& sh) {
     const int r = (count + 64 * WAVES - 1) / (64 * WAVES);
-    if (r <= 1) { return choose<1, WAVES>(of, count, want, first, out, lane, wave, sh); }
-    if (r <= 2) { return choose<2, WAVES>(of, count, want, first, out, lane, wave, sh); }
-    if (r <= 3) { return choose<3, WAVES>(of, count, want, first, out, lane, wave, sh); }
-    if (r <= 4) { return choose<4, WAVES>(of, count, want, first, out, lane, wave, sh); }
-    if (r <= 5) { return choose<5, WAVES>(of, count, want, first, out, lane, wave, sh); }
-    if (r <= 6) { return choose<6, WAVES>(of, count, want, first, out, lane, wave, sh); }
-    if (r <= 8) { return choose<8, WAVES>(of, count, want, first, out, lane, wave, sh); }
+    if constexpr (WAVES > 1) { // (a wave alone has more keys)
+        if (r <= 1) { return choose<1, WAVES>(of, count, want, first, out, lane, wave, sh); }
+        if (r <= 2) { return choose<2, WAVES>(of, count, want, first, out, lane, wave, sh); }
+        if (r <= 4) { return choose<4, WAVES>(of, count, want, first, out, lane, wave, sh); }
+        if (r <= 8) { return choose<8, WAVES>(of, count, want, first, out, lane, wave, sh); }
+    }
     if (r <= 16) { return choose<16, WAVES>(of, count, want, first, out, lane, wave, sh); }
     if (WAVES == 1 || r <= 32) { return choose<32, WAVES>(of, count, want, first, out, lane, wave, sh); }
     return choose<64, WAVES>(of, count, want, first, out, lane, wave, sh);
 }
 
-// NW: 4 for tiles of 16 tokens (a wave chooses for a token, of at most 2,048 keys), 8 for smaller ones (all waves for one). 32 single
-// tokens over up to 2,001 blocks: 24.3 us; with 16 waves 27.4 (barriers), with one wave choosing 39.7.
+// ---- four tokens of a wave, one a row of 16 lanes
+
+template <typename F>
+__device__ __forceinline__ uint32_t row_all(uint32_t v, F op) {
+    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xB1, 0xf, 0xf, true)));  // lane ^ 1
+    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4E, 0xf, 0xf, true)));  // lane ^ 2
+    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x141, 0xf, 0xf, true))); // the other four of eight
+    return op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x140, 0xf, 0xf, true)));
+}
+
+__device__ __forceinline__ int row_sum(int v) {
+    return static_cast<int>(row_all(static_cast<uint32_t>(v), [](uint32_t a, uint32_t b) { return a + b; }));
+}
+
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    return row_all(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+
+// As `choose`, for the token of the lane's row of 16, with R keys a lane: every row has its own interval, and the wave goes on until
+// the last one's is closed.
+template <int R>
+__device__ __forceinline__ int choose_rows(const uint32_t* of, int count, int want, int first, int32_t* out, int lane) {
+    const int li = lane & 15;
+    asm("" : "+v"(want)); // in a vector register: as a scalar it is spilled and read back at every use
+    uint32_t k[R];
+    uint32_t most = 0u, least = 0u; // least as its complement
+    int there = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        k[i] = 16 * i + li < count ? of[16 * i + li] : 0u;
+        there += k[i] != 0u ? 1 : 0;
+        most = max(most, k[i]);
+        least = max(least, k[i] != 0u ? ~k[i] : 0u);
+    }
+    there = row_sum(there);
+    uint32_t lo = ~row_max(least), hi = row_max(most), than = 0u;
+    bool open = there > want;
+    float over = static_cast<float>(there - want), under = static_cast<float>(want);
+    int side = 0;
+#pragma unroll 1
+    for (int step = 0; __any(open); ++step) {
+        uint32_t mid = lo + (hi - lo) / 2 + 1;
+        if (step < 12) {
+            const float a = value_of(lo), b = value_of(hi);
+            const float share = fminf(0.984375f, fmaxf(0.015625f, over * __builtin_amdgcn_rcpf(over + under)));
+            const float v = a + (b - a) * share;
+            const uint32_t between = ordered(v); // lo < between < hi where a < v < b (not so for infinite ends)
+            mid = ((v > a) & (v < b)) ? between : mid;
+        }
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) { n += k[i] >= mid ? 1 : 0; }
+        n = row_sum(n);
+        // as in top_keys, without branches; a row whose interval has closed stays as it is
+        const int d = n - want;
+        const float f = static_cast<float>(d);
+        const float fewer_under = under * (side > 0 ? 0.5f : 1.0f), fewer_over = over * (side < 0 ? 0.5f : 1.0f);
+        const uint32_t low = mid - 1u, closed = lo >= hi ? lo : low;
+        const bool met = (d == 0) | (lo >= hi);
+        than = (open & met) ? closed : than;
+        open = open & !met;
+        lo = (open & (d > 0)) ? mid : lo;
+        hi = (open & (d < 0)) ? low : hi;
+        under = d > 0 ? fewer_under : -f;
+        over = d > 0 ? f : fewer_over;
+        side = d > 0 ? 1 : -1;
+    }
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) { above += k[i] > than ? 1 : 0; }
+    int left = there > want ? want - row_sum(above) : 0; // how many of those that equal it
+    int taken = 0;
+    const int row = lane & 48;
+    const uint32_t below = (1u << li) - 1u;
+    const auto of_row = [&](bool v) { return static_cast<uint32_t>(__ballot(v) >> row) & 0xffffu; };
+    if (!__any(left > 0)) { // no choice among equals
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const bool take = k[i] > than;
+            const uint32_t all = of_row(take);
+            if (take) { out[taken + __popc(all & below)] = first + 16 * i + li; }
+            taken += __popc(all);
+        }
+        return min(there, want);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const bool equal = k[i] == than && k[i] != 0u;
+        const uint32_t same = of_row(equal);
+        const bool take = k[i] > than || (equal && static_cast<int>(__popc(same & below)) < left);
+        const uint32_t all = of_row(take);
+        if (take) { out[taken + __popc(all & below)] = first + 16 * i + li; }
+        taken += __popc(all);
+        left = max(0, left - static_cast<int>(__popc(same)));
+    }
+    return min(there, want);
+}
+
+// Up to as many keys as 64 registers a lane hold. A wave per token takes longer: 2,048 tokens at 40/8/128 over 60, 250, 500, 750 and 1,000
+// blocks 17.6, 24.8, 35.4, 66.3 and 75.2 us so, 12.3, 19.7, 29.7, 49.9 and 64.4 us with rows.
+constexpr int kRowKeys = 1024;
+
+__device__ __forceinline__ int choose_rows(const uint32_t* of, int count, int most, int want, int first, int32_t* out, int lane) {
+    const int r = (most + 15) / 16;
+    if (r <= 4) { return choose_rows<4>(of, count, want, first, out, lane); }
+    if (r <= 8) { return choose_rows<8>(of, count, want, first, out, lane); }
+    if (r <= 12) { return choose_rows<12>(of, count, want, first, out, lane); }
+    if (r <= 16) { return choose_rows<16>(of, count, want, first, out, lane); }
+    if (r <= 20) { return choose_rows<20>(of, count, want, first, out, lane); }
+    if (r <= 24) { return choose_rows<24>(of, count, want, first, out, lane); }
+    if (r <= 32) { return choose_rows<32>(of, count, want, first, out, lane); }
+    if (r <= 48) { return choose_rows<48>(of, count, want, first, out, lane); }
+    return choose_rows<64>(of, count, want, first, out, lane);
+}
+
+// NW: 4 for tiles of 16 tokens (a wave chooses for four of them, or for one, of at most 2,048 keys), 8 for smaller ones (all waves for
+// one). 32 single tokens over up to 2,001 blocks: 23.2 us; with 16 waves 27.4 (barriers), with one wave choosing 39.7; 4,096 tokens
+// over up to 320 blocks 37.5 us.
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
     constexpr int L = D / 8;
@@ -454,6 +569,26 @@ __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
     // ---- lists
     const int S = first + local + x.a.top;
     constexpr int TOGETHER = NW == 4 ? 1 : NW; // waves of a token
+    const auto ends = [&](int32_t* out, int own, int heads, int tail, int taken, int at, int lanes) {
+        for (int i = at; i < heads; i += lanes) { out[i] = i; }
+        for (int i = tail + at; i <= own; i += lanes) { out[taken + i - tail] = i; }
+        for (int i = taken + own - tail + 1 + at; i < S; i += lanes) { out[i] = -1; }
+    };
+    if constexpr (NW == 4) {
+        const int most = last - first + 1;
+        if (most <= kRowKeys) {
+            const int t = 4 * wave + (lane >> 4);
+            const bool there = t < tokens;
+            const int own = there ? (pos0 + t) >> bs : -1; // no block, no candidate
+            int32_t* out = x.a.selected + (static_cast<int64_t>(f.s.start + t0 + (there ? t : 0)) * x.c.Hkv + h) * S;
+            const int heads = min(first, own + 1);
+            const int tail = max(heads, own - local + 1);
+            const int count = there && x.a.top > 0 ? max(0, own - local - first + 1) : 0;
+            const int taken = heads + choose_rows(keys + t * x.cap + (first - from), count, most, x.a.top, first, out + heads, lane);
+            if (there) { ends(out, own, heads, tail, taken, lane & 15, 16); }
+            return;
+        }
+    }
     for (int t = NW == 4 ? wave : 0; t < tokens; t += NW / TOGETHER) {
         const int own = (pos0 + t) >> bs;
         const int64_t token = f.s.start + t0 + t;
@@ -466,11 +601,7 @@ __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
         if (x.a.top > 0 && count > 0) {
             taken += choose<TOGETHER>(keys + t * x.cap + (first - from), count, x.a.top, first, out + heads, lane, part, sh);
         }
-        if (part == 0) {
-            for (int i = lane; i < heads; i += 64) { out[i] = i; }
-            for (int i = tail + lane; i <= own; i += 64) { out[taken + i - tail] = i; }
-            for (int i = taken + own - tail + 1 + lane; i < S; i += 64) { out[i] = -1; }
-        }
+        if (part == 0) { ends(out, own, heads, tail, taken, lane, 64); }
     }
 }
 

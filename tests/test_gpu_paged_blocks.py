@@ -155,6 +155,22 @@ def test_selection_of_many_blocks(gpu, tokens, rows):
     _select(c, 32, (1, 2, 61), seed=rows)
 
 
+@pytest.mark.parametrize("blocks", [3, 40, 65, 129, 193, 256, 300, 321, 385, 512, 520, 769, 1020, 1027, 1030, 1300, 2000])
+@pytest.mark.parametrize("pick", [(1, 2, 29), (0, 1, 400)])
+def test_selection_of_a_tile_of_sixteen(gpu, blocks, pick):
+    """As many candidates as the forms of the choice take, with scores all over, a few values, and one value but for a few."""
+    def some(c, codes, scales):
+        scales[:] = 1.0
+        codes[:] = 0
+        codes[..., 5] = np.random.default_rng(4).integers(-2, 3, codes.shape[:-1])
+
+    def one(c, codes, scales):
+        scales[:] = np.where(np.random.default_rng(5).random(scales.shape) < 0.02, np.float32(3.0), np.float32(1.0))
+        codes[:] = codes[0, :1, :1]
+    for edit in (None, some, one):
+        _select(_long(18, 32 * blocks + 7, 1 << 12), 32, pick, seed=blocks, edit=edit)
+
+
 def _long(tokens, rows, page):
     """A sequence of many rows of which only the pages matter."""
     c = PagedCase([(tokens, 10)], Hq=4, Hkv=1, page=page, seed=tokens)
