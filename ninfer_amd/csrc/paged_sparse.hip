@@ -626,7 +626,7 @@ __global__ __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2,
                         const int v = v0 + cw * WK + wk;
                         if (v >= chunks || !takes(v)) { continue; }
                         const int tile = __builtin_amdgcn_readfirstlane(chunk_key(v)) >> 5;
-                        if (32 * tile > r.hi || ((32 * tile + 16) >> x.c.page_shift) >= x.c.max_pages) { continue; }
+                        if (32 * tile > r.hi) { continue; }
                         const Halves hv = halves_of(x, table, tile, p1);
                         Probs<NT> pr;
                         {

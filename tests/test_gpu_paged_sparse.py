@@ -305,6 +305,21 @@ def test_sizes_far_apart(gpu, kv, shape):
     Sparse(c, lists(c, 8, 32, fill=0.8), 32).call().check(tokens={0, 1, tokens // 2, tokens - 1})
 
 
+@pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_a_table_that_ends_inside_a_tile(gpu, kv, shape):
+    """An odd number of pages of 16 rows, the last of them with values far larger than the others'."""
+    tokens, Hq, Hkv, D = SHAPES[shape]
+    h = 96 + (-(tokens - 1) % 32 + 9) % 32  # the last row is the tenth of a tile
+
+    def edit(c):
+        rows = slice(h + tokens - 10, h + tokens)
+        c.v[0][rows] = bf16_bits(bf16_values(c.v[0][rows]) * np.float32(1e4))
+    c = PagedCase([(tokens, h)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, page=16, seed=20, edit=edit)
+    assert c.max_pages % 2 == 1
+    Sparse(c, lists(c, (h + tokens - 1) // 32 + 1, 32), 32).call().check(tokens={0, tokens // 2, tokens - 2, tokens - 1})
+
+
 @pytest.mark.parametrize("block", [32, 128, 256, 512])
 @pytest.mark.parametrize("S", [3, 150])
 def test_prompts_of_many_blocks(gpu, block, S):
