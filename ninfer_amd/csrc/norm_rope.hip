@@ -199,7 +199,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs x) {
             }
             ss = head_sum<D>(ss);
             float r = __builtin_amdgcn_rsqf(fmaf(ss, 1.0f / D, a.eps));
-            if (__builtin_expect(__any(ss > 0x1p120f), 0)) { // beyond FP32's squares: 2^-70 of the values, eps is nothing next to them
+            const bool huge = __any(ss > 0x1p120f);
+            if (__builtin_expect(huge, 0)) { // beyond FP32's squares: 2^-70 of the values, eps is nothing next to them
                 float s2 = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) { s2 = fmaf(v[e] * 0x1p-70f, v[e] * 0x1p-70f, s2); }
@@ -230,6 +231,11 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs x) {
                 apply(q);
             } else {
                 apply(k);
+            }
+            if (__builtin_expect(huge && a.interleaved, 0)) { // an infinite value stays out of the dims next to it that do not turn with it
+                const Turn& t = run.kind == 0 ? q : k;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) { out[w] = rotated ? out[w] : bf16_pair(v[2 * w] * t.own[2 * w], v[2 * w + 1] * t.own[2 * w + 1]); }
             }
         }
         if (run.kind == 0) {

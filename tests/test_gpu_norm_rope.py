@@ -118,6 +118,18 @@ def test_infinite_and_nan_values_stay_in_their_head(gpu, value):
         assert (row[~np.isnan(row)] == 0).all()
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("half", [0, 16])
+def test_an_infinite_value_outside_the_rotated_part(gpu, half, interleaved):
+    def edit(c):
+        c.q[1, 2, 41] = 0x7F80
+    c = RopeCase(2, 5, 2, 128, half, [5, 6], interleaved=interleaved, edit=edit, seed=3)
+    c.call()
+    synchronize()
+    row = bf16_values(c.outs[0].numpy(np.uint16).reshape(c.q.shape))[1, 2]
+    assert np.isnan(row[41]) and (np.delete(row, 41) == 0).all()
+
+
 def test_in_place(gpu):
     c, d = RopeCase(40, 8, 2, 128, 64, np.arange(40), seed=4), RopeCase(40, 8, 2, 128, 64, np.arange(40), seed=4)
     c.call()
