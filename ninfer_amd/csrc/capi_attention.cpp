@@ -355,7 +355,7 @@ const char* nmi_build_info(void) {
            "stochastic, general fixed-point), kv commit/rollback/compaction, gdn_recurrent<{16,32,64,128}> "
            "(snapshot), conv1d_silu (snapshot), device scalars, linear_q6<{4,8,16} cols> f16-MFMA (Q6G64 lm_head, "
            "fused argmax), paged KV rows (append, read back), paged_attn_few<{1,2},{128,256}> and paged_attn_many<{1,2,4},{128,256}> (INT8-G64 and BF16), "
-           "norm_rope<{128,256}> (head norms with rotation, append), block_update and block_select<{128,256}>, sparse_attn<{1,2},{128,256}>, "
+           "norm_rope<{128,256}> (head norms with rotation, append), block_update and block_select<{128,256}>, sparse_attn<{1,2},{128,256}> and sparse_many<{1,2,4},{128,256}>, "
            "paged pages (copy, reserve, release, fork, compact)";
 }
 

@@ -77,7 +77,9 @@ __device__ __forceinline__ Found find_unit(int B, int u, int lane, S span, F uni
         const uint64_t past = __ballot(end > u);
         if (past != 0u) {
             const int l = __ffsll(static_cast<long long>(past)) - 1;
-            return Found{base + l, u - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(n, l)),
+            const int count = __builtin_amdgcn_readlane(n, l), at = u - (__builtin_amdgcn_readlane(end, l) - count);
+            if (at < 0 || at >= count) { break; } // (starts that descend may promise more units than whole numbers count)
+            return Found{base + l, at,
                          Span{__builtin_amdgcn_readlane(s.start, l), __builtin_amdgcn_readlane(s.tokens, l), __builtin_amdgcn_readlane(s.history, l)}};
         }
         sum = __builtin_amdgcn_readlane(end, 63);
