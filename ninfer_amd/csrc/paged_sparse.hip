@@ -237,8 +237,9 @@ __device__ __forceinline__ void walk_rows(const SparseArgs& y, const Item& it, c
 
 // WAVES: four waves, a token and KV head each; otherwise four waves share one, and `parts` workgroups may.
 // What bounds it: HBM for many rows (32 tokens over 64 blocks of 64 rows at 40/8/128 INT8, 277 MB, 59 us with the merge, 4.7 TB/s);
-// for one token the chain list -> page -> rows, twice two waits for them, and the merge's launch (over 32 blocks 13.3 us, 10.6 and 3.8
-// in the kernels). At least two tiles of 32 keys a wave: with one 13.1 us and twice the parts, with four 15.5.
+// for one token the chain list -> page -> rows, a tile's products in one wave (1.1 us, at head_dim 256 up to 3) and the merge's launch: over
+// 32 blocks 13.1 us, with two tiles a wave 13.4, with four 15.5; at 24/4/256 17.0, 18.4 and 24.6. Tiles two ahead instead of one: 1 to 8%
+// more.
 template <int D, bool BF, int NT, bool WAVES>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : 1, D == 128 ? 2 : 1))) void sparse_attn_kernel(SparseArgs y) {
     const PagedAttnArgs& x = y.x;
@@ -740,8 +741,8 @@ SparsePlan plan_sparse(int32_t Hq, int32_t Hkv, int32_t D, bool bf16, int64_t to
     const int64_t slots = kCus * (D == 128 ? 2 : 1); // workgroups of four waves at a time
     p.waves = p.items >= 4 * slots || tiles < 4;
     if (!p.waves) {
-        // at least two tiles for a wave
-        p.parts = static_cast<int32_t>(std::max<int64_t>(1, std::min(slots / p.items, tiles / 8)));
+        // a tile for a wave, if that takes no more workgroups than run at a time
+        p.parts = static_cast<int32_t>(std::max<int64_t>(1, std::min(slots / p.items, tiles / 4)));
     }
     if (p.parts > 1) {
         const size_t rows = static_cast<size_t>(p.items) * 16 * p.nt * p.parts;
