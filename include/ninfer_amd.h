@@ -371,7 +371,8 @@ int nmi_paged_kv_copy_pages(const nmi_paged_kv_layer_view* cache, const nmi_page
 
 /* Pages for the new rows history[b] .. of the packed tokens: every absent entry of theirs gets a free page, the lowest first, in
  * the order of the sequences and their entries. granted I32 [B]: the sequence's new tokens whose rows all have a page now (all of them
- * unless the pool or the table ends). */
+ * unless the pool or the table ends). An entry that holds a page keeps it, also one that other entries share: new rows must not
+ * lie in such a page (a sequence that goes back into rows it shares is forked from one that stays). */
 int nmi_paged_pages_reserve(nmi_tensor* page_table, nmi_tensor* refs, const nmi_tensor* starts, const nmi_tensor* history,
                             int32_t page_size, nmi_tensor* granted, nmi_stream_t stream);
 
