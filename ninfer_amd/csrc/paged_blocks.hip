@@ -1,6 +1,6 @@
 // Blocks of keys of a paged KV cache on gfx950: a mean for each, and the blocks that a token's queries score highest.
 //
-// Mathematics: a block's rows are summed in 64 bits (sums of stored values, exact unless they span more than 2^53), step = max
+// Mathematics: a block's rows are summed in 64 bits (sums of stored values, exact unless they span more than 2^49), step = max
 // |sum| * FP64(1 / 127), code = rne(sum * (1 / step)), scale = FP32(step / rows): code * scale is the mean with 8 bits. A token's query for a
 // KV head is the sum of its group's heads, made codes the same way; a block's score is scale * <codes, codes>, the product of
 // whole numbers exact on the matrix cores (up to 2^22), so it does not depend on any order, and which blocks are
@@ -49,8 +49,8 @@ __device__ __forceinline__ i2 codes_of(const double (&x)[8], double amax, double
 // ---- means ---------------------------------------------------------------------------------------
 //
 // A wave per touched block and head: D / 8 lanes a row, eight values a lane, so 512 values (four or two rows) at a time.
-// What bounds it: latency and launch. 27,090 rows of 8 x 128 INT8 in blocks of 64 (30.9 MB) take 15.0 us, 10.8 in the kernel; with 4 or
-// 16 rows' loads on their way instead of 8, one wave a workgroup, or two waves a block the same, with four waves a block 18.2.
+// What bounds it: latency and launch. 27,090 rows of 8 x 128 INT8 in blocks of 64 (30.9 MB) take 14.9 us (with
+// codes made FP32, times the scale, made FP64 and added 15.8); with 4 or 16 rows' loads on their way instead of 8, one wave a workgroup, or two waves a block the same, with four waves a block 18.2.
 
 struct UpdateArgs {
     int64_t tokens;
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void block_update_kernel(UpdateArgs x) {
     constexpr int GROUPS = 64 / L;
     const char* k = x.c.k + page * x.c.k_page + first * (BF ? 2 * D : D) + li * (BF ? 16 : 8);
     const char* ks = x.c.ks + page * x.c.ks_page + first * (D / 32) + (li >> 3) * 2;
-    double sum[8] = {};
+    double sum[8] = {}, scales = 0.0;
 #pragma unroll 8
     for (int r = group; r < rows; r += GROUPS) {
         if constexpr (BF) {
@@ -98,12 +98,20 @@ __global__ __launch_bounds__(256) void block_update_kernel(UpdateArgs x) {
             }
         } else {
             const i2 raw = *reinterpret_cast<const i2*>(k + r * D);
-            const float s = f16_bits_to_f32(*reinterpret_cast<const uint16_t*>(ks + r * (D / 32)));
+            const double s = f16_bits_to_f32(*reinterpret_cast<const uint16_t*>(ks + r * (D / 32)));
+            scales += s;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                sum[e] += static_cast<float>(static_cast<int8_t>(static_cast<uint32_t>(raw[e >> 2]) >> (8 * (e & 3)))) * s;
+                // the byte code + 128 in the high word of 4096: 4224 + code without a conversion
+                const uint32_t high = __builtin_amdgcn_perm(0x40b00000u, static_cast<uint32_t>(raw[e >> 2]) ^ 0x80808080u,
+                                                            0x0706000cu | static_cast<uint32_t>(e & 3) << 8);
+                sum[e] = fma(__hiloint2double(static_cast<int>(high), 0), s, sum[e]);
             }
         }
+    }
+    if constexpr (!BF) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { sum[e] = fma(-4224.0, scales, sum[e]); }
     }
 #pragma unroll
     for (int d = L; d < 64; d *= 2) {
