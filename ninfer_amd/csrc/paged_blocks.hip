@@ -1,8 +1,8 @@
 // Blocks of keys of a paged KV cache on gfx950: a mean for each, and the blocks that a token's queries score highest.
 //
-// Mathematics: a block's rows are summed in 64 bits (sums of stored values, exact unless they span more than 2^49), step = max
-// |sum| * FP64(1 / 127), code = rne(sum * (1 / step)), scale = FP32(step / rows): code * scale is the mean with 8 bits. A token's query for a
-// KV head is the sum of its group's heads, made codes the same way; a block's score is scale * <codes, codes>, the product of
+// Mathematics: a block's rows are summed in 64 bits (sums of stored values, for 128 rows exact while INT8 scales lie within 2^22 of each
+// other and BF16 values within 2^38), step = max |sum| * FP64(1 / 127), code = rne(sum * (1 / step)), scale = FP32(step / rows): code *
+// scale is the mean with 8 bits. A token's query for a KV head is the sum of its group's heads, made codes the same way; a block's score is scale * <codes, codes>, the product of
 // whole numbers exact on the matrix cores (up to 2^22), so it does not depend on any order, and which blocks are
 // selected is defined to the bit. A token always takes the first blocks and the last ones up to its own; of those
 // between it takes the `top` highest scores, the lower index of equals. A block with an infinite or NaN key has an infinite scale
@@ -50,7 +50,8 @@ __device__ __forceinline__ i2 codes_of(const double (&x)[8], double amax, double
 //
 // A wave per touched block and head: D / 8 lanes a row, eight values a lane, so 512 values (four or two rows) at a time.
 // What bounds it: latency and launch. 27,090 rows of 8 x 128 INT8 in blocks of 64 (30.9 MB) take 14.9 us (with
-// codes made FP32, times the scale, made FP64 and added 15.8); with 4 or 16 rows' loads on their way instead of 8, one wave a workgroup, or two waves a block the same, with four waves a block 18.2.
+// codes made FP32, times the scale, made FP64 and added 15.8); with 4 or 16 rows' loads on their way instead of 8, one wave a
+// workgroup, or two waves a block the same, with four waves a block 18.2.
 
 struct UpdateArgs {
     int64_t tokens;
