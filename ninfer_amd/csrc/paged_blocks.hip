@@ -132,8 +132,8 @@ __global__ __launch_bounds__(256) void block_update_kernel(UpdateArgs x) {
 // A workgroup per (tile of up to 16 tokens of a sequence, KV head): the tile's query codes, then 16 blocks at a time as
 // 16x16x64 products of whole numbers (rows: tokens, columns: blocks), the scores to LDS as ordered keys; then the keys of a
 // token, in registers, are counted against a middle that closes in on the `top`-th largest, and the list is written in order.
-// What bounds it: for single tokens the means' reads (9 of 23 us at 4.6 TB/s for 32 tokens over up to 2,001 blocks), the choice (6 us,
-// a barrier at each step) and launch; for prompts the choice's VALU (14 of 37 us for 4,096 tokens over 320 blocks, the VALU busy 89%).
+// What bounds it: for single tokens the means' reads (9 of 23 us at 4.6 TB/s for 32 tokens over up to 2,001 blocks), the choice (6 us
+// of reductions and barriers) and launch; for prompts the choice's VALU (14 of 37 us for 4,096 tokens over 320 blocks, the VALU busy 89%).
 
 struct SelectArgs {
     BlockSelect a;
@@ -160,12 +160,20 @@ __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key ^ ((key & 0x80000000u) != 0u ? 0x80000000u : 0xffffffffu));
 }
 
+// Where the `under` largest of over + under values end if they are spread as normal ones with this sum and these squares'. (log2(x) 0.407
+// is close to the normal quantile of 1 / (1 + x).)
+__device__ __forceinline__ float normal_end(float sum, float squares, float over, float under) {
+    const float inv = __builtin_amdgcn_rcpf(over + under), mean = sum * inv;
+    const float deviation = __builtin_amdgcn_sqrtf(fmaxf(0.0f, fmaf(squares, inv, -mean * mean)));
+    return fmaf(__builtin_amdgcn_logf(over * __builtin_amdgcn_rcpf(under)) * 0.407f, deviation, mean);
+}
+
 // The `want` largest of `there` keys from lo to hi (zeros are none); `count_from` says how many there are from a key on. The interval of the
 // smallest chosen key closes in from both sides until as many keys as are wanted lie at its middle or above, or one value is
-// left: first where the counts at its ends put the middle among the scores' values (six to nine steps for scores spread as
-// sums are; halving takes 14), then, for scores that are not, at the keys' own middle.
+// left: at `guess`, then where the counts at its ends put the middle among the scores' values (four to five steps for scores spread
+// as sums are, without a guess six to nine; halving takes 14), then, for scores that are not, at the keys' own middle.
 template <typename F>
-__device__ __forceinline__ Threshold top_keys(F count_from, int there, int want, uint32_t lo, uint32_t hi) {
+__device__ __forceinline__ Threshold top_keys(F count_from, int there, int want, uint32_t lo, uint32_t hi, float guess) {
     float over = static_cast<float>(there - want), under = static_cast<float>(want); // keys from lo on that are too many, above hi too few
     int side = 0;
 #pragma unroll 1
@@ -174,7 +182,7 @@ __device__ __forceinline__ Threshold top_keys(F count_from, int there, int want,
         if (step < 12) {
             const float a = value_of(lo), b = value_of(hi);
             const float share = fminf(0.984375f, fmaxf(0.015625f, over * __builtin_amdgcn_rcpf(over + under)));
-            const float v = a + (b - a) * share;
+            const float v = step == 0 && guess > a && guess < b ? guess : a + (b - a) * share;
             if (v > a && v < b) { mid = __builtin_amdgcn_readfirstlane(max(lo + 1u, min(hi, ordered(v)))); } // (not for infinite ends)
         }
         const int n = count_from(mid);
@@ -214,6 +222,7 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 struct Shared {
     int count[2][8]; // by turns: a wave may be a step ahead
     uint32_t least[8], most[8];
+    float sum[8], squares[8];
     int taken[8], equal[8];
 };
 
@@ -222,6 +231,7 @@ template <int R, int WAVES>
 __device__ __forceinline__ int choose(const uint32_t* of, int count, int want, int first, int32_t* out, int lane, int wave, Shared& sh) {
     uint32_t k[R];
     uint32_t most = 0u, least = 0u; // least as its complement
+    float sum = 0.0f, squares = 0.0f;
     int there = 0;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -230,6 +240,9 @@ __device__ __forceinline__ int choose(const uint32_t* of, int count, int want, i
         there += static_cast<int>(__popcll(__ballot(k[i] != 0u)));
         most = max(most, k[i]);
         least = max(least, k[i] != 0u ? ~k[i] : 0u);
+        const float v = k[i] != 0u ? value_of(k[i]) : 0.0f;
+        sum += v;
+        squares = fmaf(v, v, squares);
     }
     int turn = 0;
     const auto total = [&](int n) {
@@ -247,18 +260,25 @@ __device__ __forceinline__ int choose(const uint32_t* of, int count, int want, i
     };
     most = wave_max_u32(most);
     least = wave_max_u32(least);
+    sum = wave_sum(sum);
+    squares = wave_sum(squares);
     if constexpr (WAVES > 1) {
         if (lane == 0) {
             sh.most[wave] = most;
             sh.least[wave] = least;
+            sh.sum[wave] = sum;
+            sh.squares[wave] = squares;
         }
     }
     there = total(there);
-    if constexpr (WAVES > 1) {
+    if constexpr (WAVES > 1) { // every wave the same sums in the same order: they have to go the same ways
+        sum = squares = 0.0f;
 #pragma unroll
         for (int i = 0; i < WAVES; ++i) {
             most = max(most, sh.most[i]);
             least = max(least, sh.least[i]);
+            sum += sh.sum[i];
+            squares += sh.squares[i];
         }
     }
     Threshold y{0u, 0};
@@ -270,7 +290,8 @@ __device__ __forceinline__ int choose(const uint32_t* of, int count, int want, i
                 for (int i = 0; i < R; ++i) { n += static_cast<int>(__popcll(__ballot(k[i] >= from))); }
                 return total(n);
             },
-            there, want, __builtin_amdgcn_readfirstlane(~least), __builtin_amdgcn_readfirstlane(most));
+            there, want, __builtin_amdgcn_readfirstlane(~least), __builtin_amdgcn_readfirstlane(most),
+            normal_end(sum, squares, static_cast<float>(there - want), static_cast<float>(want)));
     }
     // what the waves before take, of both kinds
     int taken = 0, equal = 0;
@@ -446,7 +467,7 @@ __device__ __forceinline__ int choose_rows(const uint32_t* of, int count, int mo
 }
 
 // NW: 4 for tiles of 16 tokens (a wave chooses for four of them, or for one, of at most 2,048 keys), 8 for smaller ones (all waves for
-// one). 32 single tokens over up to 2,001 blocks: 23.2 us; with 16 waves 27.4 (barriers), with one wave choosing 39.7; 4,096 tokens
+// one). 32 single tokens over up to 2,001 blocks: 22.8 us, without the guess 23.2; with 16 waves 27.4 (barriers), with one wave choosing 39.7; 4,096 tokens
 // over up to 320 blocks 37.5 us.
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW) void block_select_kernel(SelectArgs x) {
