@@ -327,7 +327,7 @@ __global__ __launch_bounds__(256) void sparse_merge_kernel(SparseArgs y, int row
 // FP16 operands and the apart walk of tiles beyond them stand there). A wave skips the chunks that none of its tokens takes,
 // and a row whose token does not take a chunk sees none of it.
 // What bounds it: the waves of a workgroup wait for each other at every tile, whichever of them have work there (the matrix cores are
-// busy 14% of the time, the VALU 36%, LDS 23%). 2,048 tokens over 16 blocks of 64 rows each at 24/4/256 BF16: 310 us; every token by
+// busy 14% of the time, the VALU 36%, LDS 23%). 2,048 tokens over 16 blocks of 64 rows each at 24/4/256 BF16: 310 to 334 us; every token by
 // itself 816.
 
 constexpr int kListMost = 2048;               // blocks of a workgroup's list

@@ -76,6 +76,21 @@ def test_means_of_any_value(gpu):
     _update(PagedCase([(400, 0)], Hq=4, Hkv=2, kv="bf16", page=64, seed=2, edit=edit), 64)
 
 
+@pytest.mark.parametrize("geo", ["40-8-128", "24-4-256"])
+def test_means_of_rows_of_any_scale(gpu, geo):
+    """INT8 rows 2^20 apart in one block, rows of zeros, and one whose scale is infinite."""
+    Hq, Hkv, D = GEO[geo]
+
+    def edit(c):
+        r = np.random.default_rng(3)
+        rows = bf16_values(c.k[0]) * np.float32(2.0) ** r.integers(-10, 9, (len(c.k[0]), 1, 1)).astype(np.float32)
+        rows[40:70] = 0
+        rows[300, 1, 7] = 3e38
+        c.k[0] = bf16_bits(rows)
+    with np.errstate(over="ignore", invalid="ignore"):
+        _update(PagedCase([(700, 0)], Hq=Hq, Hkv=Hkv, D=D, kv="i8", page=128, seed=3, edit=edit), 128)
+
+
 @pytest.mark.parametrize("batch", [65, 1024])
 def test_means_of_many_sequences(gpu, batch):
     r = np.random.default_rng(batch)
