@@ -63,7 +63,7 @@ def listed():
         # 48 answers to four prompts: shared pages, a page of its own for each answer's unfinished one
         _case(name="fork_answers", kind="fork", cache="bf16", batch=64, forks=48, tokens=700, tokens_min=300, pages=4096),
         # half of the conversations end, the gaps close, the next prompts come in
-        _case(name="turnover", kind="turnover", cache="bf16", page=32, batch=64, tokens=2000, tokens_min=300, pages=6000),
+        _case(name="turnover", kind="turnover", cache="bf16", page=32, batch=64, tokens=2000, tokens_min=300, pages=6144),
     ]
 
 
