@@ -180,8 +180,9 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs x) {
         }
         q.own[e] *= c;
         k.own[e] *= c;
-        q.other[e] *= s;
-        k.other[e] *= s;
+        // (an infinite weight times zero would be no number)
+        q.other[e] = rotated ? q.other[e] * s : 0.0f;
+        k.other[e] = rotated ? k.other[e] * s : 0.0f;
     }
 
     while (at < runs) {

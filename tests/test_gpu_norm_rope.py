@@ -130,6 +130,38 @@ def test_an_infinite_value_outside_the_rotated_part(gpu, half, interleaved):
     assert np.isnan(row[41]) and (np.delete(row, 41) == 0).all()
 
 
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("half", [0, 16])
+def test_a_weight_without_a_number_outside_the_rotated_part(gpu, half, interleaved, kind, value):
+    """It is the factor of its own dim alone: an infinite one gives an infinity, and every other dim keeps its bits."""
+    c, d = (RopeCase(2, 5, 2, 128, half, [5, 6], weight=kind, interleaved=interleaved, seed=3) for _ in range(2))
+    for i, w in enumerate(c.weights):
+        w[41] = value
+        c.d_weights[i] = DeviceArray.from_numpy(na.FP32, w) if kind == "fp32" else DeviceArray.from_numpy(na.BF16, bf16_bits(w))
+    c.call()
+    d.call()
+    synchronize()
+    for x, o, p in zip((c.q, c.k), c.outs, d.outs):
+        got, ref = (y.numpy(np.uint16).reshape(x.shape) for y in (o, p))
+        assert (np.delete(got, 41, -1) == np.delete(ref, 41, -1)).all()
+        want = np.copysign(np.float32(1), bf16_values(x[..., 41])) * np.float32(value)
+        assert np.array_equal(bf16_values(got[..., 41]), want, equal_nan=True)
+    # on the way into a cache: the same bits
+    p = PagedCase([(2, 5)], Hq=5, Hkv=2, kv="bf16", page=16, seed=3)
+    one, two = p.upload(p.planes(new_rows=False)), p.upload(p.planes(new_rows=False))
+    two.k = c.outs[1]
+    two.append()
+    q_out = Strided(na.BF16, (128, 5, 2), 64)
+    qw, kw, _, freq, norm = c.args()
+    ops.paged_qk_norm_rope_append(c.d_q.t, c.d_k.t, one.v.t, qw, kw, one.starts.tensor(), one.history.tensor(), freq, norm, one.view, q_out.t)
+    synchronize()
+    for a, b in zip(one.pool(), two.pool()):
+        assert (a == b).all()
+    assert (q_out.numpy(np.uint16) == c.outs[0].numpy(np.uint16)).all()
+
+
 def test_in_place(gpu):
     c, d = RopeCase(40, 8, 2, 128, 64, np.arange(40), seed=4), RopeCase(40, 8, 2, 128, 64, np.arange(40), seed=4)
     c.call()
