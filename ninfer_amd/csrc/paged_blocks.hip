@@ -1,7 +1,8 @@
 // Blocks of keys of a paged KV cache on gfx950: a mean for each, and the blocks that a token's queries score highest.
 //
-// Mathematics: a block's rows are summed in 64 bits (sums of stored values, for 128 rows exact while INT8 scales lie within 2^22 of each
-// other and BF16 values within 2^38), step = max |sum| * FP64(1 / 127), code = rne(sum * (1 / step)), scale = FP32(step / rows): code *
+// Mathematics: a block's rows are summed in 64 bits (sums of stored values, exact while INT8 scales lie within 2^29 / rows of each other:
+// a lane adds at most rows / 2 products, each below 2^12.1 times the largest scale and a multiple of 2^-11 of the smallest; BF16 values
+// within 2^45 / rows), step = max |sum| * FP64(1 / 127), code = rne(sum * (1 / step)), scale = FP32(step / rows): code *
 // scale is the mean with 8 bits. A token's query for a KV head is the sum of its group's heads, made codes the same way; a block's score is scale * <codes, codes>, the product of
 // whole numbers exact on the matrix cores (up to 2^22), so it does not depend on any order, and which blocks are
 // selected is defined to the bit. A token always takes the first blocks and the last ones up to its own; of those

@@ -91,6 +91,25 @@ def test_means_of_rows_of_any_scale(gpu, geo):
         _update(PagedCase([(700, 0)], Hq=Hq, Hkv=Hkv, D=D, kv="i8", page=128, seed=3, edit=edit), 128)
 
 
+@pytest.mark.parametrize("kv", ["i8", "bf16"])
+@pytest.mark.parametrize("geo", ["40-8-128", "24-4-256"])
+@pytest.mark.parametrize("page,block,spread", [(512, 256, 9), (1024, 1024, 8), (4096, 4096, 7)])
+def test_means_of_large_blocks(gpu, kv, geo, page, block, spread):
+    """Up to the largest block, whole and partly filled, rows of sizes far apart. INT8: a lane adds at most rows / 2 products
+    (code + 4224) * scale, each below 2^12.1 times the largest scale and a multiple of 2^-11 of the smallest: in 53 bits while scales lie
+    within 2^30 / rows. BF16: `rows` values of 8 bits, in 53 bits while those that are not zero lie within 2^45 / rows. Here the rows'
+    sizes lie within 2^(2 spread - 1), their scales within 2^4 more and their values, none below 2^-10, within 2^15 more."""
+    Hq, Hkv, D = GEO[geo]
+
+    def edit(c):
+        r = np.random.default_rng(block)
+        for k in c.k:
+            x = bf16_values(k)
+            k[:] = bf16_bits(np.where(np.abs(x) < 2.0**-10, 0, x) * np.float32(2.0) ** r.integers(-spread, spread, (len(k), 1, 1)).astype(np.float32))
+        c.k[0][block // 2:block // 2 + 30] = 0
+    _update(PagedCase([(2 * block + 100, 0), (3, block - 2), (1, 0)], Hq=Hq, Hkv=Hkv, D=D, kv=kv, page=page, seed=block, edit=edit), block, pad=16)
+
+
 @pytest.mark.parametrize("batch", [65, 1024])
 def test_means_of_many_sequences(gpu, batch):
     r = np.random.default_rng(batch)
