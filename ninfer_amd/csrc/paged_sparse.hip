@@ -91,7 +91,9 @@ __device__ __forceinline__ Listed list_of(const SparseArgs& y, const Item& it, i
     return l;
 }
 
-// Which entries repeat an earlier one. An ascending list has none; in any other every entry is compared with those before it.
+// Which entries repeat an earlier one. An ascending list has none; in any other every entry is compared with those before it, by every
+// wave that walks the list: one token at 40/8/128 INT8 over 64, 256 and 1,024 blocks of 64 rows 15.5, 25.2 and 44.9 us with ascending
+// lists, 19.4, 63.6 and 585 with shuffled ones.
 static_assert(kPagedMaxSelected <= 64 * 32);
 __device__ __forceinline__ void find_repeats(Listed& l, int count, int lane) {
     const int first = __shfl_up(l.entry, 1);
@@ -734,6 +736,9 @@ SparsePlan plan_sparse(int32_t Hq, int32_t Hkv, int32_t D, bool bf16, int64_t to
                        int32_t block_shift) {
     SparsePlan p;
     const int32_t G = Hq / Hkv;
+    // More than 16 query heads: two row tiles at once. One after the other reads a list's rows twice (from L2 the second time) and takes,
+    // for 32 tokens over 64 blocks, INT8 and BF16, 25.1 and 31.8 us instead of 28.4 and 34.0 at 32/1/128, 39.1 and 53.4 instead of 39.9
+    // and 76.5 at 32/1/256, 59.4 and 81.9 instead of 53.9 and 116.3 at 40/1/256: the registers of two tiles do not hold at head_dim 256.
     p.nt = G <= 16 ? 1 : 2;
     p.row_tiles = (G + 16 * p.nt - 1) / (16 * p.nt);
     p.items = tokens * Hkv * p.row_tiles;
@@ -765,8 +770,10 @@ SparsePlan plan_sparse(int32_t Hq, int32_t Hkv, int32_t D, bool bf16, int64_t to
         if (std::min<int64_t>(blocks, static_cast<int64_t>(t) * selected) > kListMost) { continue; }
         const int64_t groups = (tokens + static_cast<int64_t>(B) * (most - 1)) / most * Hkv;
         // Tokens next to each other mostly take the same blocks: reckoned as if 2 of them took 1.34 times as many as one, 16 3.2 times (where
-        // they agree less the tiles are more, up to as many as there are blocks). A round of workgroups with WK = 1, 2, 4 at 40/8/128 INT8
-        // over 16 blocks each: 190, 111 and 76 us; at 24/4/256 BF16 165 and 98.
+        // they agree less the tiles are more, up to as many as there are blocks). The host does not see the lists: 1,024 tokens at 40/8/128
+        // INT8 over 60,000 rows with lists that agree, agree in part (16 tokens 60 blocks) and do not (190) take 58, 271 and 899 us so,
+        // every token by itself 292, 302 and 396. A round of workgroups with WK = 1, 2, 4 at 40/8/128 INT8 over 16 blocks each: 190, 111
+        // and 76 us; at 24/4/256 BF16 165 and 98.
         const double merged = std::min<double>(static_cast<double>(blocks), selected * std::pow(static_cast<double>(t), 0.42));
         const double us_tile = D == 128 ? (wk == 1 ? 4.4 : wk == 2 ? 3.35 : 2.95) : (wk == 1 ? 3.05 : 2.35);
         const double us = static_cast<double>((groups + kCus - 1) / kCus) * (10.0 + merged * (1 << block_shift) / (16384 / D) * us_tile);

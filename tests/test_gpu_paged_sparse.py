@@ -162,6 +162,21 @@ def test_a_block_that_stands_twice_counts_once(gpu, kv, shape):
 
 
 @pytest.mark.parametrize("kv", CACHES)
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_the_longest_list_in_any_order(gpu, kv, tokens):
+    """1,024 entries, shuffled, a third of them repeats of others, some no block."""
+    c = PagedCase([(tokens, 40000)], Hq=8, Hkv=2, kv=kv, page=64, seed=21)
+    sel = lists(c, 1024, 32, seed=2)
+    r = np.random.default_rng(3)
+    for n in range(tokens):
+        for hh in range(c.Hkv):
+            sel[n, hh, 680:] = r.choice(sel[n, hh, :680], 344)
+            r.shuffle(sel[n, hh])
+    sel[:, :, 5::97] = -1
+    Sparse(c, sel, 32).call().check()
+
+
+@pytest.mark.parametrize("kv", CACHES)
 @pytest.mark.parametrize("shape", SHAPES)
 def test_absent_pages(gpu, kv, shape):
     gone = {(0, p) for p in (0, 3, 4, 5, 9, 20)}
