@@ -7,7 +7,7 @@
 // whole numbers exact on the matrix cores (up to 2^22), so it does not depend on any order, and which blocks are
 // selected is defined to the bit. A token always takes the first blocks and the last ones up to its own; of those
 // between it takes the `top` highest scores, the lower index of equals. A block with an infinite or NaN key has an infinite scale
-// and comes first.
+// and scores +infinity.
 #include "common.h"
 #include "device_utils.h"
 #include "paged_internal.h"
@@ -135,6 +135,10 @@ __global__ __launch_bounds__(256) void block_update_kernel(UpdateArgs x) {
 // token, in registers, are counted against a middle that closes in on the `top`-th largest, and the list is written in order.
 // What bounds it: for single tokens the means' reads (9 of 23 us at 4.6 TB/s for 32 tokens over up to 2,001 blocks), the choice (6 us
 // of reductions and barriers) and launch; for prompts the choice's VALU (14 of 37 us for 4,096 tokens over 320 blocks, the VALU busy 89%).
+// A sequence's blocks are not split over workgroups, so few tokens over many blocks leave CUs idle: one token at 40/8/128 over 2,049, 4,065
+// and 15,626 blocks 20.5, 31.3 and 93.3 us (eight workgroups); and past 2,032 blocks a tile has fewer tokens and reads the means again
+// for each: 4,096 tokens over 60,000, 131,072 and 260,096 rows in blocks of 64 121, 965 and 1,705 us. The forms of the choice share one
+// kernel, whose scalars do not fit: 380 of them spilled to lanes of vector registers with four waves, 696 with eight.
 
 struct SelectArgs {
     BlockSelect a;
@@ -672,6 +676,7 @@ void launch_block_update(int64_t tokens, const int32_t* starts, const int32_t* h
     check_launch("block_update_kernel");
 }
 
+// The scores of a tile fit the LDS, so the call needs none.
 size_t block_select_bytes(int32_t, int32_t, int64_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
 
 void launch_block_select(const BlockSelect& a, const PagedRef& c, const BlocksRef& b, void*, hipStream_t stream) {
