@@ -331,8 +331,8 @@ int nmi_paged_qk_norm_rope_append(const nmi_tensor* q, const nmi_tensor* k, cons
  * each over the block's rows up to the sequence's last one: sums in 64 bits, step = max |sum| * FP64(1 / 127) over the head,
  * code = rne(sum * (1 / step)), scale = FP32(step / rows). The sums are exact, and the codes defined to the bit, while the block's INT8
  * scales that are not zero lie within 2^29 / rows of each other (2^22 for 128 rows, 2^17 for 4,096), its BF16 values within 2^45 / rows;
- * beyond that a sum is rounded to 64 bits in the kernel's own, fixed order. A block with an infinite or NaN key gets codes 0 and an infinite
- * scale. Blocks past the page table or in absent pages are left out. */
+ * beyond that sums are rounded in the kernel's own, fixed order (INT8: off by at most rows 2^-41 times the sum of the scales). A block with
+ * an infinite or NaN key gets codes 0 and an infinite scale. Blocks past the page table or in absent pages are left out. */
 int nmi_paged_block_update(const nmi_paged_kv_layer_view* cache, const nmi_tensor* starts, const nmi_tensor* history,
                            int32_t tokens, const nmi_paged_block_view* blocks, nmi_stream_t stream);
 
